@@ -1260,6 +1260,86 @@ int oige_episode_stats_fold(const double* slots, int64_t num_slots, double* acc 
                             oige_stream_t stream);
 int64_t oige_episode_stats_fold_scratch(int64_t num_slots);
 
+/* ---- operators of a policy with a memory ---------------------------------------------------------------------------------
+ * What runs between two environment steps, and over a rollout when it is trained: the recurrent policies that the reference
+ * registers a task for (ShadowHandOpenAI_LSTM, utils/task_util.py) keep a state per env that reset_buf clears.  Here the memory
+ * is linear attention with one decay per head, and the norm around it a layer norm; both with their backward pass.
+ * Activations are fp32, fp16 or bf16; every sum, statistic and state is fp32.                                            */
+#define OIGE_F32 1
+#define OIGE_F16 2
+#define OIGE_BF16 3
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis, 1 <= width <= 16384.
+ * backward: dx, and dweight / dbias summed over the rows in a fixed order.                                                */
+typedef struct oige_layer_norm_io {
+  const void* x;       /* (rows, width), rows x_row_stride elements apart */
+  const void* weight;  /* (width,) of weight_dtype, or NULL: ones */
+  const void* bias;    /* (width,) of weight_dtype, or NULL: zeros */
+  void* y;             /* (rows, width), contiguous */
+  float* mean;         /* (rows,) written by the forward pass (or NULL there), read by the backward pass */
+  float* rstd;         /* (rows,) */
+  const void* dy;      /* backward: (rows, width), rows dy_row_stride elements apart */
+  void* dx;            /* (rows, width), contiguous, or NULL */
+  void* dweight;       /* (width,) of weight_dtype, or NULL */
+  void* dbias;         /* (width,) of weight_dtype, or NULL */
+  float* workspace;    /* backward, with dweight or dbias: oige_layer_norm_workspace_floats floats */
+  int64_t workspace_floats;
+  int64_t rows, x_row_stride, dy_row_stride;
+  int32_t width, dtype, weight_dtype; /* weight_dtype: dtype or OIGE_F32 */
+  float eps;
+} oige_layer_norm_io;
+
+int oige_layer_norm_forward(const oige_layer_norm_io* io, oige_stream_t stream);
+int64_t oige_layer_norm_workspace_floats(int64_t rows, int32_t width);
+int oige_layer_norm_backward(const oige_layer_norm_io* io, oige_stream_t stream);
+
+/* Linear attention with a decay per head over sequences of tokens:
+ *     S_t = a_t S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t,   a_t = decay[h], 0 where resets flags token t
+ * Tensors are (N, T, heads, d) with element strides for the first three axes (the last one is contiguous); heads a multiple of
+ * kv_heads; head sizes 1 .. 128.  Tokens from lengths[n] on (clamped to 0 .. T) are not part of sequence n: they are not read
+ * into anything, their rows of o and of the gradients are zero.  An infinite or NaN value reaches only the rows whose
+ * tokens see it.  States are fp32, contiguous (N, heads, key_dim, value_dim).                                             */
+typedef struct oige_decay_attention_io {
+  const void *q, *k, *v; /* (N, T, heads, key_dim), (N, T, kv_heads, key_dim), (N, T, kv_heads, value_dim) */
+  void* o;               /* (N, T, heads, value_dim) */
+  const float* decay;    /* (heads,) */
+  const float* state_in; /* or NULL: zeros */
+  float* state_out;      /* the state behind each sequence's last token, or NULL */
+  const void* resets;    /* (N, T) bool / uint8 or int64, or NULL; element strides resets_stride */
+  const void* lengths;   /* (N,) int32 or int64, or NULL: T */
+  const void* d_o;       /* backward: gradient of o */
+  const float* d_state_out; /* gradient of state_out, or NULL: zeros */
+  void *dq, *dk, *dv;
+  float* d_state_in;     /* or NULL */
+  float* workspace;      /* oige_decay_attention_workspace_floats floats, 16-byte aligned; NULL when that is 0 */
+  int64_t workspace_floats;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3], d_o_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+  int64_t resets_stride[2];
+  int64_t num_envs, num_tokens;
+  int32_t heads, kv_heads, key_dim, value_dim;
+  int32_t dtype, resets_bytes, lengths_bytes;
+  float scale;
+} oige_decay_attention_io;
+
+int64_t oige_decay_attention_workspace_floats(const oige_decay_attention_io* io, int32_t backward);
+int oige_decay_attention_forward(const oige_decay_attention_io* io, oige_stream_t stream);
+int oige_decay_attention_backward(const oige_decay_attention_io* io, oige_stream_t stream);
+
+/* The same recurrence for one token per sequence: `state` is updated in place.                                            */
+typedef struct oige_decay_attention_step_io {
+  const void *q, *k, *v; /* (N, heads, key_dim), (N, kv_heads, key_dim), (N, kv_heads, value_dim) */
+  void* o;               /* (N, heads, value_dim), contiguous */
+  float* state;          /* (N, heads, key_dim, value_dim) */
+  const float* decay;    /* (heads,) */
+  const void* resets;    /* (N,) bool / uint8 or int64 (a task's reset_buf), or NULL */
+  int64_t q_stride[2], k_stride[2], v_stride[2], resets_stride, num_envs;
+  int32_t heads, kv_heads, key_dim, value_dim, dtype, resets_bytes;
+  float scale;
+  int32_t reserved0;
+} oige_decay_attention_step_io;
+
+int oige_decay_attention_step(const oige_decay_attention_step_io* io, oige_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -354,6 +354,32 @@ class NoiseArgs(C.Structure):
         ("reserved0", _f), ("on_reset", NoiseTerm), ("on_interval", NoiseTerm)]) + [("step_ptr", _fp)]
 
 
+F32, F16, BF16 = 1, 2, 3
+ELEM_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+class LayerNormIo(C.Structure):
+    _fields_ = [(n, _fp) for n in ("x", "weight", "bias", "y", "mean", "rstd", "dy", "dx", "dweight", "dbias", "workspace")] + [
+        (n, C.c_int64) for n in ("workspace_floats", "rows", "x_row_stride", "dy_row_stride")] + [
+        (n, C.c_int32) for n in ("width", "dtype", "weight_dtype")] + [("eps", _f)]
+
+
+class DecayAttentionIo(C.Structure):
+    _fields_ = [(n, _fp) for n in ("q", "k", "v", "o", "decay", "state_in", "state_out", "resets", "lengths", "d_o", "d_state_out",
+                                   "dq", "dk", "dv", "d_state_in", "workspace")] + [("workspace_floats", C.c_int64)] + [
+        (n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride", "d_o_stride", "dq_stride", "dk_stride",
+                                     "dv_stride")] + [("resets_stride", C.c_int64 * 2)] + [
+        (n, C.c_int64) for n in ("num_envs", "num_tokens")] + [
+        (n, C.c_int32) for n in ("heads", "kv_heads", "key_dim", "value_dim", "dtype", "resets_bytes", "lengths_bytes")] + [("scale", _f)]
+
+
+class DecayAttentionStepIo(C.Structure):
+    _fields_ = [(n, _fp) for n in ("q", "k", "v", "o", "state", "decay", "resets")] + [
+        (n, C.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride")] + [(n, C.c_int64) for n in ("resets_stride", "num_envs")] + [
+        (n, C.c_int32) for n in ("heads", "kv_heads", "key_dim", "value_dim", "dtype", "resets_bytes")] + [
+        ("scale", _f), ("reserved0", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/oige_hip.h declares
 _P = C.c_void_p
 SIGNATURES = {
@@ -443,6 +469,13 @@ SIGNATURES = {
     "oige_episode_stats_fold_scratch": (C.c_int64, [C.c_int64]),
     "oige_observer_accumulate": (C.c_int, [C.POINTER(ObserverBatch), _P, _P, _P]),
     "oige_observer_means": (C.c_int, [_P, _P, _P, C.c_int32, C.c_int32, _P]),
+    "oige_layer_norm_forward": (C.c_int, [C.POINTER(LayerNormIo), _P]),
+    "oige_layer_norm_workspace_floats": (C.c_int64, [C.c_int64, C.c_int32]),
+    "oige_layer_norm_backward": (C.c_int, [C.POINTER(LayerNormIo), _P]),
+    "oige_decay_attention_workspace_floats": (C.c_int64, [C.POINTER(DecayAttentionIo), C.c_int32]),
+    "oige_decay_attention_forward": (C.c_int, [C.POINTER(DecayAttentionIo), _P]),
+    "oige_decay_attention_backward": (C.c_int, [C.POINTER(DecayAttentionIo), _P]),
+    "oige_decay_attention_step": (C.c_int, [C.POINTER(DecayAttentionStepIo), _P]),
     "oige_stream_copy": (C.c_int, [_P, _P, C.c_int64, C.c_int32, _P]),
     "oige_dr_noise_count": (C.c_int, [C.POINTER(NoiseArgs), C.c_int64, _P]),
     "oige_dr_noise_apply": (C.c_int, [C.POINTER(NoiseArgs), C.c_int64, _P]),

@@ -18,7 +18,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liboige_hip.so")
-SOURCES = ["oige_core.hip", "locomotion.hip", "cartpole.hip", "hand.hip", "anymal_terrain.hip", "dr_noise.hip", "anymal.hip", "quadcopter.hip", "ball_balance.hip", "ingenuity.hip", "crazyflie.hip", "franka_cabinet.hip", "newhand_cabinet.hip", "observer.hip"]
+SOURCES = ["oige_core.hip", "locomotion.hip", "cartpole.hip", "hand.hip", "anymal_terrain.hip", "dr_noise.hip", "anymal.hip", "quadcopter.hip", "ball_balance.hip", "ingenuity.hip", "crazyflie.hip", "franka_cabinet.hip", "newhand_cabinet.hip", "observer.hip", "layer_norm.hip", "decay_attention.hip"]
 
 
 def dependencies():

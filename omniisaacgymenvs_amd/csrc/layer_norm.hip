@@ -1,0 +1,358 @@
+// Layer norm over the last axis, forward and backward, for gfx950 (MI355X).
+//
+//   forward   m = mean(x), r = 1 / sqrt(mean((x - m)^2) + eps), y = (x - m) r w + b
+//   backward  h = (x - m) r, g = dy w:   dx = r (g - mean(g) - h mean(g h)),   dw = sum_rows dy h,   db = sum_rows dy
+//
+// Both are bound by HBM: every row is read once into registers, the mean and the variance are taken from there in two passes (the
+// variance from centred values: no cancellation), and written once.  All sums are fp32; the only rounding to fewer bits is the
+// store.  Small rows share a wave (lanes = a power of two that covers the row in K pieces per lane, reductions by shuffles); long
+// ones take a workgroup (reductions through LDS).  The weight's and the bias's gradients are kept per lane in registers over
+// all rows a workgroup walks, written as one partial row per workgroup and added up by a second launch in a fixed order
+// (no atomics: the result does not depend on scheduling).
+#include "oige_elem.hpp"
+
+namespace oige {
+
+constexpr int LN_THREADS = 256;
+constexpr int LN_MAX_THREADS = 1024;
+constexpr int LN_MAX_WIDTH = 16384;
+constexpr int LN_LDS_COLS = 2048;  // most columns of a wave row: 64 lanes x 4 pieces x 8 elements
+
+// Sum over the lanes that share a row: `lanes` (a power of two) neighbours of a wave, or the workgroup.
+template <bool BLOCK>
+__device__ __forceinline__ float row_sum(float v, int lanes, float* lds) {
+  const int top = BLOCK ? WAVE : lanes;
+  for (int off = top / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, WAVE);
+  if (BLOCK) {
+    const int w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    __syncthreads();  // the last sum's readers are done
+    if (lane_id() == 0) lds[w] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int i = 0; i < waves; ++i) v += lds[i];
+  }
+  return v;
+}
+
+template <bool BLOCK>
+__device__ __forceinline__ float2 row_sum2(float2 v, int lanes, float* lds) {
+  const int top = BLOCK ? WAVE : lanes;
+  for (int off = top / 2; off > 0; off >>= 1) {
+    v.x += __shfl_xor(v.x, off, WAVE);
+    v.y += __shfl_xor(v.y, off, WAVE);
+  }
+  if (BLOCK) {
+    const int w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    __syncthreads();
+    if (lane_id() == 0) {
+      lds[2 * w] = v.x;
+      lds[2 * w + 1] = v.y;
+    }
+    __syncthreads();
+    v = make_float2(0.f, 0.f);
+    for (int i = 0; i < waves; ++i) {
+      v.x += lds[2 * i];
+      v.y += lds[2 * i + 1];
+    }
+  }
+  return v;
+}
+
+template <typename T, int VEC, int K, bool BLOCK>
+__global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_norm_forward_kernel(const oige_layer_norm_io a, int lanes) {
+  __shared__ float lds[2 * LN_MAX_THREADS / WAVE];
+  const int l = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
+  const int rows_per_block = BLOCK ? 1 : LN_THREADS / lanes;
+  const int sub = BLOCK ? 0 : (int)threadIdx.x / lanes;
+  const int width = a.width;
+  const float inv = 1.f / (float)width;
+  float w[K][VEC], b[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int col = (k * lanes + l) * VEC + e;
+      w[k][e] = a.weight && col < width ? load_elem(a.weight, col, a.weight_dtype) : 1.f;
+      b[k][e] = a.bias && col < width ? load_elem(a.bias, col, a.weight_dtype) : 0.f;
+    }
+  for (int64_t row = (int64_t)blockIdx.x * rows_per_block + sub; row < a.rows; row += (int64_t)gridDim.x * rows_per_block) {
+    const T* xr = static_cast<const T*>(a.x) + row * a.x_row_stride;
+    float x[K][VEC];
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) load_run<T, VEC, (VEC > 1)>(x[k], xr, (k * lanes + l) * VEC, width);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s += x[k][e];
+    const float mean = row_sum<BLOCK>(s, lanes, lds) * inv;
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        x[k][e] = (k * lanes + l) * VEC + e < width ? x[k][e] - mean : 0.f;
+        q = fmaf(x[k][e], x[k][e], q);
+      }
+    const float rstd = 1.f / sqrtf(row_sum<BLOCK>(q, lanes, lds) * inv + a.eps);
+    T* yr = static_cast<T*>(a.y) + row * (int64_t)width;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float y[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y[e] = fmaf(x[k][e] * rstd, w[k][e], b[k][e]);
+      store_run<T, VEC, (VEC > 1)>(y, yr, (k * lanes + l) * VEC, width);
+    }
+    if (a.mean && l == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+  }
+}
+
+template <typename T, int VEC, int K, bool BLOCK>
+__global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_norm_backward_kernel(const oige_layer_norm_io a, int lanes) {
+  __shared__ float lds[2 * LN_MAX_THREADS / WAVE];
+  __shared__ float cols[BLOCK ? 1 : LN_THREADS / WAVE * LN_LDS_COLS];
+  const int l = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
+  const int rows_per_block = BLOCK ? 1 : LN_THREADS / lanes;
+  const int sub = BLOCK ? 0 : (int)threadIdx.x / lanes;
+  const int width = a.width;
+  const float inv = 1.f / (float)width;
+  float w[K][VEC], dw[K][VEC], db[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int col = (k * lanes + l) * VEC + e;
+      w[k][e] = a.weight && col < width ? load_elem(a.weight, col, a.weight_dtype) : 1.f;
+      dw[k][e] = db[k][e] = 0.f;
+    }
+  for (int64_t row = (int64_t)blockIdx.x * rows_per_block + sub; row < a.rows; row += (int64_t)gridDim.x * rows_per_block) {
+    const T* xr = static_cast<const T*>(a.x) + row * a.x_row_stride;
+    const T* dyr = static_cast<const T*>(a.dy) + row * a.dy_row_stride;
+    float x[K][VEC], g[K][VEC];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      load_run<T, VEC, (VEC > 1)>(x[k], xr, (k * lanes + l) * VEC, width);
+      load_run<T, VEC, (VEC > 1)>(g[k], dyr, (k * lanes + l) * VEC, width);
+    }
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        x[k][e] = (k * lanes + l) * VEC + e < width ? (x[k][e] - mean) * rstd : 0.f;
+        dw[k][e] = fmaf(g[k][e], x[k][e], dw[k][e]);
+        db[k][e] += g[k][e];
+        g[k][e] *= w[k][e];
+        s.x += g[k][e];
+        s.y = fmaf(g[k][e], x[k][e], s.y);
+      }
+    s = row_sum2<BLOCK>(s, lanes, lds);
+    const float mg = s.x * inv, mgx = s.y * inv;
+    if (a.dx) {
+      T* dxr = static_cast<T*>(a.dx) + row * (int64_t)width;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float d[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d[e] = rstd * (g[k][e] - fmaf(x[k][e], mgx, mg));
+        store_run<T, VEC, (VEC > 1)>(d, dxr, (k * lanes + l) * VEC, width);
+      }
+    }
+  }
+  if (!a.workspace) return;
+  float* part = a.workspace + (int64_t)blockIdx.x * 2 * width;
+  if (BLOCK) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int col = (k * lanes + l) * VEC + e;
+        if (col < width) {
+          part[col] = dw[k][e];
+          part[width + col] = db[k][e];
+        }
+      }
+    return;
+  }
+  const int wv = threadIdx.x >> 6;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();  // the last table's readers are done
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float v = which ? db[k][e] : dw[k][e];
+        for (int off = lanes; off < WAVE; off <<= 1) v += __shfl_xor(v, off, WAVE);  // the rows that shared this wave
+        const int col = (k * lanes + l) * VEC + e;
+        if (col < width && lane_id() < lanes) cols[wv * LN_LDS_COLS + col] = v;
+      }
+    __syncthreads();
+    for (int col = threadIdx.x; col < width; col += LN_THREADS) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < LN_THREADS / WAVE; ++i) v += cols[i * LN_LDS_COLS + col];
+      part[which * width + col] = v;
+    }
+  }
+}
+
+// dweight / dbias = the column sums of the partial rows: 32 columns x 32 row slices per workgroup, every slice's rows and then
+// the slices in a fixed order.
+constexpr int LN_FOLD = 32;
+__global__ __launch_bounds__(LN_FOLD * LN_FOLD) void layer_norm_fold_kernel(const oige_layer_norm_io a, int parts) {
+  __shared__ float lds[LN_FOLD][LN_FOLD + 1];
+  const int c = threadIdx.x % LN_FOLD, s = threadIdx.x / LN_FOLD;
+  const int64_t col = (int64_t)blockIdx.x * LN_FOLD + c, cols = 2 * (int64_t)a.width;
+  float v = 0.f;
+  if (col < cols)
+    for (int i = s; i < parts; i += LN_FOLD) v += a.workspace[i * cols + col];
+  lds[s][c] = v;
+  __syncthreads();
+  if (s == 0 && col < cols) {
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < LN_FOLD; ++i) v += lds[i][c];
+    void* out = col < a.width ? a.dweight : a.dbias;
+    if (out) store_elem(out, col < a.width ? col : col - a.width, v, a.weight_dtype);
+  }
+}
+
+// How a row is laid over lanes: `vec` elements per access (16 bytes where width, strides and pointers allow), K accesses per lane,
+// `lanes` of a wave -- or of a workgroup of 256 to 1024, where 64 lanes would need more than 4 accesses each (8 single-element ones).
+struct LnShape {
+  int lanes, k;
+  bool block;
+};
+static LnShape layer_norm_shape(int width, int vec) {
+  const int slots = (width + vec - 1) / vec;
+  const int kmax = vec > 1 ? 4 : 8;
+  LnShape s{1, 1, false};
+  if (slots <= WAVE * kmax) {
+    while (s.lanes < slots && s.lanes < WAVE) s.lanes *= 2;
+    while (s.lanes * s.k < slots) s.k *= 2;
+    return s;
+  }
+  s.block = true;
+  s.lanes = LN_THREADS;
+  while (s.lanes < LN_MAX_THREADS && s.lanes * (vec == 8 ? 2 : 4) < slots) s.lanes *= 2;  // at most 16 elements a lane while it can
+  while (s.lanes * s.k < slots) s.k *= 2;
+  return s;
+}
+
+constexpr int64_t LN_MAX_BLOCKS = 2048, LN_MAX_PARTS = 1024;  // forward: 8 workgroups per CU; backward: one partial row each
+
+static int64_t layer_norm_blocks(int64_t rows, const LnShape& s, int64_t most) {
+  const int64_t per = s.block ? 1 : LN_THREADS / s.lanes;
+  const int64_t b = (rows + per - 1) / per;
+  return b < most ? b : most;
+}
+
+template <typename T, int VEC, int K, bool BLOCK, bool BACKWARD>
+static int layer_norm_launch(const oige_layer_norm_io& io, const LnShape& s, int64_t blocks, hipStream_t stream) {
+  const dim3 grid((unsigned)blocks), threads(BLOCK ? s.lanes : LN_THREADS);
+  if (BACKWARD) hipLaunchKernelGGL((layer_norm_backward_kernel<T, VEC, K, BLOCK>), grid, threads, 0, stream, io, s.lanes);
+  else hipLaunchKernelGGL((layer_norm_forward_kernel<T, VEC, K, BLOCK>), grid, threads, 0, stream, io, s.lanes);
+  return check_launch(BACKWARD ? "layer_norm_backward_kernel" : "layer_norm_forward_kernel");
+}
+
+template <typename T, int VEC, bool BACKWARD>
+static int layer_norm_pick(const oige_layer_norm_io& io, const LnShape& s, int64_t blocks, hipStream_t stream) {
+#define LN_CASE(K, BLOCK, OFFERED) \
+  if constexpr (OFFERED) {           \
+    if (s.k == K && s.block == BLOCK) return layer_norm_launch<T, VEC, K, BLOCK, BACKWARD>(io, s, blocks, stream); \
+  }
+  LN_CASE(1, false, true)
+  LN_CASE(2, false, true)
+  LN_CASE(4, false, true)
+  LN_CASE(8, false, VEC == 1)
+  LN_CASE(1, true, true)
+  LN_CASE(2, true, true)
+  LN_CASE(4, true, VEC < 8)
+  LN_CASE(8, true, VEC == 1)
+  LN_CASE(16, true, VEC == 1)
+#undef LN_CASE
+  return fail(OIGE_EINVAL, "layer_norm: no variant for %d lanes x %d accesses", s.lanes, s.k);
+}
+
+static int layer_norm_check(const oige_layer_norm_io* io, const char* what) {
+  OIGE_REQUIRE(io != nullptr, "%s: null io", what);
+  OIGE_REQUIRE(elem_bytes(io->dtype) && elem_bytes(io->weight_dtype), "%s: dtype must be OIGE_F32, OIGE_F16 or OIGE_BF16", what);
+  OIGE_REQUIRE(io->weight_dtype == io->dtype || io->weight_dtype == OIGE_F32, "%s: weight and bias have the activations' type or fp32", what);
+  OIGE_REQUIRE(io->rows >= 0 && io->width >= 1 && io->width <= LN_MAX_WIDTH, "%s: rows %lld, width %d (1 .. %d)", what,
+               (long long)io->rows, io->width, LN_MAX_WIDTH);
+  OIGE_REQUIRE(io->rows == 0 || io->x, "%s: null x", what);
+  OIGE_REQUIRE(io->eps >= 0.f, "%s: eps must not be negative", what);
+  return OIGE_OK;
+}
+
+// 16-byte accesses: rows of whole vectors that start on a boundary, in every tensor walked row by row.
+static bool layer_norm_wide(const oige_layer_norm_io& io, bool backward) {
+  const int v = 16 / elem_bytes(io.dtype);
+  bool ok = io.width % v == 0 && io.x_row_stride % v == 0 && aligned16(io.x);
+  if (!backward) return ok && aligned16(io.y);
+  return ok && io.dy_row_stride % v == 0 && aligned16(io.dy) && aligned16(io.dx);
+}
+
+template <bool BACKWARD>
+static int layer_norm_dispatch(const oige_layer_norm_io& io, bool wide, const LnShape& s, int64_t blocks, hipStream_t stream) {
+  if (io.dtype == OIGE_F32)
+    return wide ? layer_norm_pick<float, 4, BACKWARD>(io, s, blocks, stream) : layer_norm_pick<float, 1, BACKWARD>(io, s, blocks, stream);
+  if (io.dtype == OIGE_F16)
+    return wide ? layer_norm_pick<_Float16, 8, BACKWARD>(io, s, blocks, stream) : layer_norm_pick<_Float16, 1, BACKWARD>(io, s, blocks, stream);
+  return wide ? layer_norm_pick<__bf16, 8, BACKWARD>(io, s, blocks, stream) : layer_norm_pick<__bf16, 1, BACKWARD>(io, s, blocks, stream);
+}
+
+}  // namespace oige
+
+using namespace oige;
+
+extern "C" {
+
+int oige_layer_norm_forward(const oige_layer_norm_io* io, oige_stream_t stream) {
+  const int rc = layer_norm_check(io, "layer_norm_forward");
+  if (rc) return rc;
+  if (io->rows == 0) return OIGE_OK;
+  OIGE_REQUIRE(io->y, "layer_norm_forward: null y");
+  OIGE_REQUIRE((io->mean == nullptr) == (io->rstd == nullptr), "layer_norm_forward: mean and rstd are kept together or not at all");
+  const bool wide = layer_norm_wide(*io, false);
+  const LnShape s = layer_norm_shape(io->width, wide ? 16 / elem_bytes(io->dtype) : 1);
+  return layer_norm_dispatch<false>(*io, wide, s, layer_norm_blocks(io->rows, s, LN_MAX_BLOCKS), (hipStream_t)stream);
+}
+
+int64_t oige_layer_norm_workspace_floats(int64_t rows, int32_t width) {
+  if (rows < 1 || width < 1 || width > LN_MAX_WIDTH)
+    return fail(OIGE_EINVAL, "layer_norm_workspace: rows %lld, width %d (1 .. %d)", (long long)rows, width, LN_MAX_WIDTH);
+  return (rows < LN_MAX_PARTS ? rows : LN_MAX_PARTS) * 2 * (int64_t)width;
+}
+
+int oige_layer_norm_backward(const oige_layer_norm_io* io, oige_stream_t stream) {
+  const int rc = layer_norm_check(io, "layer_norm_backward");
+  if (rc) return rc;
+  const bool params = io->dweight || io->dbias;
+  OIGE_REQUIRE(io->rows == 0 || (io->dy && io->mean && io->rstd), "layer_norm_backward: null dy, mean or rstd");
+  OIGE_REQUIRE(io->dx || params, "layer_norm_backward: no gradient asked for");
+  OIGE_REQUIRE(!params || io->rows == 0 || io->workspace, "layer_norm_backward: the weight's gradient needs a workspace");
+  OIGE_REQUIRE(!params || io->rows == 0 || io->workspace_floats >= oige_layer_norm_workspace_floats(io->rows, io->width),
+               "layer_norm_backward: workspace of %lld floats is too small", (long long)io->workspace_floats);
+  oige_layer_norm_io a = *io;
+  if (!params) a.workspace = nullptr;
+  int64_t blocks = 0;
+  if (a.rows > 0) {
+    const bool wide = layer_norm_wide(a, true);
+    const LnShape s = layer_norm_shape(a.width, wide ? 16 / elem_bytes(a.dtype) : 1);
+    blocks = layer_norm_blocks(a.rows, s, LN_MAX_PARTS);
+    const int rc2 = layer_norm_dispatch<true>(a, wide, s, blocks, (hipStream_t)stream);
+    if (rc2) return rc2;
+  }
+  if (!params) return OIGE_OK;
+  hipLaunchKernelGGL(layer_norm_fold_kernel, dim3((unsigned)((2 * (int64_t)a.width + LN_FOLD - 1) / LN_FOLD)), dim3(LN_FOLD * LN_FOLD), 0,
+                     (hipStream_t)stream, a, (int)blocks);  // no rows: zeroes
+  return check_launch("layer_norm_fold_kernel");
+}
+
+}  // extern "C"

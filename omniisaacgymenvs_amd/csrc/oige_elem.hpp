@@ -1,0 +1,59 @@
+// Element types of the recurrent-policy operators (layer_norm.hip, decay_attention.hip): fp32, fp16 and bf16 in memory, fp32 in
+// registers, vectors of up to 16 bytes.  Narrowing is the hardware's round to nearest even.
+#pragma once
+#include "oige_common.hpp"
+
+namespace oige {
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+template <typename T>
+constexpr int VEC16 = 16 / (int)sizeof(T);  // elements of a 16-byte access
+
+inline int elem_bytes(int dtype) { return dtype == OIGE_F32 ? 4 : (dtype == OIGE_F16 || dtype == OIGE_BF16 ? 2 : 0); }
+
+// One element of a buffer whose type is a launch constant (parameters of another type than the activations).
+__device__ __forceinline__ float load_elem(const void* p, int64_t i, int dtype) {
+  if (dtype == OIGE_F32) return static_cast<const float*>(p)[i];
+  if (dtype == OIGE_F16) return (float)static_cast<const _Float16*>(p)[i];
+  return (float)static_cast<const __bf16*>(p)[i];
+}
+__device__ __forceinline__ void store_elem(void* p, int64_t i, float x, int dtype) {
+  if (dtype == OIGE_F32) static_cast<float*>(p)[i] = x;
+  else if (dtype == OIGE_F16) static_cast<_Float16*>(p)[i] = (_Float16)x;
+  else static_cast<__bf16*>(p)[i] = (__bf16)x;
+}
+
+// CNT consecutive elements from `off` of a row of `limit`, as floats; elements behind the limit read as 0.  VEC: the row starts
+// on a 16-byte boundary, `off` and `limit` are multiples of the access width.  A piece behind the end re-reads the row's first
+// one (no load inside a conditional block).
+template <typename T, int CNT, bool VEC>
+__device__ __forceinline__ void load_run(float (&out)[CNT], const T* row, int off, int limit) {
+  constexpr int W = VEC ? (CNT < VEC16<T> ? CNT : VEC16<T>) : 1;
+#pragma unroll
+  for (int b = 0; b < CNT; b += W) {
+    const bool ok = off + b < limit;
+    const Pack<T, W> x = *reinterpret_cast<const Pack<T, W>*>(row + (ok ? off + b : 0));
+#pragma unroll
+    for (int e = 0; e < W; ++e) out[b + e] = ok ? (float)x.v[e] : 0.f;
+  }
+}
+
+template <typename T, int CNT, bool VEC>
+__device__ __forceinline__ void store_run(const float (&in)[CNT], T* row, int off, int limit) {
+  constexpr int W = VEC ? (CNT < VEC16<T> ? CNT : VEC16<T>) : 1;
+#pragma unroll
+  for (int b = 0; b < CNT; b += W) {
+    if (off + b < limit) {
+      Pack<T, W> x;
+#pragma unroll
+      for (int e = 0; e < W; ++e) x.v[e] = (T)in[b + e];
+      *reinterpret_cast<Pack<T, W>*>(row + off + b) = x;
+    }
+  }
+}
+
+}  // namespace oige
