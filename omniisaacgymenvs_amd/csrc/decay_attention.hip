@@ -75,31 +75,37 @@ __device__ __forceinline__ double da_power(double decay, int64_t n) {
   }
   return r;
 }
-struct DaPowers {  // decay^n for n in 0 .. 16 without a loop
-  double p1, p2, p4, p8, p16;
-  __device__ __forceinline__ explicit DaPowers(double d) : p1(d), p2(d * d), p4(p2 * p2), p8(p4 * p4), p16(p8 * p8) {}
-  __device__ __forceinline__ double operator()(int n) const {
-    double r = (n & 1) ? p1 : 1.0;
-    r *= (n & 2) ? p2 : 1.0;
-    r *= (n & 4) ? p4 : 1.0;
-    r *= (n & 8) ? p8 : 1.0;
-    return (n & 16) ? r * p16 : r;
+struct DaPowers {  // decay^n for n in 0 .. 16 without a loop, within 4 roundings
+  float p1, p2, p4, p8, p16;
+  __device__ __forceinline__ explicit DaPowers(double d) : p1((float)d), p2((float)(d * d)) {
+    const double d4 = (d * d) * (d * d);
+    p4 = (float)d4;
+    p8 = (float)(d4 * d4);
+    p16 = (float)((d4 * d4) * (d4 * d4));
+  }
+  __device__ __forceinline__ float operator()(int n) const {
+    float r = (n & 1) ? p1 : 1.f;
+    r *= (n & 2) ? p2 : 1.f;
+    r *= (n & 4) ? p4 : 1.f;
+    r *= (n & 8) ? p8 : 1.f;
+    return (n & 16) ? p16 : r;
   }
 };
 
 // This wave's piece of a state matrix in memory: tile (s, sv), register r, lane (c, g) holds dk = NK (4 g + r) + s,
 // dv = dv0 + NV c + sv.
-template <int NK, int NV, bool VEC>
+template <int NK, int NV, int MODE>
 __device__ __forceinline__ void da_load_state(f32x4 (&S)[NK][NV], const float* p, const DaCore& a, int dv0, int c, int g) {
   if (a.transposed) {
 #pragma unroll
     for (int sv = 0; sv < NV; ++sv) {
       const int d = dv0 + NV * c + sv;
       float x[4 * NK];
-      load_run<float, 4 * NK, VEC>(x, p + (int64_t)(d < a.dv ? d : 0) * a.dk, 4 * NK * g, d < a.dv ? a.dk : 0);
+      load_run<float, 4 * NK, MODE>(x, p + (int64_t)(d < a.dv ? d : 0) * a.dk, 4 * NK * g, d < a.dv ? a.dk : 0);
 #pragma unroll
       for (int s = 0; s < NK; ++s) S[s][sv] = f32x4{x[s], x[NK + s], x[2 * NK + s], x[3 * NK + s]};
     }
+    asm volatile("" ::: "memory");  // keeps the two branches' ends apart: merged, they address S's tiles, which then leave the registers
   } else {
 #pragma unroll
     for (int s = 0; s < NK; ++s) {
@@ -107,7 +113,7 @@ __device__ __forceinline__ void da_load_state(f32x4 (&S)[NK][NV], const float* p
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int d = NK * (4 * g + r) + s;
-        load_run<float, NV, VEC>(x[r], p + (int64_t)(d < a.dk ? d : 0) * a.dv, dv0 + NV * c, d < a.dk ? a.dv : 0);
+        load_run<float, NV, MODE>(x[r], p + (int64_t)(d < a.dk ? d : 0) * a.dv, dv0 + NV * c, d < a.dk ? a.dv : 0);
       }
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) S[s][sv] = f32x4{x[0][sv], x[1][sv], x[2][sv], x[3][sv]};
@@ -115,7 +121,7 @@ __device__ __forceinline__ void da_load_state(f32x4 (&S)[NK][NV], const float* p
   }
 }
 
-template <int NK, int NV, bool VEC>
+template <int NK, int NV, int MODE>
 __device__ __forceinline__ void da_store_state(const f32x4 (&S)[NK][NV], float* p, const DaCore& a, int dv0, int c, int g) {
   if (a.transposed) {
 #pragma unroll
@@ -129,7 +135,7 @@ __device__ __forceinline__ void da_store_state(const f32x4 (&S)[NK][NV], float* 
         x[2 * NK + s] = S[s][sv].z;
         x[3 * NK + s] = S[s][sv].w;
       }
-      if (d < a.dv) store_run<float, 4 * NK, VEC>(x, p + (int64_t)d * a.dk, 4 * NK * g, a.dk);
+      if (d < a.dv) store_run<float, 4 * NK, MODE>(x, p + (int64_t)d * a.dk, 4 * NK * g, a.dk);
     }
   } else {
 #pragma unroll
@@ -145,7 +151,7 @@ __device__ __forceinline__ void da_store_state(const f32x4 (&S)[NK][NV], float* 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int d = NK * (4 * g + r) + s;
-        if (d < a.dk) store_run<float, NV, VEC>(x[r], p + (int64_t)d * a.dv, dv0 + NV * c, a.dv);
+        if (d < a.dk) store_run<float, NV, MODE>(x[r], p + (int64_t)d * a.dv, dv0 + NV * c, a.dv);
       }
     }
   }
@@ -177,9 +183,34 @@ __device__ __forceinline__ void da_state_part(f32x4 (&acc)[NV], const f32x4 (&S)
 // da_settle() stands where the state's tiles leave the loop.
 __device__ __forceinline__ void da_settle() { asm volatile("s_nop 15" ::: "memory"); }
 
+// One block's rows of the operands.  Rows behind the block's L tokens re-read its last one; `low` is the earliest of its tokens
+// in memory, and in reverse the block's first token is the latest.
+struct DaBlock {
+  int64_t low;
+  int L, reverse;
+  __device__ __forceinline__ int row(int i) const {
+    const int r = i < L ? i : L - 1;
+    return reverse ? L - 1 - r : r;
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* at(const T* head, int64_t st, int i) const {  // row * stride in 32 x 32 bits: checked on the host
+    return head + low * st + (uint64_t)(uint32_t)row(i) * (uint32_t)st;
+  }
+};
+__device__ __forceinline__ DaBlock da_block(const DaCore& a, int64_t p0, int64_t end, int64_t len) {
+  DaBlock b;
+  b.L = end - p0 < DA_TOKENS ? (int)(end - p0) : DA_TOKENS;
+  b.reverse = a.reverse;
+  b.low = a.reverse ? len - p0 - b.L : p0;
+  return b;
+}
+
 // STATES: only the states at the segments' ends (no q, no o), for sequences cut over time.
-template <typename T, int NK, int NV, bool VEC, bool STATES>
-__global__ __launch_bounds__(DA_WAVES* WAVE) void decay_attention_kernel(const DaCore a) {
+//
+// The next block's rows are asked for as soon as the registers of this block's are free: q and the first copy of k behind the
+// products that read them, the other copy and v at the end, so that their way from memory runs beside the matrix instructions.
+template <typename T, int NK, int NV, int MODE, bool STATES>
+__global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(const DaCore a) {
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const int64_t u = (int64_t)blockIdx.x * DA_WAVES + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int64_t units = a.n * a.h * a.slices;
@@ -199,7 +230,33 @@ __global__ __launch_bounds__(DA_WAVES* WAVE) void decay_attention_kernel(const D
   const T* kh = static_cast<const T*>(a.k.p) + n * a.k.sn + (int64_t)(h / a.k.group) * a.k.sh;
   const T* vh = static_cast<const T*>(a.v.p) + n * a.v.sn + (int64_t)(h / a.v.group) * a.v.sh;
 
+  Run<T, 4 * NK, MODE> q_run, k1_run;
+  Run<T, NK, MODE> k2_run[4];
+  Run<T, NV, MODE> v_run[4];
+  bool flag = false;
+  auto issue_rows = [&](const DaBlock& b) {
+    if (!STATES) {
+      q_run.issue(b.at(qh, a.q.st, c), 4 * NK * g, a.dk);
+      k1_run.issue(b.at(kh, a.k.st, c), 4 * NK * g, a.dk);
+    }
+  };
+  auto issue_columns = [&](const DaBlock& b, bool not_first) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      v_run[r].issue(b.at(vh, a.v.st, 4 * g + r), dv0 + NV * c, a.dv);
+      k2_run[r].issue(b.at(kh, a.k.st, 4 * g + r), NK * c, a.dk);
+    }
+    if (a.resets) flag = (not_first || !b.reverse || c > 0) && c < b.L && da_reset(a, n, b.low + b.row(c) + b.reverse);
+  };
+
+  DaBlock blk = da_block(a, begin, end, len);
+  if (begin < end) {
+    issue_rows(blk);
+    issue_columns(blk, begin > 0);
+  }
+
   f32x4 S[NK][NV];
+  const f32x4 zero{0.f, 0.f, 0.f, 0.f};
   constexpr int UNIT = NK * NV * 4 * WAVE;  // floats of a wave's state
   float* seg_slot = a.seg_states + ((nh * a.nseg + seg) * a.slices + slice) * (int64_t)UNIT;
   if (seg > 0 && !STATES) {
@@ -208,92 +265,80 @@ __global__ __launch_bounds__(DA_WAVES* WAVE) void decay_attention_kernel(const D
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) S[s][sv] = *reinterpret_cast<const f32x4*>(seg_slot + ((s * NV + sv) * WAVE + lane) * 4);
   } else if (seg == 0 && a.s_in) {
-    da_load_state<NK, NV, VEC>(S, a.s_in + nh * a.dk * a.dv, a, dv0, c, g);
+    da_load_state<NK, NV, MODE>(S, a.s_in + nh * a.dk * a.dv, a, dv0, c, g);
   } else {
 #pragma unroll
     for (int s = 0; s < NK; ++s)
 #pragma unroll
-      for (int sv = 0; sv < NV; ++sv) S[s][sv] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int sv = 0; sv < NV; ++sv) S[s][sv] = zero;
   }
 
   const double decay = (double)a.decay[h];
   const DaPowers pw(decay);
   bool dropped = false;  // a reset inside the segment
   float head_w = 0.f, pair_w[4], tail_w[4], keep_hi = 0.f, keep_lo = 0.f;
+  const uint32_t upto = (2u << c) - 1u;  // bits 0 .. i
 
   for (int64_t p0 = begin; p0 < end; p0 += DA_TOKENS) {
-    const int L = end - p0 < DA_TOKENS ? (int)(end - p0) : DA_TOKENS;
-    const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
+    const int L = blk.L;
     if (p0 == begin || p0 == DA_TOKENS || L < DA_TOKENS) {
-      const double keep = pw(L - first);
+      const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
+      const double keep = da_power(decay, L - first);
       keep_hi = (float)keep;
       keep_lo = (float)(keep - (double)keep_hi);  // the rounding of decay^16 would pile up over a long memory
-      head_w = (float)pw(c + 1 - first);
+      head_w = pw(c + 1 - first);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = 4 * g + r;
-        pair_w[r] = j <= c ? (float)pw(c - j) * a.kv_scale : 0.f;
-        tail_w[r] = j < L ? (float)pw(L - 1 - j) * a.kv_scale : 0.f;
+        pair_w[r] = j <= c ? pw(c - j) * a.kv_scale : 0.f;
+        tail_w[r] = j < L ? pw(L - 1 - j) * a.kv_scale : 0.f;
       }
     }
-    // token rows; those behind the end re-read the last one and are cleared
-    const int64_t pc = p0 + (c < L ? c : L - 1);
-    const int64_t tc = a.reverse ? len - 1 - pc : pc;
-    float K2[4][NK], V[4][NV];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = 4 * g + r;
-      const int64_t pj = p0 + (j < L ? j : L - 1);
-      const int64_t tj = a.reverse ? len - 1 - pj : pj;
-      load_run<T, NK, VEC>(K2[r], kh + tj * a.k.st, NK * c, a.dk);
-      load_run<T, NV, VEC>(V[r], vh + tj * a.v.st, dv0 + NV * c, a.dv);
-    }
-    uint32_t m = 0;  // bit i: a reset in front of the block's token i
-    if (a.resets) {
-      bool f = false;
-      if (c < L) {
-        if (!a.reverse) f = da_reset(a, n, tc);
-        else if (pc > 0) f = da_reset(a, n, tc + 1);
-      }
-      m = (uint32_t)(__ballot(f) & 0xFFFFull);
-    }
-    const uint32_t upto = (2u << c) - 1u;  // bits 0 .. i
-    if (L < DA_TOKENS) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int sv = 0; sv < NV; ++sv) V[r][sv] = 4 * g + r < L ? V[r][sv] : 0.f;
-    }
+    const uint32_t m = (uint32_t)(__ballot(flag) & 0xFFFFull);  // bit i: a reset in front of the block's token i
+    const bool more = p0 + DA_TOKENS < end;
+    const DaBlock next = da_block(a, more ? p0 + DA_TOKENS : p0, end, len);  // behind the last block: the same rows once more
 
+    float P[4];
+    f32x4 acc[NV];
+    float Q[4 * NK];
+    const bool from_state = !(m & upto);
     if (!STATES) {
-      float Q[4 * NK], K1[4 * NK];
-      load_run<T, 4 * NK, VEC>(Q, qh + tc * a.q.st, 4 * NK * g, a.dk);
-      load_run<T, 4 * NK, VEC>(K1, kh + tc * a.k.st, 4 * NK * g, a.dk);
-      f32x4 pt{0.f, 0.f, 0.f, 0.f};
+      float K1[4 * NK];
+      q_run.take(Q, 4 * NK * g, a.dk);
+      k1_run.take(K1, 4 * NK * g, a.dk);
+      f32x4 pt = zero;
 #pragma unroll
       for (int e = 0; e < 4 * NK; ++e) pt = __builtin_amdgcn_mfma_f32_16x16x4f32(K1[e], Q[e], pt, 0, 0, 0);
-      float P[4] = {pt.x, pt.y, pt.z, pt.w};
+      const float p4[4] = {pt.x, pt.y, pt.z, pt.w};
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = 4 * g + r;
         const bool sees = j <= c && !(m & upto & ~((2u << j) - 1u));
-        P[r] = sees ? P[r] * pair_w[r] : 0.f;  // a masked product may be infinite or NaN: selected away, not multiplied
+        P[r] = sees ? p4[r] * pair_w[r] : 0.f;  // a masked product may be infinite or NaN: selected away, not multiplied
       }
-      f32x4 acc[NV];
-      const bool from_state = !(m & upto);
       da_state_part<NK, NV>(acc, S, Q, from_state, head_w);
+    }
+    float V[4][NV], K2[4][NK];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      v_run[r].take(V[r], dv0 + NV * c, a.dv);
+#pragma unroll
+      for (int sv = 0; sv < NV; ++sv) V[r][sv] = 4 * g + r < L ? V[r][sv] : 0.f;
+    }
+    if (!STATES) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int sv = 0; sv < NV; ++sv) acc[sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[r][sv], P[r], acc[sv], 0, 0, 0);
       // An infinite or NaN value in a row that some tokens must not see has met their zero weights in the product.  Such blocks
       // (any output not finite) are summed again pair by pair.
-      f32x4 z{0.f, 0.f, 0.f, 0.f};
+      f32x4 z = zero;
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) z += acc[sv] * 0.f;
       const float z1 = (z.x + z.y) + (z.z + z.w);
       if (__any(c < L && z1 != z1)) {
         da_state_part<NK, NV>(acc, S, Q, from_state, head_w);
+#pragma unroll 1
         for (int gj = 0; gj < 4; ++gj) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -308,6 +353,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE) void decay_attention_kernel(const D
           }
         }
       }
+      issue_rows(next);
       if (c < L) {
         float out[4 * NV];
 #pragma unroll
@@ -317,38 +363,34 @@ __global__ __launch_bounds__(DA_WAVES* WAVE) void decay_attention_kernel(const D
           out[2 * NV + sv] = acc[sv].z * a.out_scale;
           out[3 * NV + sv] = acc[sv].w * a.out_scale;
         }
-        const int64_t row = n * a.on + tc * a.ot + (int64_t)h * a.oh;
-        if (a.o_float) store_run<float, 4 * NV, VEC>(out, static_cast<float*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
-        else store_run<T, 4 * NV, VEC>(out, static_cast<T*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
+        const int64_t row = n * a.on + (blk.low + blk.row(c)) * a.ot + (int64_t)h * a.oh;
+        if (a.o_float) store_run<float, 4 * NV, MODE>(out, static_cast<float*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
+        else store_run<T, 4 * NV, MODE>(out, static_cast<T*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
       }
     }
 
     // the state behind the block: rows in front of its last reset, and behind the end, stay out of the sum altogether
-    if (m || L < DA_TOKENS) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool in = 4 * g + r < L && !(m & ~((2u << (4 * g + r)) - 1u));
+    for (int r = 0; r < 4; ++r) {
+      const bool in = 4 * g + r < L && !(m & ~((2u << (4 * g + r)) - 1u));
+      k2_run[r].take(K2[r], NK * c, a.dk);
 #pragma unroll
-        for (int s = 0; s < NK; ++s) K2[r][s] = in ? K2[r][s] : 0.f;
+      for (int s = 0; s < NK; ++s) K2[r][s] = in ? K2[r][s] : 0.f;
 #pragma unroll
-        for (int sv = 0; sv < NV; ++sv) V[r][sv] = in ? V[r][sv] : 0.f;
-      }
+      for (int sv = 0; sv < NV; ++sv) V[r][sv] = in ? V[r][sv] * tail_w[r] : 0.f;
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int sv = 0; sv < NV; ++sv) V[r][sv] *= tail_w[r];
     dropped |= m != 0;
+    issue_columns(next, true);
 #pragma unroll
     for (int s = 0; s < NK; ++s)
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) {
-        const f32x4 zero{0.f, 0.f, 0.f, 0.f};
         S[s][sv] = m ? zero : __builtin_elementwise_fma(S[s][sv], f32x4(keep_hi), S[s][sv] * keep_lo);
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[s][sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(K2[r][s], V[r][sv], S[s][sv], 0, 0, 0);
       }
     da_settle();
+    blk = next;
   }
 
   if (STATES) {
@@ -366,9 +408,9 @@ __global__ __launch_bounds__(DA_WAVES* WAVE) void decay_attention_kernel(const D
   const int64_t stop = begin + a.seg_len < a.t ? begin + a.seg_len : a.t;
   for (int64_t t = (begin > len ? begin : len) + c; t < stop; t += 16) {
     const int64_t row = n * a.on + t * a.ot + (int64_t)h * a.oh;
-    const float zero[4 * NV] = {};
-    if (a.o_float) store_run<float, 4 * NV, VEC>(zero, static_cast<float*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
-    else store_run<T, 4 * NV, VEC>(zero, static_cast<T*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
+    const float none[4 * NV] = {};
+    if (a.o_float) store_run<float, 4 * NV, MODE>(none, static_cast<float*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
+    else store_run<T, 4 * NV, MODE>(none, static_cast<T*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
   }
   if (a.s_out && seg == a.nseg - 1) {
     if (a.reverse && len > 0) {  // dS_0 = a_0 G_0
@@ -376,9 +418,9 @@ __global__ __launch_bounds__(DA_WAVES* WAVE) void decay_attention_kernel(const D
 #pragma unroll
       for (int s = 0; s < NK; ++s)
 #pragma unroll
-        for (int sv = 0; sv < NV; ++sv) S[s][sv] = drop ? f32x4{0.f, 0.f, 0.f, 0.f} : S[s][sv] * (float)decay;
+        for (int sv = 0; sv < NV; ++sv) S[s][sv] = drop ? zero : S[s][sv] * (float)decay;
     }
-    da_store_state<NK, NV, VEC>(S, a.s_out + nh * a.dk * a.dv, a, dv0, c, g);
+    da_store_state<NK, NV, MODE>(S, a.s_out + nh * a.dk * a.dv, a, dv0, c, g);
   }
 }
 
@@ -391,13 +433,23 @@ __global__ __launch_bounds__(256) void decay_attention_join_kernel(float* __rest
   const int64_t nh = i / per_head, e = i % per_head;
   f32x4* s = reinterpret_cast<f32x4*>(states) + nh * nseg * per_head + e;
   f32x4 carry = s[0];
-  for (int seg = 1; seg < nseg - 1; ++seg) {
-    const f32x4 end = s[seg * per_head];
-    const float f = factors[nh * nseg + seg];
-    s[seg * per_head] = carry;
-    carry = f < 0.f ? end : __builtin_elementwise_fma(carry, f32x4(f), end);
+  constexpr int U = 8;  // ends in flight (they do not depend on the carry, but lie where it goes)
+  for (int seg0 = 1; seg0 < nseg; seg0 += U) {
+    f32x4 end[U];
+    float f[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int seg = seg0 + i < nseg - 1 ? seg0 + i : nseg - 2;  // (the last segment's own end is nobody's start)
+      end[i] = s[seg * per_head];
+      f[i] = factors[nh * nseg + seg];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (seg0 + i >= nseg) break;
+      s[(seg0 + i) * per_head] = carry;
+      carry = f[i] < 0.f ? end[i] : __builtin_elementwise_fma(carry, f32x4(f[i]), end[i]);
+    }
   }
-  s[(nseg - 1) * per_head] = carry;  // the last segment's own end is nobody's start
 }
 
 // Gradients of shared key / value heads: the sum over the query heads that share one, from fp32 rows (N, T, H, d) -> T.
@@ -537,7 +589,7 @@ static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv) 
   return p;
 }
 
-template <typename T, int NK, int NV, bool VEC>
+template <typename T, int NK, int NV, int MODE>
 static int decay_attention_run(DaCore c, const DaPlan& p, float* workspace, hipStream_t stream) {
   c.slices = p.slices;
   c.nseg = p.nseg;
@@ -548,7 +600,7 @@ static int decay_attention_run(DaCore c, const DaPlan& p, float* workspace, hipS
   if (p.nseg > 1) {
     c.seg_states = workspace;
     c.seg_factors = workspace + c.n * c.h * p.nseg * per_head * 4;
-    hipLaunchKernelGGL((decay_attention_kernel<T, NK, NV, VEC, true>), dim3((unsigned)blocks, (unsigned)(p.nseg - 1)), dim3(DA_WAVES * WAVE), 0,
+    hipLaunchKernelGGL((decay_attention_kernel<T, NK, NV, MODE, true>), dim3((unsigned)blocks, (unsigned)(p.nseg - 1)), dim3(DA_WAVES * WAVE), 0,
                        stream, c);
     int rc = check_launch("decay_attention_kernel (states)");
     if (rc) return rc;
@@ -558,24 +610,24 @@ static int decay_attention_run(DaCore c, const DaPlan& p, float* workspace, hipS
     rc = check_launch("decay_attention_join_kernel");
     if (rc) return rc;
   }
-  hipLaunchKernelGGL((decay_attention_kernel<T, NK, NV, VEC, false>), dim3((unsigned)blocks, (unsigned)p.nseg), dim3(DA_WAVES * WAVE), 0, stream, c);
+  hipLaunchKernelGGL((decay_attention_kernel<T, NK, NV, MODE, false>), dim3((unsigned)blocks, (unsigned)p.nseg), dim3(DA_WAVES * WAVE), 0, stream, c);
   return check_launch("decay_attention_kernel");
 }
 
-template <typename T, bool VEC>
+template <typename T, int MODE>
 static int decay_attention_tiles(const DaCore& c, const DaPlan& p, float* ws, hipStream_t s) {
   switch (p.nk * 8 + p.nv) {
-    case 8 + 1: return decay_attention_run<T, 1, 1, VEC>(c, p, ws, s);
-    case 8 + 2: return decay_attention_run<T, 1, 2, VEC>(c, p, ws, s);
-    case 8 + 4: return decay_attention_run<T, 1, 4, VEC>(c, p, ws, s);
-    case 16 + 1: return decay_attention_run<T, 2, 1, VEC>(c, p, ws, s);
-    case 16 + 2: return decay_attention_run<T, 2, 2, VEC>(c, p, ws, s);
-    case 16 + 4: return decay_attention_run<T, 2, 4, VEC>(c, p, ws, s);
-    case 32 + 1: return decay_attention_run<T, 4, 1, VEC>(c, p, ws, s);
-    case 32 + 2: return decay_attention_run<T, 4, 2, VEC>(c, p, ws, s);
-    case 32 + 4: return decay_attention_run<T, 4, 4, VEC>(c, p, ws, s);
-    case 64 + 1: return decay_attention_run<T, 8, 1, VEC>(c, p, ws, s);
-    case 64 + 2: return decay_attention_run<T, 8, 2, VEC>(c, p, ws, s);
+    case 8 + 1: return decay_attention_run<T, 1, 1, MODE>(c, p, ws, s);
+    case 8 + 2: return decay_attention_run<T, 1, 2, MODE>(c, p, ws, s);
+    case 8 + 4: return decay_attention_run<T, 1, 4, MODE>(c, p, ws, s);
+    case 16 + 1: return decay_attention_run<T, 2, 1, MODE>(c, p, ws, s);
+    case 16 + 2: return decay_attention_run<T, 2, 2, MODE>(c, p, ws, s);
+    case 16 + 4: return decay_attention_run<T, 2, 4, MODE>(c, p, ws, s);
+    case 32 + 1: return decay_attention_run<T, 4, 1, MODE>(c, p, ws, s);
+    case 32 + 2: return decay_attention_run<T, 4, 2, MODE>(c, p, ws, s);
+    case 32 + 4: return decay_attention_run<T, 4, 4, MODE>(c, p, ws, s);
+    case 64 + 1: return decay_attention_run<T, 8, 1, MODE>(c, p, ws, s);
+    case 64 + 2: return decay_attention_run<T, 8, 2, MODE>(c, p, ws, s);
   }
   return fail(OIGE_EINVAL, "decay_attention: no variant for %d x %d tiles", p.nk, p.nv);
 }
@@ -591,12 +643,21 @@ static bool da_wide(const DaCore& c, int bytes) {
          c.on % v == 0 && c.ot % v == 0 && c.oh % v == 0 && aligned16(c.s_in) && aligned16(c.s_out);
 }
 
+template <typename T>
+static int decay_attention_typed(const DaCore& c, const DaPlan& p, float* ws, hipStream_t s) {
+  if (!da_wide(c, sizeof(T))) return decay_attention_tiles<T, ELEMS_SINGLE>(c, p, ws, s);
+  if (c.dk == 16 * p.nk && c.dv == 16 * p.nv * p.slices) return decay_attention_tiles<T, ELEMS_FULL>(c, p, ws, s);
+  return decay_attention_tiles<T, ELEMS_WIDE>(c, p, ws, s);
+}
+
 static int decay_attention_core(const DaCore& c, int dtype, float* ws, hipStream_t s) {
+  const int64_t most = (int64_t)1 << 32;
+  OIGE_REQUIRE(c.q.st >= 0 && c.q.st < most && c.k.st >= 0 && c.k.st < most && c.v.st >= 0 && c.v.st < most,
+               "decay_attention: token strides must be below 2^32 elements and not negative");
   const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv);
-  const bool wide = da_wide(c, elem_bytes(dtype));
-  if (dtype == OIGE_F32) return wide ? decay_attention_tiles<float, true>(c, p, ws, s) : decay_attention_tiles<float, false>(c, p, ws, s);
-  if (dtype == OIGE_F16) return wide ? decay_attention_tiles<_Float16, true>(c, p, ws, s) : decay_attention_tiles<_Float16, false>(c, p, ws, s);
-  return wide ? decay_attention_tiles<__bf16, true>(c, p, ws, s) : decay_attention_tiles<__bf16, false>(c, p, ws, s);
+  if (dtype == OIGE_F32) return decay_attention_typed<float>(c, p, ws, s);
+  if (dtype == OIGE_F16) return decay_attention_typed<_Float16>(c, p, ws, s);
+  return decay_attention_typed<__bf16>(c, p, ws, s);
 }
 
 static int decay_attention_share(const float* in, void* out, const oige_decay_attention_io& io, int d, const int64_t* stride, hipStream_t s) {

@@ -80,7 +80,7 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
     float x[K][VEC];
     float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) load_run<T, VEC, (VEC > 1)>(x[k], xr, (k * lanes + l) * VEC, width);
+    for (int k = 0; k < K; ++k) load_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(x[k], xr, (k * lanes + l) * VEC, width);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
       float y[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) y[e] = fmaf(x[k][e] * rstd, w[k][e], b[k][e]);
-      store_run<T, VEC, (VEC > 1)>(y, yr, (k * lanes + l) * VEC, width);
+      store_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(y, yr, (k * lanes + l) * VEC, width);
     }
     if (a.mean && l == 0) {
       a.mean[row] = mean;
@@ -134,8 +134,8 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
     float x[K][VEC], g[K][VEC];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      load_run<T, VEC, (VEC > 1)>(x[k], xr, (k * lanes + l) * VEC, width);
-      load_run<T, VEC, (VEC > 1)>(g[k], dyr, (k * lanes + l) * VEC, width);
+      load_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(x[k], xr, (k * lanes + l) * VEC, width);
+      load_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(g[k], dyr, (k * lanes + l) * VEC, width);
     }
     const float mean = a.mean[row], rstd = a.rstd[row];
     float2 s = make_float2(0.f, 0.f);
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
         float d[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d[e] = rstd * (g[k][e] - fmaf(x[k][e], mgx, mg));
-        store_run<T, VEC, (VEC > 1)>(d, dxr, (k * lanes + l) * VEC, width);
+        store_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(d, dxr, (k * lanes + l) * VEC, width);
       }
     }
   }

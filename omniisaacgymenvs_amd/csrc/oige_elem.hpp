@@ -27,27 +27,49 @@ __device__ __forceinline__ void store_elem(void* p, int64_t i, float x, int dtyp
   else static_cast<__bf16*>(p)[i] = (__bf16)x;
 }
 
-// CNT consecutive elements from `off` of a row of `limit`, as floats; elements behind the limit read as 0.  VEC: the row starts
-// on a 16-byte boundary, `off` and `limit` are multiples of the access width.  A piece behind the end re-reads the row's first
-// one (no load inside a conditional block).
-template <typename T, int CNT, bool VEC>
+// How a row's elements are reached.  ELEMS_FULL: 16-byte accesses and every lane's piece lies inside the row.  ELEMS_WIDE: 16-byte
+// accesses (the row starts on a boundary, its length is a multiple of the access width), pieces behind its end are left out.
+// ELEMS_SINGLE: element by element.
+constexpr int ELEMS_FULL = 0, ELEMS_WIDE = 1, ELEMS_SINGLE = 2;
+
+// CNT consecutive elements from `off` of a row of `limit`, as floats; elements behind the limit read as 0.  A piece behind the end
+// re-reads the row's first one (no load inside a conditional block).
+template <typename T, int CNT, int MODE>
 __device__ __forceinline__ void load_run(float (&out)[CNT], const T* row, int off, int limit) {
-  constexpr int W = VEC ? (CNT < VEC16<T> ? CNT : VEC16<T>) : 1;
+  constexpr int W = MODE == ELEMS_SINGLE ? 1 : (CNT < VEC16<T> ? CNT : VEC16<T>);
 #pragma unroll
   for (int b = 0; b < CNT; b += W) {
-    const bool ok = off + b < limit;
+    const bool ok = MODE == ELEMS_FULL || off + b < limit;
     const Pack<T, W> x = *reinterpret_cast<const Pack<T, W>*>(row + (ok ? off + b : 0));
 #pragma unroll
     for (int e = 0; e < W; ++e) out[b + e] = ok ? (float)x.v[e] : 0.f;
   }
 }
 
-template <typename T, int CNT, bool VEC>
+// The same in two halves, the second where the values are needed: until then they stay as they are in memory, in flight.
+template <typename T, int CNT, int MODE>
+struct Run {
+  static constexpr int W = MODE == ELEMS_SINGLE ? 1 : (CNT < VEC16<T> ? CNT : VEC16<T>);
+  Pack<T, W> x[CNT / W];
+  __device__ __forceinline__ void issue(const T* row, int off, int limit) {
+#pragma unroll
+    for (int b = 0; b < CNT / W; ++b)
+      x[b] = *reinterpret_cast<const Pack<T, W>*>(row + (MODE == ELEMS_FULL || off + b * W < limit ? off + b * W : 0));
+  }
+  __device__ __forceinline__ void take(float (&out)[CNT], int off, int limit) const {
+#pragma unroll
+    for (int b = 0; b < CNT / W; ++b)
+#pragma unroll
+      for (int e = 0; e < W; ++e) out[b * W + e] = MODE == ELEMS_FULL || off + b * W < limit ? (float)x[b].v[e] : 0.f;
+  }
+};
+
+template <typename T, int CNT, int MODE>
 __device__ __forceinline__ void store_run(const float (&in)[CNT], T* row, int off, int limit) {
-  constexpr int W = VEC ? (CNT < VEC16<T> ? CNT : VEC16<T>) : 1;
+  constexpr int W = MODE == ELEMS_SINGLE ? 1 : (CNT < VEC16<T> ? CNT : VEC16<T>);
 #pragma unroll
   for (int b = 0; b < CNT; b += W) {
-    if (off + b < limit) {
+    if (MODE == ELEMS_FULL || off + b < limit) {
       Pack<T, W> x;
 #pragma unroll
       for (int e = 0; e < W; ++e) x.v[e] = (T)in[b + e];
