@@ -75,20 +75,23 @@ __device__ __forceinline__ double da_power(double decay, int64_t n) {
   }
   return r;
 }
-struct DaPowers {  // decay^n for n in 0 .. 16 without a loop, within 4 roundings
-  float p1, p2, p4, p8, p16;
+struct DaPowers {  // decay^n for n in 0 .. 32 without a loop, within 5 roundings
+  float p1, p2, p4, p8, p16, p32;
   __device__ __forceinline__ explicit DaPowers(double d) : p1((float)d), p2((float)(d * d)) {
     const double d4 = (d * d) * (d * d);
     p4 = (float)d4;
     p8 = (float)(d4 * d4);
-    p16 = (float)((d4 * d4) * (d4 * d4));
+    const double d16 = (d4 * d4) * (d4 * d4);
+    p16 = (float)d16;
+    p32 = (float)(d16 * d16);
   }
   __device__ __forceinline__ float operator()(int n) const {
     float r = (n & 1) ? p1 : 1.f;
     r *= (n & 2) ? p2 : 1.f;
     r *= (n & 4) ? p4 : 1.f;
     r *= (n & 8) ? p8 : 1.f;
-    return (n & 16) ? p16 : r;
+    r *= (n & 16) ? p16 : 1.f;
+    return (n & 32) ? p32 : r;
   }
 };
 
@@ -197,12 +200,118 @@ struct DaBlock {
     return head + low * st + (uint64_t)(uint32_t)row(i) * (uint32_t)st;
   }
 };
+template <int TOKENS>
 __device__ __forceinline__ DaBlock da_block(const DaCore& a, int64_t p0, int64_t end, int64_t len) {
   DaBlock b;
-  b.L = end - p0 < DA_TOKENS ? (int)(end - p0) : DA_TOKENS;
+  b.L = end - p0 < TOKENS ? (int)(end - p0) : TOKENS;
   b.reverse = a.reverse;
   b.low = a.reverse ? len - p0 - b.L : p0;
   return b;
+}
+
+// The lane's coordinates once more, computed where they are used: blocks that few rounds of the loop enter would otherwise have
+// their masks and weights hoisted out of it, into registers that the loop needs.
+__device__ __forceinline__ int da_here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+__device__ __forceinline__ bool da_finite(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu) < 0x7F800000u; }
+__device__ __forceinline__ f32x4 da_poison(f32x4 x, f32x4 hit) {
+  const float nan = __builtin_nanf("");
+  return f32x4{hit.x > 0.f ? nan : x.x, hit.y > 0.f ? nan : x.y, hit.z > 0.f ? nan : x.z, hit.w > 0.f ? nan : x.w};
+}
+
+// What a wave works on: a slice of the state's columns of one head of one sequence, over one segment of its tokens.
+struct DaWave {
+  int64_t n, nh, len, begin, end;
+  int h, seg, slice, dv0;
+  bool live;
+};
+template <int NV>
+__device__ __forceinline__ DaWave da_wave(const DaCore& a) {
+  DaWave w{};
+  const int64_t u = (int64_t)blockIdx.x * DA_WAVES + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  w.live = u < a.n * a.h * a.slices;
+  if (!w.live) return w;
+  w.seg = blockIdx.y;
+  w.slice = (int)(u % a.slices);
+  w.nh = u / a.slices;
+  w.h = (int)(w.nh % a.h);
+  w.n = w.nh / a.h;
+  w.dv0 = w.slice * 16 * NV;
+  w.len = da_length(a, w.n);
+  w.begin = (int64_t)w.seg * a.seg_len;
+  w.end = w.begin + a.seg_len < w.len ? w.begin + a.seg_len : w.len;
+  return w;
+}
+
+// The state in front of the segment's first token ...
+template <int NK, int NV, int MODE, bool STATES>
+__device__ __forceinline__ void da_open(f32x4 (&S)[NK][NV], const DaCore& a, const DaWave& w, int lane) {
+  if (w.seg > 0 && !STATES) {
+    const float* slot = a.seg_states + ((w.nh * a.nseg + w.seg) * a.slices + w.slice) * (int64_t)(NK * NV * 4 * WAVE);
+#pragma unroll
+    for (int s = 0; s < NK; ++s)
+#pragma unroll
+      for (int sv = 0; sv < NV; ++sv) S[s][sv] = *reinterpret_cast<const f32x4*>(slot + ((s * NV + sv) * WAVE + lane) * 4);
+  } else if (w.seg == 0 && a.s_in) {
+    da_load_state<NK, NV, MODE>(S, a.s_in + w.nh * a.dk * a.dv, a, w.dv0, lane & 15, lane >> 4);
+  } else {
+#pragma unroll
+    for (int s = 0; s < NK; ++s)
+#pragma unroll
+      for (int sv = 0; sv < NV; ++sv) S[s][sv] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// ... and what becomes of the one behind its last; rows behind the sequence's end inside this segment's stretch are cleared.
+template <typename T, int NK, int NV, int MODE, bool STATES>
+__device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, const DaWave& w, int lane, double decay, bool dropped) {
+  const int c = lane & 15, g = lane >> 4;
+  if (STATES) {
+    float* slot = a.seg_states + ((w.nh * a.nseg + w.seg) * a.slices + w.slice) * (int64_t)(NK * NV * 4 * WAVE);
+#pragma unroll
+    for (int s = 0; s < NK; ++s)
+#pragma unroll
+      for (int sv = 0; sv < NV; ++sv) *reinterpret_cast<f32x4*>(slot + ((s * NV + sv) * WAVE + lane) * 4) = S[s][sv];
+    if (w.slice == 0 && lane == 0) {
+      const int64_t count = (w.end > w.begin ? w.end - w.begin : 0) - (a.reverse && w.seg == 0 && w.end > 0 ? 1 : 0);
+      a.seg_factors[w.nh * a.nseg + w.seg] = dropped ? -1.f : (float)da_power(decay, count);
+    }
+    return;
+  }
+  const int64_t stop = w.begin + a.seg_len < a.t ? w.begin + a.seg_len : a.t;
+  for (int64_t t = (w.begin > w.len ? w.begin : w.len) + c; t < stop; t += 16) {
+    const int64_t row = w.n * a.on + t * a.ot + (int64_t)w.h * a.oh;
+    const float none[4 * NV] = {};
+    if (a.o_float) store_run<float, 4 * NV, MODE>(none, static_cast<float*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
+    else store_run<T, 4 * NV, MODE>(none, static_cast<T*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
+  }
+  if (a.s_out && w.seg == a.nseg - 1) {
+    if (a.reverse && w.len > 0) {  // dS_0 = a_0 G_0
+      const bool drop = a.resets && da_reset(a, w.n, 0);
+#pragma unroll
+      for (int s = 0; s < NK; ++s)
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) S[s][sv] = drop ? f32x4{0.f, 0.f, 0.f, 0.f} : S[s][sv] * (float)decay;
+    }
+    da_store_state<NK, NV, MODE>(S, a.s_out + w.nh * a.dk * a.dv, a, w.dv0, c, g);
+  }
+}
+
+template <typename T, int NV, int MODE>
+__device__ __forceinline__ void da_store_out(const f32x4 (&acc)[NV], const DaCore& a, int64_t row, int col) {
+  float out[4 * NV];
+#pragma unroll
+  for (int sv = 0; sv < NV; ++sv) {
+    out[sv] = acc[sv].x * a.out_scale;
+    out[NV + sv] = acc[sv].y * a.out_scale;
+    out[2 * NV + sv] = acc[sv].z * a.out_scale;
+    out[3 * NV + sv] = acc[sv].w * a.out_scale;
+  }
+  if (a.o_float) store_run<float, 4 * NV, MODE>(out, static_cast<float*>(a.o) + row, col, a.dv);
+  else store_run<T, 4 * NV, MODE>(out, static_cast<T*>(a.o) + row, col, a.dv);
 }
 
 // STATES: only the states at the segments' ends (no q, no o), for sequences cut over time.
@@ -212,19 +321,10 @@ __device__ __forceinline__ DaBlock da_block(const DaCore& a, int64_t p0, int64_t
 template <typename T, int NK, int NV, int MODE, bool STATES>
 __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(const DaCore a) {
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
-  const int64_t u = (int64_t)blockIdx.x * DA_WAVES + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t units = a.n * a.h * a.slices;
-  if (u >= units) return;
-  const int seg = blockIdx.y;
-  const int slice = (int)(u % a.slices);
-  const int64_t nh = u / a.slices;
-  const int h = (int)(nh % a.h);
-  const int64_t n = nh / a.h;
-  const int dv0 = slice * 16 * NV;
-  const int64_t len = da_length(a, n);
-  const int64_t begin = (int64_t)seg * a.seg_len;
-  int64_t end = begin + a.seg_len;
-  if (end > len) end = len;
+  const DaWave w = da_wave<NV>(a);
+  if (!w.live) return;
+  const int64_t n = w.n, nh = w.nh, len = w.len, begin = w.begin, end = w.end;
+  const int h = w.h, seg = w.seg, slice = w.slice, dv0 = w.dv0;
 
   const T* qh = static_cast<const T*>(a.q.p) + n * a.q.sn + (int64_t)(h / a.q.group) * a.q.sh;
   const T* kh = static_cast<const T*>(a.k.p) + n * a.k.sn + (int64_t)(h / a.k.group) * a.k.sh;
@@ -249,7 +349,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     if (a.resets) flag = (not_first || !b.reverse || c > 0) && c < b.L && da_reset(a, n, b.low + b.row(c) + b.reverse);
   };
 
-  DaBlock blk = da_block(a, begin, end, len);
+  DaBlock blk = da_block<DA_TOKENS>(a, begin, end, len);
   if (begin < end) {
     issue_rows(blk);
     issue_columns(blk, begin > 0);
@@ -257,21 +357,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
 
   f32x4 S[NK][NV];
   const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-  constexpr int UNIT = NK * NV * 4 * WAVE;  // floats of a wave's state
-  float* seg_slot = a.seg_states + ((nh * a.nseg + seg) * a.slices + slice) * (int64_t)UNIT;
-  if (seg > 0 && !STATES) {
-#pragma unroll
-    for (int s = 0; s < NK; ++s)
-#pragma unroll
-      for (int sv = 0; sv < NV; ++sv) S[s][sv] = *reinterpret_cast<const f32x4*>(seg_slot + ((s * NV + sv) * WAVE + lane) * 4);
-  } else if (seg == 0 && a.s_in) {
-    da_load_state<NK, NV, MODE>(S, a.s_in + nh * a.dk * a.dv, a, dv0, c, g);
-  } else {
-#pragma unroll
-    for (int s = 0; s < NK; ++s)
-#pragma unroll
-      for (int sv = 0; sv < NV; ++sv) S[s][sv] = zero;
-  }
+  da_open<NK, NV, MODE, STATES>(S, a, w, lane);
 
   const double decay = (double)a.decay[h];
   const DaPowers pw(decay);
@@ -283,6 +369,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     const int L = blk.L;
     if (p0 == begin || p0 == DA_TOKENS || L < DA_TOKENS) {
       const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
+      const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
       const double keep = da_power(decay, L - first);
       keep_hi = (float)keep;
       keep_lo = (float)(keep - (double)keep_hi);  // the rounding of decay^16 would pile up over a long memory
@@ -296,132 +383,484 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     }
     const uint32_t m = (uint32_t)(__ballot(flag) & 0xFFFFull);  // bit i: a reset in front of the block's token i
     const bool more = p0 + DA_TOKENS < end;
-    const DaBlock next = da_block(a, more ? p0 + DA_TOKENS : p0, end, len);  // behind the last block: the same rows once more
+    const DaBlock next = da_block<DA_TOKENS>(a, more ? p0 + DA_TOKENS : p0, end, len);  // behind the last block: the same rows once more
 
-    float P[4];
     f32x4 acc[NV];
-    float Q[4 * NK];
-    const bool from_state = !(m & upto);
+    float V[4][NV];
     if (!STATES) {
-      float K1[4 * NK];
+      float Q[4 * NK], K1[4 * NK];
       q_run.take(Q, 4 * NK * g, a.dk);
       k1_run.take(K1, 4 * NK * g, a.dk);
       f32x4 pt = zero;
 #pragma unroll
       for (int e = 0; e < 4 * NK; ++e) pt = __builtin_amdgcn_mfma_f32_16x16x4f32(K1[e], Q[e], pt, 0, 0, 0);
-      const float p4[4] = {pt.x, pt.y, pt.z, pt.w};
+      da_state_part<NK, NV>(acc, S, Q, !(m & upto), head_w);
+      // a masked product may be infinite or NaN: selected away, not multiplied
+      float P[4] = {pt.x, pt.y, pt.z, pt.w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) P[r] = 4 * g + r <= c ? P[r] * pair_w[r] : 0.f;
+      if (m) {
+        const int g = da_here(lane) >> 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) P[r] = m & upto & ~((2u << (4 * g + r)) - 1u) ? 0.f : P[r];
+      }
+      uint32_t top = 0;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int j = 4 * g + r;
-        const bool sees = j <= c && !(m & upto & ~((2u << j) - 1u));
-        P[r] = sees ? p4[r] * pair_w[r] : 0.f;  // a masked product may be infinite or NaN: selected away, not multiplied
+        v_run[r].take(V[r], dv0 + NV * c, a.dv);
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) top = max(top, __builtin_bit_cast(uint32_t, V[r][sv]) & 0x7FFFFFFFu);
       }
-      da_state_part<NK, NV>(acc, S, Q, from_state, head_w);
-    }
-    float V[4][NV], K2[4][NK];
+      if (__any(top >= 0x7F800000u)) {
+        // An infinite or NaN value: where a token sees it the result is NaN, everywhere else (its weight is zero) it is left out.
+        const int g = da_here(lane) >> 4;
+        f32x4 hit[NV];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      v_run[r].take(V[r], dv0 + NV * c, a.dv);
+        for (int sv = 0; sv < NV; ++sv) hit[sv] = zero;
 #pragma unroll
-      for (int sv = 0; sv < NV; ++sv) V[r][sv] = 4 * g + r < L ? V[r][sv] : 0.f;
-    }
-    if (!STATES) {
+        for (int r = 0; r < 4; ++r) {
+          const float seen = 4 * g + r <= c && !(m & upto & ~((2u << (4 * g + r)) - 1u)) ? 1.f : 0.f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int sv = 0; sv < NV; ++sv) acc[sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[r][sv], P[r], acc[sv], 0, 0, 0);
-      // An infinite or NaN value in a row that some tokens must not see has met their zero weights in the product.  Such blocks
-      // (any output not finite) are summed again pair by pair.
-      f32x4 z = zero;
-#pragma unroll
-      for (int sv = 0; sv < NV; ++sv) z += acc[sv] * 0.f;
-      const float z1 = (z.x + z.y) + (z.z + z.w);
-      if (__any(c < L && z1 != z1)) {
-        da_state_part<NK, NV>(acc, S, Q, from_state, head_w);
-#pragma unroll 1
-        for (int gj = 0; gj < 4; ++gj) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = 4 * gj + r, at = gj * 16 + 4 * g;
-            const float w = __shfl(P[r], gj * 16 + c, WAVE);
-            const bool sees = j <= c && !(m & upto & ~((2u << j) - 1u));
-#pragma unroll
-            for (int sv = 0; sv < NV; ++sv) {
-              const f32x4 v{__shfl(V[r][sv], at, WAVE), __shfl(V[r][sv], at + 1, WAVE), __shfl(V[r][sv], at + 2, WAVE), __shfl(V[r][sv], at + 3, WAVE)};
-              acc[sv] = sees ? acc[sv] + v * w : acc[sv];
-            }
-          }
+          for (int sv = 0; sv < NV; ++sv) hit[sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(da_finite(V[r][sv]) ? 0.f : 1.f, seen, hit[sv], 0, 0, 0);
         }
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) acc[sv] = da_poison(acc[sv], hit[sv]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int sv = 0; sv < NV; ++sv)
+            acc[sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(da_finite(V[r][sv]) ? V[r][sv] : 0.f, P[r], acc[sv], 0, 0, 0);
+        da_settle();
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int sv = 0; sv < NV; ++sv) acc[sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[r][sv], P[r], acc[sv], 0, 0, 0);
+        da_settle();
       }
       issue_rows(next);
-      if (c < L) {
-        float out[4 * NV];
+      if (c < L) da_store_out<T, NV, MODE>(acc, a, n * a.on + (blk.low + blk.row(c)) * a.ot + (int64_t)h * a.oh, dv0 + 4 * NV * g);
+    } else {
 #pragma unroll
-        for (int sv = 0; sv < NV; ++sv) {
-          out[sv] = acc[sv].x * a.out_scale;
-          out[NV + sv] = acc[sv].y * a.out_scale;
-          out[2 * NV + sv] = acc[sv].z * a.out_scale;
-          out[3 * NV + sv] = acc[sv].w * a.out_scale;
-        }
-        const int64_t row = n * a.on + (blk.low + blk.row(c)) * a.ot + (int64_t)h * a.oh;
-        if (a.o_float) store_run<float, 4 * NV, MODE>(out, static_cast<float*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
-        else store_run<T, 4 * NV, MODE>(out, static_cast<T*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
-      }
+      for (int r = 0; r < 4; ++r) v_run[r].take(V[r], dv0 + NV * c, a.dv);
     }
 
-    // the state behind the block: rows in front of its last reset, and behind the end, stay out of the sum altogether
+    float K2[4][NK];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool in = 4 * g + r < L && !(m & ~((2u << (4 * g + r)) - 1u));
-      k2_run[r].take(K2[r], NK * c, a.dk);
+    for (int r = 0; r < 4; ++r) k2_run[r].take(K2[r], NK * c, a.dk);
+    // rows in front of the block's last reset, and behind the end, stay out of the state's sum altogether
+    if (m || L < DA_TOKENS) {
+      const int g = da_here(lane) >> 4;
 #pragma unroll
-      for (int s = 0; s < NK; ++s) K2[r][s] = in ? K2[r][s] : 0.f;
+      for (int r = 0; r < 4; ++r) {
+        const bool in = 4 * g + r < L && !(m & ~((2u << (4 * g + r)) - 1u));
 #pragma unroll
-      for (int sv = 0; sv < NV; ++sv) V[r][sv] = in ? V[r][sv] * tail_w[r] : 0.f;
+        for (int s = 0; s < NK; ++s) K2[r][s] = in ? K2[r][s] : 0.f;
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) V[r][sv] = in ? V[r][sv] : 0.f;
+      }
     }
-    dropped |= m != 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int sv = 0; sv < NV; ++sv) V[r][sv] *= tail_w[r];
+    if (m) {  // (a state that is not finite is dropped too: cleared, not multiplied)
+      dropped = true;
+#pragma unroll
+      for (int s = 0; s < NK; ++s)
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) S[s][sv] = zero;
+    }
     issue_columns(next, true);
 #pragma unroll
     for (int s = 0; s < NK; ++s)
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) {
-        S[s][sv] = m ? zero : __builtin_elementwise_fma(S[s][sv], f32x4(keep_hi), S[s][sv] * keep_lo);
+        S[s][sv] = __builtin_elementwise_fma(S[s][sv], f32x4(keep_hi), S[s][sv] * keep_lo);
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[s][sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(K2[r][s], V[r][sv], S[s][sv], 0, 0, 0);
       }
     da_settle();
     blk = next;
   }
+  da_close<T, NK, NV, MODE, STATES>(S, a, w, lane, decay, dropped);
+}
 
-  if (STATES) {
+// ---------------------------------------------------------------- the same for bf16 tensors
+// bf16 operands go into v_mfma_f32_16x16x32_bf16, 16 times the rate of the 32-bit instruction, in blocks of 32 tokens:
+//   K Q^T        both operands as they are: exact products, 32-bit sums
+//   S Q, P V     the 32-bit factor as a sum of two bf16 numbers (hi + lo; what is left out is at most 2^-18 of it), two products
+//   K^T (w V)    w V as a sum of three (at most 2^-27 of it is left out): the state stays a 32-bit sum
+// The operand that a product sums over lies packed along registers, eight to a lane: for tokens, lane group g holds 4 g + {0..3} and
+// 16 + 4 g + {0..3}, as K Q^T leaves them; for dk, the four rows of two neighbouring tiles, as the state keeps them.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr int DB_TOKENS = 32;
+
+__device__ __forceinline__ f32x4 db_mfma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t db_pack(float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, bf16x2)); }
+__device__ __forceinline__ float db_low(uint32_t p) { return __builtin_bit_cast(float, p << 16); }
+__device__ __forceinline__ float db_high(uint32_t p) { return __builtin_bit_cast(float, p & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t db_lows(uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x05040100); }   // {x.low, y.low}
+__device__ __forceinline__ uint32_t db_highs(uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x07060302); }  // {x.high, y.high}
+// x, y = hi + lo up to 2^-18 of each; with a third, up to 2^-27
+__device__ __forceinline__ void db_split(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = db_pack(x, y);
+  lo = db_pack(x - db_low(hi), y - db_high(hi));
+}
+__device__ __forceinline__ void db_split(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = db_pack(x, y);
+  x -= db_low(hi);
+  y -= db_high(hi);
+  mid = db_pack(x, y);
+  lo = db_pack(x - db_low(mid), y - db_high(mid));
+}
+
+// CNT bf16 elements of a row, two to a register (one, where CNT is 1); elements behind the limit are 0.
+template <int CNT, int MODE>
+struct Bits {
+  static constexpr int REGS = CNT == 1 ? 1 : CNT / 2;
+  Run<uint16_t, CNT, MODE> run;
+  // `base` is the same for the whole wave, `row` this lane's row in elements behind it
+  __device__ __forceinline__ void issue(const __bf16* base, uint32_t row, int off, int limit) {
+    constexpr int W = Run<uint16_t, CNT, MODE>::W;
 #pragma unroll
-    for (int s = 0; s < NK; ++s)
-#pragma unroll
-      for (int sv = 0; sv < NV; ++sv) *reinterpret_cast<f32x4*>(seg_slot + ((s * NV + sv) * WAVE + lane) * 4) = S[s][sv];
-    if (slice == 0 && lane == 0) {
-      const int64_t count = (end > begin ? end - begin : 0) - (a.reverse && seg == 0 && end > 0 ? 1 : 0);
-      a.seg_factors[nh * a.nseg + seg] = dropped ? -1.f : (float)da_power(decay, count);
+    for (int b = 0; b < CNT / W; ++b) {
+      const uint32_t at = 2u * (row + (uint32_t)(MODE == ELEMS_FULL || off + b * W < limit ? off + b * W : 0));
+      run.x[b] = *reinterpret_cast<const Pack<uint16_t, W>*>(reinterpret_cast<const char*>(base) + at);
     }
-    return;
   }
-  // rows behind the sequence's end inside this segment's stretch of the tensor
-  const int64_t stop = begin + a.seg_len < a.t ? begin + a.seg_len : a.t;
-  for (int64_t t = (begin > len ? begin : len) + c; t < stop; t += 16) {
-    const int64_t row = n * a.on + t * a.ot + (int64_t)h * a.oh;
-    const float none[4 * NV] = {};
-    if (a.o_float) store_run<float, 4 * NV, MODE>(none, static_cast<float*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
-    else store_run<T, 4 * NV, MODE>(none, static_cast<T*>(a.o) + row, dv0 + 4 * NV * g, a.dv);
+  __device__ __forceinline__ void take(uint32_t (&out)[REGS], int off, int limit) const {
+    constexpr int W = Run<uint16_t, CNT, MODE>::W;
+#pragma unroll
+    for (int i = 0; i < REGS; ++i) {
+      const int e = CNT == 1 ? 0 : 2 * i;
+      const bool ok0 = MODE == ELEMS_FULL || off + e / W * W < limit, ok1 = MODE == ELEMS_FULL || off + (e + 1) / W * W < limit;
+      const uint32_t lo = run.x[e / W].v[e % W];
+      const uint32_t hi = CNT == 1 ? 0u : (uint32_t)run.x[(e + 1) / W].v[(e + 1) % W];
+      out[i] = (ok0 ? lo : 0u) | (CNT == 1 || !ok1 ? 0u : hi << 16);
+    }
   }
-  if (a.s_out && seg == a.nseg - 1) {
-    if (a.reverse && len > 0) {  // dS_0 = a_0 G_0
-      const bool drop = a.resets && da_reset(a, n, 0);
+};
+// element e of a row held that way, paired over two rows
+template <int E>
+__device__ __forceinline__ uint32_t db_pair(uint32_t x, uint32_t y) {
+  return E & 1 ? db_highs(x, y) : db_lows(x, y);
+}
+
+// O^T's part from the state: for both halves of the block's tokens, the state's hi and lo parts against q.
+template <int NK, int NV>
+__device__ __forceinline__ void db_state_part(f32x4 (&acc)[2][NV], const f32x4 (&S)[NK][NV], const uint32_t (&Q)[2][2 * NK],
+                                              const bool (&from_state)[2], const float (&head_w)[2]) {
+  const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int it = 0; it < 2; ++it)
+#pragma unroll
+    for (int sv = 0; sv < NV; ++sv) acc[it][sv] = zero;
+#pragma unroll
+  for (int p = 0; p < NK / 2; ++p) {
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 q[2];
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      const uint32_t x0 = Q[it][p], x1 = Q[it][NK / 2 + p], x2 = Q[it][NK + p], x3 = Q[it][3 * NK / 2 + p];
+      q[it] = u32x4{db_lows(x0, x1), db_lows(x2, x3), db_highs(x0, x1), db_highs(x2, x3)};
+    }
+#pragma unroll
+    for (int sv = 0; sv < NV; ++sv) {
+      const f32x4 s0 = S[2 * p][sv], s1 = S[2 * p + 1][sv];
+      uint32_t hi[4], lo[4];
+      db_split(s0.x, s0.y, hi[0], lo[0]);
+      db_split(s0.z, s0.w, hi[1], lo[1]);
+      db_split(s1.x, s1.y, hi[2], lo[2]);
+      db_split(s1.z, s1.w, hi[3], lo[3]);
+      const u32x4 h{hi[0], hi[1], hi[2], hi[3]}, l{lo[0], lo[1], lo[2], lo[3]};
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        acc[it][sv] = db_mfma(l, q[it], acc[it][sv]);
+        acc[it][sv] = db_mfma(h, q[it], acc[it][sv]);
+      }
+    }
+  }
+#pragma unroll
+  for (int it = 0; it < 2; ++it)
+#pragma unroll
+    for (int sv = 0; sv < NV; ++sv) acc[it][sv] = from_state[it] ? acc[it][sv] * head_w[it] : zero;
+}
+
+// Offset of token `i` of a block of L from its earliest one, in elements of less than 32 bits: `step` = the token stride times i.
+__device__ __forceinline__ uint32_t db_offset(const DaBlock& b, uint32_t step, uint32_t st) {
+  const uint32_t last = (uint32_t)(b.L - 1) * st;
+  const uint32_t off = step < last ? step : last;
+  return b.reverse ? last - off : off;
+}
+
+template <int NK, int NV, int MODE, bool STATES>
+__global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel(const DaCore a) {
+  const int lane = lane_id(), c = lane & 15, g = lane >> 4;
+  const DaWave w = da_wave<NV>(a);
+  if (!w.live) return;
+  const int64_t n = w.n, len = w.len, begin = w.begin, end = w.end;
+  const int h = w.h, dv0 = w.dv0;
+  const __bf16* qh = static_cast<const __bf16*>(a.q.p) + n * a.q.sn + (int64_t)(h / a.q.group) * a.q.sh;
+  const __bf16* kh = static_cast<const __bf16*>(a.k.p) + n * a.k.sn + (int64_t)(h / a.k.group) * a.k.sh;
+  const __bf16* vh = static_cast<const __bf16*>(a.v.p) + n * a.v.sn + (int64_t)(h / a.v.group) * a.v.sh;
+
+  Bits<4 * NK, MODE> q_run[2], k1_run[2];
+  Bits<NK, MODE> k2_run[8];
+  Bits<NV, MODE> v_run[8];
+  bool flag = false;
+  const uint32_t qst = (uint32_t)a.q.st, kst = (uint32_t)a.k.st, vst = (uint32_t)a.v.st;
+  const uint32_t q_lane = c * qst, k_lane = c * kst, k_group = 4 * g * kst, v_group = 4 * g * vst;
+  const auto issue_rows = [&](const DaBlock& b) {
+    if (STATES) return;
+    const __bf16 *q0 = qh + b.low * a.q.st, *k0 = kh + b.low * a.k.st;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      k1_run[i].issue(k0, db_offset(b, k_lane + 16 * i * kst, kst), 4 * NK * g, a.dk);
+      q_run[i].issue(q0, db_offset(b, q_lane + 16 * i * qst, qst), 4 * NK * g, a.dk);
+    }
+  };
+  const auto issue_v = [&](const DaBlock& b, bool not_first) {
+    const __bf16* v0 = vh + b.low * a.v.st;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v_run[e].issue(v0, db_offset(b, v_group + (uint32_t)(e < 4 ? e : 12 + e) * vst, vst), dv0 + NV * c, a.dv);
+    const int i = lane & 31;
+    if (a.resets) flag = (not_first || !b.reverse || i > 0) && i < b.L && da_reset(a, n, b.low + b.row(i) + b.reverse);
+  };
+  const auto issue_k = [&](const DaBlock& b) {
+    const __bf16* k0 = kh + b.low * a.k.st;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) k2_run[e].issue(k0, db_offset(b, k_group + (uint32_t)(e < 4 ? e : 12 + e) * kst, kst), NK * c, a.dk);
+  };
+
+  DaBlock blk = da_block<DB_TOKENS>(a, begin, end, len);
+  if (begin < end) {
+    issue_rows(blk);
+    issue_v(blk, begin > 0);
+    issue_k(blk);
+  }
+  f32x4 S[NK][NV];
+  const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+  da_open<NK, NV, MODE, STATES>(S, a, w, lane);
+
+  const double decay = (double)a.decay[h];
+  const DaPowers pw(decay);
+  bool dropped = false;
+  float head_w[2] = {0.f, 0.f}, pair_w[4], cross_w[4], tail_w[8], keep_hi = 0.f, keep_lo = 0.f;
+
+  for (int64_t p0 = begin; p0 < end; p0 += DB_TOKENS) {
+    const int L = blk.L;
+    if (p0 == begin || p0 == DB_TOKENS || L < DB_TOKENS) {
+      const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
+      const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
+      const double keep = da_power(decay, L - first);
+      keep_hi = (float)keep;
+      keep_lo = (float)(keep - (double)keep_hi);  // the rounding of decay^32 would pile up over a long memory
+      head_w[0] = pw(c + 1 - first);
+      head_w[1] = pw(c + 17 - first);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = 4 * g + r;
+        pair_w[r] = j <= c ? pw(c - j) * a.kv_scale : 0.f;
+        cross_w[r] = pw(16 + c - j) * a.kv_scale;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = (e < 4 ? 0 : 12) + 4 * g + e;
+        tail_w[e] = j < L ? pw(L - 1 - j) * a.kv_scale : 0.f;
+      }
+    }
+    const uint32_t m = (uint32_t)__ballot(flag);  // bit i: a reset in front of the block's token i
+    const bool more = p0 + DB_TOKENS < end;
+    const DaBlock next = da_block<DB_TOKENS>(a, more ? p0 + DB_TOKENS : p0, end, len);  // behind the last block: the same rows once more
+    const uint32_t upto[2] = {(2u << c) - 1u, (0x20000u << c) - 1u};  // bits 0 .. i for token i = c, 16 + c
+
+    uint32_t V[8][Bits<NV, MODE>::REGS];
+    if (!STATES) {
+      f32x4 acc[2][NV];
+      uint32_t Q[2][2 * NK], K1[2][2 * NK];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        q_run[i].take(Q[i], 4 * NK * g, a.dk);
+        k1_run[i].take(K1[i], 4 * NK * g, a.dk);
+      }
+      f32x4 pt[3] = {zero, zero, zero};  // P^T: tokens 0-15 for 0-15, 0-15 for 16-31, 16-31 for 16-31
+#pragma unroll
+      for (int p = 0; p < NK / 2; ++p) {
+        u32x4 q[2], k[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          q[i] = u32x4{Q[i][4 * p], Q[i][4 * p + 1], Q[i][4 * p + 2], Q[i][4 * p + 3]};
+          k[i] = u32x4{K1[i][4 * p], K1[i][4 * p + 1], K1[i][4 * p + 2], K1[i][4 * p + 3]};
+        }
+        pt[0] = db_mfma(k[0], q[0], pt[0]);
+        pt[1] = db_mfma(k[0], q[1], pt[1]);
+        pt[2] = db_mfma(k[1], q[1], pt[2]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const bool from_state[2] = {!(m & upto[0]), !(m & upto[1])};
+      db_state_part<NK, NV>(acc, S, Q, from_state, head_w);
+      __builtin_amdgcn_sched_barrier(0);
+      // a masked product may be infinite or NaN: selected away, not multiplied
+      float P[3][4] = {{pt[0].x, pt[0].y, pt[0].z, pt[0].w}, {pt[1].x, pt[1].y, pt[1].z, pt[1].w}, {pt[2].x, pt[2].y, pt[2].z, pt[2].w}};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        P[0][r] = 4 * g + r <= c ? P[0][r] * pair_w[r] : 0.f;
+        P[1][r] *= cross_w[r];
+        P[2][r] = 4 * g + r <= c ? P[2][r] * pair_w[r] : 0.f;
+      }
+      if (m) {
+        const int g = da_here(lane) >> 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t behind = ~((2u << (4 * g + r)) - 1u);  // bits j + 1 ..
+          P[0][r] = m & upto[0] & behind ? 0.f : P[0][r];
+          P[1][r] = m & upto[1] & behind ? 0.f : P[1][r];
+          P[2][r] = m & upto[1] & (behind << 16) ? 0.f : P[2][r];
+        }
+      }
+      u32x4 hi[2], lo[2];
+      hi[0] = lo[0] = u32x4{0u, 0u, 0u, 0u};
+      {
+        uint32_t x[12];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          db_split(P[i][0], P[i][1], x[4 * i], x[4 * i + 1]);
+          db_split(P[i][2], P[i][3], x[4 * i + 2], x[4 * i + 3]);
+        }
+        hi[0] = u32x4{x[0], x[2], 0u, 0u};
+        lo[0] = u32x4{x[1], x[3], 0u, 0u};
+        hi[1] = u32x4{x[4], x[6], x[8], x[10]};
+        lo[1] = u32x4{x[5], x[7], x[9], x[11]};
+      }
+      bool odd = false;  // infinite or NaN
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v_run[e].take(V[e], dv0 + NV * c, a.dv);
+#pragma unroll
+        for (int i = 0; i < Bits<NV, MODE>::REGS; ++i) odd |= (V[e][i] & 0x7F80u) == 0x7F80u || (V[e][i] & 0x7F800000u) == 0x7F800000u;
+      }
+      if (__any(odd)) {
+        // An infinite or NaN value: where a token sees it the result is NaN, everywhere else (its weight is zero) it is left out.
+        const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
+        u32x4 seen[2];
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          uint32_t x[4];
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const int j = (p < 2 ? 0 : 12) + 4 * g + 2 * p;
+            const bool s0 = j <= 16 * it + c && !(m & upto[it] & ~((2u << j) - 1u)), s1 = j + 1 <= 16 * it + c && !(m & upto[it] & ~((4u << j) - 1u));
+            x[p] = (s0 ? 0x3F80u : 0u) | (s1 ? 0x3F800000u : 0u);
+          }
+          seen[it] = u32x4{x[0], x[1], x[2], x[3]};
+        }
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) {
+          uint32_t kept[4], bad[4];
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const uint32_t x = sv & 1 ? db_highs(V[2 * p][sv / 2], V[2 * p + 1][sv / 2]) : db_lows(V[2 * p][sv / 2], V[2 * p + 1][sv / 2]);
+            const bool b0 = (x & 0x7F80u) == 0x7F80u, b1 = (x & 0x7F800000u) == 0x7F800000u;
+            bad[p] = (b0 ? 0x3F80u : 0u) | (b1 ? 0x3F800000u : 0u);
+            kept[p] = x & ((b0 ? 0u : 0xFFFFu) | (b1 ? 0u : 0xFFFF0000u));
+          }
+          const u32x4 v{kept[0], kept[1], kept[2], kept[3]}, b{bad[0], bad[1], bad[2], bad[3]};
+#pragma unroll
+          for (int it = 0; it < 2; ++it) {
+            acc[it][sv] = da_poison(acc[it][sv], db_mfma(b, seen[it], zero));
+            acc[it][sv] = db_mfma(v, lo[it], acc[it][sv]);
+            acc[it][sv] = db_mfma(v, hi[it], acc[it][sv]);
+          }
+        }
+        da_settle();
+      } else {
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) {
+          const int i = sv / 2;
+          const u32x4 v = sv & 1 ? u32x4{db_highs(V[0][i], V[1][i]), db_highs(V[2][i], V[3][i]), db_highs(V[4][i], V[5][i]), db_highs(V[6][i], V[7][i])}
+                                 : u32x4{db_lows(V[0][i], V[1][i]), db_lows(V[2][i], V[3][i]), db_lows(V[4][i], V[5][i]), db_lows(V[6][i], V[7][i])};
+#pragma unroll
+          for (int it = 0; it < 2; ++it) {
+            acc[it][sv] = db_mfma(v, lo[it], acc[it][sv]);
+            acc[it][sv] = db_mfma(v, hi[it], acc[it][sv]);
+          }
+        }
+        da_settle();
+      }
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const int i = 16 * it + c;
+        if (i < L) da_store_out<__bf16, NV, MODE>(acc[it], a, n * a.on + (blk.low + blk.row(i)) * a.ot + (int64_t)h * a.oh, dv0 + 4 * NV * g);
+      }
+      issue_rows(next);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v_run[e].take(V[e], dv0 + NV * c, a.dv);
+    }
+
+    __builtin_amdgcn_sched_barrier(0);
+    uint32_t K2[8][NK / 2];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) k2_run[e].take(K2[e], NK * c, a.dk);
+    // rows in front of the block's last reset, and behind the end, stay out of the state's sum altogether
+    if (m || L < DB_TOKENS) {
+      const int g = da_here(lane) >> 4;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = (e < 4 ? 0 : 12) + 4 * g + e;
+        const bool in = j < L && !(m & ~((2u << j) - 1u));
+#pragma unroll
+        for (int i = 0; i < NK / 2; ++i) K2[e][i] = in ? K2[e][i] : 0u;
+#pragma unroll
+        for (int i = 0; i < Bits<NV, MODE>::REGS; ++i) V[e][i] = in ? V[e][i] : 0u;
+      }
+    }
+    u32x4 vh3[NV], vm3[NV], vl3[NV];
+#pragma unroll
+    for (int sv = 0; sv < NV; ++sv) {
+      uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const uint32_t b0 = V[2 * p][sv / 2], b1 = V[2 * p + 1][sv / 2];
+        db_split((sv & 1 ? db_high(b0) : db_low(b0)) * tail_w[2 * p], (sv & 1 ? db_high(b1) : db_low(b1)) * tail_w[2 * p + 1], hi[p], mid[p], lo[p]);
+      }
+      vh3[sv] = u32x4{hi[0], hi[1], hi[2], hi[3]};
+      vm3[sv] = u32x4{mid[0], mid[1], mid[2], mid[3]};
+      vl3[sv] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+    }
+    if (m) {  // (a state that is not finite is dropped too: cleared, not multiplied)
+      dropped = true;
 #pragma unroll
       for (int s = 0; s < NK; ++s)
 #pragma unroll
-        for (int sv = 0; sv < NV; ++sv) S[s][sv] = drop ? zero : S[s][sv] * (float)decay;
+        for (int sv = 0; sv < NV; ++sv) S[s][sv] = zero;
     }
-    da_store_state<NK, NV, MODE>(S, a.s_out + nh * a.dk * a.dv, a, dv0, c, g);
+    issue_v(next, true);
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int i = s / 2;
+      const u32x4 k = s & 1 ? u32x4{db_highs(K2[0][i], K2[1][i]), db_highs(K2[2][i], K2[3][i]), db_highs(K2[4][i], K2[5][i]), db_highs(K2[6][i], K2[7][i])}
+                            : u32x4{db_lows(K2[0][i], K2[1][i]), db_lows(K2[2][i], K2[3][i]), db_lows(K2[4][i], K2[5][i]), db_lows(K2[6][i], K2[7][i])};
+#pragma unroll
+      for (int sv = 0; sv < NV; ++sv) {
+        S[s][sv] = __builtin_elementwise_fma(S[s][sv], f32x4(keep_hi), S[s][sv] * keep_lo);
+        S[s][sv] = db_mfma(k, vl3[sv], S[s][sv]);
+        S[s][sv] = db_mfma(k, vm3[sv], S[s][sv]);
+        S[s][sv] = db_mfma(k, vh3[sv], S[s][sv]);
+      }
+    }
+    issue_k(next);
+    da_settle();
+    blk = next;
   }
+  da_close<__bf16, NK, NV, MODE, STATES>(S, a, w, lane, decay, dropped);
 }
 
 // The states in front of every segment from those at the segments' ends (in place, register order): carry = factor carry + end.
@@ -570,10 +1009,10 @@ struct DaPlan {
 // joined by one small launch, then every piece by itself.
 constexpr int64_t DA_FEW_WAVES = 1024, DA_WANT_WAVES = 2048, DA_MIN_SEGMENT = 64;
 
-static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv) {
+static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, bool bf16) {
   DaPlan p;
-  p.nk = dk <= 16 ? 1 : dk <= 32 ? 2 : dk <= 64 ? 4 : 8;
-  p.nv = dv <= 16 ? 1 : (dv <= 32 || p.nk == 8) ? 2 : 4;
+  p.nk = dk <= 16 && !bf16 ? 1 : dk <= 32 ? 2 : dk <= 64 ? 4 : 8;
+  p.nv = dv <= 16 ? 1 : (dv <= 32 || p.nk == 8 || bf16) ? 2 : 4;
   p.slices = (dv + 16 * p.nv - 1) / (16 * p.nv);
   const int64_t waves = n * h * p.slices;
   p.nseg = 1;
@@ -582,14 +1021,14 @@ static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv) 
     int64_t want = (DA_WANT_WAVES + waves - 1) / waves;
     if (want > t / DA_MIN_SEGMENT) want = t / DA_MIN_SEGMENT;
     p.seg_len = (t + want - 1) / want;
-    p.seg_len = (p.seg_len + DA_TOKENS - 1) / DA_TOKENS * DA_TOKENS;
+    p.seg_len = (p.seg_len + DB_TOKENS - 1) / DB_TOKENS * DB_TOKENS;
     p.nseg = (int)((t + p.seg_len - 1) / p.seg_len);
   }
   p.seg_floats = p.nseg > 1 ? n * h * p.nseg * (p.slices * (int64_t)(p.nk * p.nv * 4 * WAVE) + 4) : 0;
   return p;
 }
 
-template <typename T, int NK, int NV, int MODE>
+template <typename T, int NK, int NV, int MODE, bool BF16>
 static int decay_attention_run(DaCore c, const DaPlan& p, float* workspace, hipStream_t stream) {
   c.slices = p.slices;
   c.nseg = p.nseg;
@@ -597,11 +1036,19 @@ static int decay_attention_run(DaCore c, const DaPlan& p, float* workspace, hipS
   const int64_t units = c.n * c.h * p.slices, blocks = (units + DA_WAVES - 1) / DA_WAVES;
   const int64_t per_head = (int64_t)p.slices * NK * NV * WAVE;  // in 16-byte quads
   OIGE_REQUIRE(blocks < ((int64_t)1 << 31), "decay_attention: %lld sequences x heads are too many for one launch", (long long)(c.n * c.h));
+  void (*states)(DaCore);
+  void (*main)(DaCore);
+  if constexpr (BF16) {
+    states = decay_attention_bf16_kernel<NK, NV, MODE, true>;
+    main = decay_attention_bf16_kernel<NK, NV, MODE, false>;
+  } else {
+    states = decay_attention_kernel<T, NK, NV, MODE, true>;
+    main = decay_attention_kernel<T, NK, NV, MODE, false>;
+  }
   if (p.nseg > 1) {
     c.seg_states = workspace;
     c.seg_factors = workspace + c.n * c.h * p.nseg * per_head * 4;
-    hipLaunchKernelGGL((decay_attention_kernel<T, NK, NV, MODE, true>), dim3((unsigned)blocks, (unsigned)(p.nseg - 1)), dim3(DA_WAVES * WAVE), 0,
-                       stream, c);
+    hipLaunchKernelGGL(states, dim3((unsigned)blocks, (unsigned)(p.nseg - 1)), dim3(DA_WAVES * WAVE), 0, stream, c);
     int rc = check_launch("decay_attention_kernel (states)");
     if (rc) return rc;
     const int64_t quads = c.n * c.h * per_head;
@@ -610,24 +1057,24 @@ static int decay_attention_run(DaCore c, const DaPlan& p, float* workspace, hipS
     rc = check_launch("decay_attention_join_kernel");
     if (rc) return rc;
   }
-  hipLaunchKernelGGL((decay_attention_kernel<T, NK, NV, MODE, false>), dim3((unsigned)blocks, (unsigned)p.nseg), dim3(DA_WAVES * WAVE), 0, stream, c);
+  hipLaunchKernelGGL(main, dim3((unsigned)blocks, (unsigned)p.nseg), dim3(DA_WAVES * WAVE), 0, stream, c);
   return check_launch("decay_attention_kernel");
 }
 
 template <typename T, int MODE>
 static int decay_attention_tiles(const DaCore& c, const DaPlan& p, float* ws, hipStream_t s) {
   switch (p.nk * 8 + p.nv) {
-    case 8 + 1: return decay_attention_run<T, 1, 1, MODE>(c, p, ws, s);
-    case 8 + 2: return decay_attention_run<T, 1, 2, MODE>(c, p, ws, s);
-    case 8 + 4: return decay_attention_run<T, 1, 4, MODE>(c, p, ws, s);
-    case 16 + 1: return decay_attention_run<T, 2, 1, MODE>(c, p, ws, s);
-    case 16 + 2: return decay_attention_run<T, 2, 2, MODE>(c, p, ws, s);
-    case 16 + 4: return decay_attention_run<T, 2, 4, MODE>(c, p, ws, s);
-    case 32 + 1: return decay_attention_run<T, 4, 1, MODE>(c, p, ws, s);
-    case 32 + 2: return decay_attention_run<T, 4, 2, MODE>(c, p, ws, s);
-    case 32 + 4: return decay_attention_run<T, 4, 4, MODE>(c, p, ws, s);
-    case 64 + 1: return decay_attention_run<T, 8, 1, MODE>(c, p, ws, s);
-    case 64 + 2: return decay_attention_run<T, 8, 2, MODE>(c, p, ws, s);
+    case 8 + 1: return decay_attention_run<T, 1, 1, MODE, false>(c, p, ws, s);
+    case 8 + 2: return decay_attention_run<T, 1, 2, MODE, false>(c, p, ws, s);
+    case 8 + 4: return decay_attention_run<T, 1, 4, MODE, false>(c, p, ws, s);
+    case 16 + 1: return decay_attention_run<T, 2, 1, MODE, false>(c, p, ws, s);
+    case 16 + 2: return decay_attention_run<T, 2, 2, MODE, false>(c, p, ws, s);
+    case 16 + 4: return decay_attention_run<T, 2, 4, MODE, false>(c, p, ws, s);
+    case 32 + 1: return decay_attention_run<T, 4, 1, MODE, false>(c, p, ws, s);
+    case 32 + 2: return decay_attention_run<T, 4, 2, MODE, false>(c, p, ws, s);
+    case 32 + 4: return decay_attention_run<T, 4, 4, MODE, false>(c, p, ws, s);
+    case 64 + 1: return decay_attention_run<T, 8, 1, MODE, false>(c, p, ws, s);
+    case 64 + 2: return decay_attention_run<T, 8, 2, MODE, false>(c, p, ws, s);
   }
   return fail(OIGE_EINVAL, "decay_attention: no variant for %d x %d tiles", p.nk, p.nv);
 }
@@ -643,21 +1090,44 @@ static bool da_wide(const DaCore& c, int bytes) {
          c.on % v == 0 && c.ot % v == 0 && c.oh % v == 0 && aligned16(c.s_in) && aligned16(c.s_out);
 }
 
+template <int MODE>
+static int decay_attention_bf16_tiles(const DaCore& c, const DaPlan& p, float* ws, hipStream_t s) {
+  switch (p.nk * 8 + p.nv) {
+    case 16 + 1: return decay_attention_run<__bf16, 2, 1, MODE, true>(c, p, ws, s);
+    case 16 + 2: return decay_attention_run<__bf16, 2, 2, MODE, true>(c, p, ws, s);
+    case 32 + 1: return decay_attention_run<__bf16, 4, 1, MODE, true>(c, p, ws, s);
+    case 32 + 2: return decay_attention_run<__bf16, 4, 2, MODE, true>(c, p, ws, s);
+    case 64 + 1: return decay_attention_run<__bf16, 8, 1, MODE, true>(c, p, ws, s);
+    case 64 + 2: return decay_attention_run<__bf16, 8, 2, MODE, true>(c, p, ws, s);
+  }
+  return fail(OIGE_EINVAL, "decay_attention: no variant for %d x %d tiles", p.nk, p.nv);
+}
+
 template <typename T>
-static int decay_attention_typed(const DaCore& c, const DaPlan& p, float* ws, hipStream_t s) {
+static int decay_attention_typed(const DaCore& c, float* ws, hipStream_t s) {
+  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, false);
   if (!da_wide(c, sizeof(T))) return decay_attention_tiles<T, ELEMS_SINGLE>(c, p, ws, s);
   if (c.dk == 16 * p.nk && c.dv == 16 * p.nv * p.slices) return decay_attention_tiles<T, ELEMS_FULL>(c, p, ws, s);
   return decay_attention_tiles<T, ELEMS_WIDE>(c, p, ws, s);
+}
+
+// bf16: the kernel of its own where 16-byte accesses are possible and a block of tokens spans less than 2^32 bytes.
+static int decay_attention_bf16(const DaCore& c, float* ws, hipStream_t s) {
+  const int64_t most = (((int64_t)1 << 32) - 1024) / (2 * DB_TOKENS);
+  if (!da_wide(c, 2) || c.q.st > most || c.k.st > most || c.v.st > most)
+    return decay_attention_tiles<__bf16, ELEMS_SINGLE>(c, decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, false), ws, s);
+  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, true);
+  if (c.dk == 16 * p.nk && c.dv == 16 * p.nv * p.slices) return decay_attention_bf16_tiles<ELEMS_FULL>(c, p, ws, s);
+  return decay_attention_bf16_tiles<ELEMS_WIDE>(c, p, ws, s);
 }
 
 static int decay_attention_core(const DaCore& c, int dtype, float* ws, hipStream_t s) {
   const int64_t most = (int64_t)1 << 32;
   OIGE_REQUIRE(c.q.st >= 0 && c.q.st < most && c.k.st >= 0 && c.k.st < most && c.v.st >= 0 && c.v.st < most,
                "decay_attention: token strides must be below 2^32 elements and not negative");
-  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv);
-  if (dtype == OIGE_F32) return decay_attention_typed<float>(c, p, ws, s);
-  if (dtype == OIGE_F16) return decay_attention_typed<_Float16>(c, p, ws, s);
-  return decay_attention_typed<__bf16>(c, p, ws, s);
+  if (dtype == OIGE_F32) return decay_attention_typed<float>(c, ws, s);
+  if (dtype == OIGE_F16) return decay_attention_typed<_Float16>(c, ws, s);
+  return decay_attention_bf16(c, ws, s);
 }
 
 static int decay_attention_share(const float* in, void* out, const oige_decay_attention_io& io, int d, const int64_t* stride, hipStream_t s) {
@@ -689,15 +1159,17 @@ static int decay_attention_check(const oige_decay_attention_io* io, const char* 
   return OIGE_OK;
 }
 
+static int64_t da_seg_floats(const oige_decay_attention_io& io, int dk, int dv) {
+  const int64_t f = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, false).seg_floats;
+  if (io.dtype != OIGE_BF16) return f;
+  const int64_t b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, true).seg_floats;
+  return f > b ? f : b;
+}
 static int64_t da_workspace(const oige_decay_attention_io& io, bool backward) {
-  const int64_t n = io.num_envs, t = io.num_tokens;
-  if (!backward) return decay_attention_plan(n, t, io.heads, io.key_dim, io.value_dim).seg_floats;
-  const int64_t a = decay_attention_plan(n, t, io.heads, io.value_dim, io.key_dim).seg_floats;
-  const int64_t b = decay_attention_plan(n, t, io.heads, io.key_dim, io.value_dim).seg_floats;
-  int64_t most = (a > b ? a : b);
-  most = (most + 3) / 4 * 4;
-  const int64_t d = io.key_dim > io.value_dim ? io.key_dim : io.value_dim;
-  return most + (io.heads != io.kv_heads ? n * t * io.heads * d : 0);  // per query head, dv and then dk
+  if (!backward) return da_seg_floats(io, io.key_dim, io.value_dim);
+  const int64_t a = da_seg_floats(io, io.value_dim, io.key_dim), b = da_seg_floats(io, io.key_dim, io.value_dim);
+  const int64_t most = ((a > b ? a : b) + 3) / 4 * 4, d = io.key_dim > io.value_dim ? io.key_dim : io.value_dim;
+  return most + (io.heads != io.kv_heads ? io.num_envs * io.num_tokens * io.heads * d : 0);  // per query head, dv and then dk
 }
 
 static DaCore da_core(const oige_decay_attention_io& io) {
