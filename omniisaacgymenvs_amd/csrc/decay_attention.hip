@@ -55,6 +55,14 @@ struct DaCore {
   int o_float;     // o is fp32 whatever T is
 };
 
+// Up to three recurrences of one shape over the same sequences in one launch (the backward pass).  A role's workgroups follow each
+// other on the same XCD (workgroup b runs on XCD b mod 8): the rows that the roles share are read from HBM once.
+constexpr int DA_XCDS = 8;
+struct DaRoles {
+  DaCore c[3];
+  int roles;
+};
+
 __device__ __forceinline__ int64_t da_length(const DaCore& c, int64_t n) {
   if (!c.lengths) return c.t;
   const int64_t l = c.lengths_bytes == 8 ? static_cast<const int64_t*>(c.lengths)[n] : static_cast<const int32_t*>(c.lengths)[n];
@@ -228,10 +236,12 @@ struct DaWave {
   int h, seg, slice, dv0;
   bool live;
 };
+__device__ __forceinline__ int da_role(const DaRoles& r) { return (int)(blockIdx.x / DA_XCDS % r.roles); }
 template <int NV>
-__device__ __forceinline__ DaWave da_wave(const DaCore& a) {
+__device__ __forceinline__ DaWave da_wave(const DaCore& a, int roles) {
   DaWave w{};
-  const int64_t u = (int64_t)blockIdx.x * DA_WAVES + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t block = (int64_t)(blockIdx.x / DA_XCDS / roles) * DA_XCDS + blockIdx.x % DA_XCDS;
+  const int64_t u = block * DA_WAVES + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   w.live = u < a.n * a.h * a.slices;
   if (!w.live) return w;
   w.seg = blockIdx.y;
@@ -319,9 +329,10 @@ __device__ __forceinline__ void da_store_out(const f32x4 (&acc)[NV], const DaCor
 // The next block's rows are asked for as soon as the registers of this block's are free: q and the first copy of k behind the
 // products that read them, the other copy and v at the end, so that their way from memory runs beside the matrix instructions.
 template <typename T, int NK, int NV, int MODE, bool STATES>
-__global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(const DaCore a) {
+__global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(const DaRoles roles) {
+  const DaCore a = roles.c[da_role(roles)];  // by value: loaded in a few wide reads, not field by field
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
-  const DaWave w = da_wave<NV>(a);
+  const DaWave w = da_wave<NV>(a, roles.roles);
   if (!w.live) return;
   const int64_t n = w.n, nh = w.nh, len = w.len, begin = w.begin, end = w.end;
   const int h = w.h, seg = w.seg, slice = w.slice, dv0 = w.dv0;
@@ -600,12 +611,14 @@ __device__ __forceinline__ uint32_t db_offset(const DaBlock& b, uint32_t step, u
 }
 
 template <int NK, int NV, int MODE, bool STATES>
-__global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel(const DaCore a) {
+__global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel(const DaRoles roles) {
+  const DaCore a = roles.c[da_role(roles)];  // by value: loaded in a few wide reads, not field by field
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
-  const DaWave w = da_wave<NV>(a);
+  const DaWave w = da_wave<NV>(a, roles.roles);
   if (!w.live) return;
   const int64_t n = w.n, len = w.len, begin = w.begin, end = w.end;
   const int h = w.h, dv0 = w.dv0;
+  __shared__ f32x4 lds_weights[DA_WAVES][4][WAVE];
   const __bf16* qh = static_cast<const __bf16*>(a.q.p) + n * a.q.sn + (int64_t)(h / a.q.group) * a.q.sh;
   const __bf16* kh = static_cast<const __bf16*>(a.k.p) + n * a.k.sn + (int64_t)(h / a.k.group) * a.k.sh;
   const __bf16* vh = static_cast<const __bf16*>(a.v.p) + n * a.v.sn + (int64_t)(h / a.v.group) * a.v.sh;
@@ -615,27 +628,56 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   Bits<NV, MODE> v_run[8];
   bool flag = false;
   const uint32_t qst = (uint32_t)a.q.st, kst = (uint32_t)a.k.st, vst = (uint32_t)a.v.st;
-  const uint32_t q_lane = c * qst, k_lane = c * kst, k_group = 4 * g * kst, v_group = 4 * g * vst;
+  // whole blocks: a lane's offset is the same in each, rows differ by a multiple of the token stride that the scalar base takes;
+  // in reverse token i lies 31 - i rows behind the block's earliest
+  const int rev = a.reverse;
+  const uint32_t q_lane = (rev ? 15 - c : c) * qst, k_lane = (rev ? 15 - c : c) * kst;
+  const uint32_t k_group = (rev ? 12 - 4 * g : 4 * g) * kst, v_group = (rev ? 12 - 4 * g : 4 * g) * vst;
+  const auto row_of = [&](int i) { return rev ? (i < 16 ? 16 : 0) : (i < 16 ? 0 : 16); };            // + 15 - c or c
+  const auto step_of = [&](int e) { return rev ? 3 - (e & 3) + (e < 4 ? 16 : 0) : (e & 3) + (e < 4 ? 0 : 16); };  // + 12 - 4 g or 4 g
   const auto issue_rows = [&](const DaBlock& b) {
     if (STATES) return;
     const __bf16 *q0 = qh + b.low * a.q.st, *k0 = kh + b.low * a.k.st;
+    if (b.L == DB_TOKENS) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      k1_run[i].issue(k0, db_offset(b, k_lane + 16 * i * kst, kst), 4 * NK * g, a.dk);
-      q_run[i].issue(q0, db_offset(b, q_lane + 16 * i * qst, qst), 4 * NK * g, a.dk);
+      for (int i = 0; i < 2; ++i) {
+        k1_run[i].issue(k0 + (int64_t)row_of(16 * i) * kst, k_lane, 4 * NK * g, a.dk);
+        q_run[i].issue(q0 + (int64_t)row_of(16 * i) * qst, q_lane, 4 * NK * g, a.dk);
+      }
+    } else {
+      const int c = da_here(lane) & 15;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        k1_run[i].issue(k0, db_offset(b, (c + 16 * i) * kst, kst), 4 * NK * g, a.dk);
+        q_run[i].issue(q0, db_offset(b, (c + 16 * i) * qst, qst), 4 * NK * g, a.dk);
+      }
     }
   };
   const auto issue_v = [&](const DaBlock& b, bool not_first) {
     const __bf16* v0 = vh + b.low * a.v.st;
+    if (b.L == DB_TOKENS) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v_run[e].issue(v0, db_offset(b, v_group + (uint32_t)(e < 4 ? e : 12 + e) * vst, vst), dv0 + NV * c, a.dv);
-    const int i = lane & 31;
-    if (a.resets) flag = (not_first || !b.reverse || i > 0) && i < b.L && da_reset(a, n, b.low + b.row(i) + b.reverse);
+      for (int e = 0; e < 8; ++e) v_run[e].issue(v0 + (int64_t)step_of(e) * vst, v_group, dv0 + NV * c, a.dv);
+    } else {
+      const int g = da_here(lane) >> 4;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v_run[e].issue(v0, db_offset(b, (uint32_t)(4 * g + (e < 4 ? e : 12 + e)) * vst, vst), dv0 + NV * c, a.dv);
+    }
+    if (a.resets) {
+      const int i = da_here(lane) & 31;
+      flag = (not_first || !b.reverse || i > 0) && i < b.L && da_reset(a, n, b.low + b.row(i) + b.reverse);
+    }
   };
   const auto issue_k = [&](const DaBlock& b) {
     const __bf16* k0 = kh + b.low * a.k.st;
+    if (b.L == DB_TOKENS) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) k2_run[e].issue(k0, db_offset(b, k_group + (uint32_t)(e < 4 ? e : 12 + e) * kst, kst), NK * c, a.dk);
+      for (int e = 0; e < 8; ++e) k2_run[e].issue(k0 + (int64_t)step_of(e) * kst, k_group, NK * c, a.dk);
+    } else {
+      const int g = da_here(lane) >> 4;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k2_run[e].issue(k0, db_offset(b, (uint32_t)(4 * g + (e < 4 ? e : 12 + e)) * kst, kst), NK * c, a.dk);
+    }
   };
 
   DaBlock blk = da_block<DB_TOKENS>(a, begin, end, len);
@@ -651,7 +693,9 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   const double decay = (double)a.decay[h];
   const DaPowers pw(decay);
   bool dropped = false;
-  float head_w[2] = {0.f, 0.f}, pair_w[4], cross_w[4], tail_w[8], keep_hi = 0.f, keep_lo = 0.f;
+  float head_w[2] = {0.f, 0.f}, keep_hi = 0.f, keep_lo = 0.f;
+  // this lane's weights: within 16 tokens, from the first 16 to the last, and the two halves' up to the block's end
+  f32x4* weights = &lds_weights[(threadIdx.x >> 6)][0][lane];
 
   for (int64_t p0 = begin; p0 < end; p0 += DB_TOKENS) {
     const int L = blk.L;
@@ -663,17 +707,18 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
       keep_lo = (float)(keep - (double)keep_hi);  // the rounding of decay^32 would pile up over a long memory
       head_w[0] = pw(c + 1 - first);
       head_w[1] = pw(c + 17 - first);
+      float x[16];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = 4 * g + r;
-        pair_w[r] = j <= c ? pw(c - j) * a.kv_scale : 0.f;
-        cross_w[r] = pw(16 + c - j) * a.kv_scale;
+        x[r] = j <= c ? pw(c - j) * a.kv_scale : 0.f;
+        x[4 + r] = pw(16 + c - j) * a.kv_scale;
+        x[8 + r] = j < L ? pw(L - 1 - j) * a.kv_scale : 0.f;
+        x[12 + r] = j + 16 < L ? pw(L - 17 - j) * a.kv_scale : 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = (e < 4 ? 0 : 12) + 4 * g + e;
-        tail_w[e] = j < L ? pw(L - 1 - j) * a.kv_scale : 0.f;
-      }
+      for (int i = 0; i < 4; ++i) weights[i * WAVE] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+      wave_lds_fence();
     }
     const uint32_t m = (uint32_t)__ballot(flag);  // bit i: a reset in front of the block's token i
     const bool more = p0 + DB_TOKENS < end;
@@ -707,6 +752,8 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
       db_state_part<NK, NV>(acc, S, Q, from_state, head_w);
       __builtin_amdgcn_sched_barrier(0);
       // a masked product may be infinite or NaN: selected away, not multiplied
+      const f32x4 w0 = weights[0], w1 = weights[WAVE];
+      const float pair_w[4] = {w0.x, w0.y, w0.z, w0.w}, cross_w[4] = {w1.x, w1.y, w1.z, w1.w};
       float P[3][4] = {{pt[0].x, pt[0].y, pt[0].z, pt[0].w}, {pt[1].x, pt[1].y, pt[1].z, pt[1].w}, {pt[2].x, pt[2].y, pt[2].z, pt[2].w}};
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -822,6 +869,8 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
       }
     }
     u32x4 vh3[NV], vm3[NV], vl3[NV];
+    const f32x4 w2 = weights[2 * WAVE], w3 = weights[3 * WAVE];
+    const float tail_w[8] = {w2.x, w2.y, w2.z, w2.w, w3.x, w3.y, w3.z, w3.w};
 #pragma unroll
     for (int sv = 0; sv < NV; ++sv) {
       uint32_t hi[4], mid[4], lo[4];
@@ -865,12 +914,13 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
 
 // The states in front of every segment from those at the segments' ends (in place, register order): carry = factor carry + end.
 // Segment 0's end already holds the initial state.  A thread owns four floats of one (sequence, head) over all segments.
-__global__ __launch_bounds__(256) void decay_attention_join_kernel(float* __restrict__ states, const float* __restrict__ factors,
-                                                                   int64_t quads, int64_t per_head, int nseg) {
+__global__ __launch_bounds__(256) void decay_attention_join_kernel(const DaRoles roles, int64_t quads, int64_t per_head, int nseg) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= quads) return;
+  const DaCore& a = roles.c[blockIdx.y];
+  const float* factors = a.seg_factors;
   const int64_t nh = i / per_head, e = i % per_head;
-  f32x4* s = reinterpret_cast<f32x4*>(states) + nh * nseg * per_head + e;
+  f32x4* s = reinterpret_cast<f32x4*>(a.seg_states) + nh * nseg * per_head + e;
   f32x4 carry = s[0];
   constexpr int U = 8;  // ends in flight (they do not depend on the carry, but lie where it goes)
   for (int seg0 = 1; seg0 < nseg; seg0 += U) {
@@ -1009,12 +1059,12 @@ struct DaPlan {
 // joined by one small launch, then every piece by itself.
 constexpr int64_t DA_FEW_WAVES = 1024, DA_WANT_WAVES = 2048, DA_MIN_SEGMENT = 64;
 
-static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, bool bf16) {
+static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, bool bf16, int roles) {
   DaPlan p;
   p.nk = dk <= 16 && !bf16 ? 1 : dk <= 32 ? 2 : dk <= 64 ? 4 : 8;
   p.nv = dv <= 16 ? 1 : (dv <= 32 || p.nk == 8 || bf16) ? 2 : 4;
   p.slices = (dv + 16 * p.nv - 1) / (16 * p.nv);
-  const int64_t waves = n * h * p.slices;
+  const int64_t waves = n * h * p.slices * roles;
   p.nseg = 1;
   p.seg_len = t > 0 ? t : 1;
   if (waves < DA_FEW_WAVES && t >= 2 * DA_MIN_SEGMENT) {
@@ -1029,15 +1079,23 @@ static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, 
 }
 
 template <typename T, int NK, int NV, int MODE, bool BF16>
-static int decay_attention_run(DaCore c, const DaPlan& p, float* workspace, hipStream_t stream) {
-  c.slices = p.slices;
-  c.nseg = p.nseg;
-  c.seg_len = p.seg_len;
-  const int64_t units = c.n * c.h * p.slices, blocks = (units + DA_WAVES - 1) / DA_WAVES;
-  const int64_t per_head = (int64_t)p.slices * NK * NV * WAVE;  // in 16-byte quads
-  OIGE_REQUIRE(blocks < ((int64_t)1 << 31), "decay_attention: %lld sequences x heads are too many for one launch", (long long)(c.n * c.h));
-  void (*states)(DaCore);
-  void (*main)(DaCore);
+static int decay_attention_run(const DaRoles& in, const DaPlan& p, float* workspace, hipStream_t stream) {
+  DaRoles r = in;
+  const int64_t heads = r.c[0].n * r.c[0].h, units = heads * p.slices, groups = ((units + DA_WAVES - 1) / DA_WAVES + DA_XCDS - 1) / DA_XCDS;
+  const int64_t blocks = groups * DA_XCDS * r.roles, per_head = (int64_t)p.slices * NK * NV * WAVE;  // the last in 16-byte quads
+  OIGE_REQUIRE(blocks < ((int64_t)1 << 31), "decay_attention: %lld sequences x heads are too many for one launch", (long long)heads);
+  for (int i = 0; i < r.roles; ++i) {
+    DaCore& c = r.c[i];
+    c.slices = p.slices;
+    c.nseg = p.nseg;
+    c.seg_len = p.seg_len;
+    if (p.nseg > 1) {
+      c.seg_states = workspace + i * p.seg_floats;
+      c.seg_factors = c.seg_states + heads * p.nseg * per_head * 4;
+    }
+  }
+  void (*states)(DaRoles);
+  void (*main)(DaRoles);
   if constexpr (BF16) {
     states = decay_attention_bf16_kernel<NK, NV, MODE, true>;
     main = decay_attention_bf16_kernel<NK, NV, MODE, false>;
@@ -1046,23 +1104,21 @@ static int decay_attention_run(DaCore c, const DaPlan& p, float* workspace, hipS
     main = decay_attention_kernel<T, NK, NV, MODE, false>;
   }
   if (p.nseg > 1) {
-    c.seg_states = workspace;
-    c.seg_factors = workspace + c.n * c.h * p.nseg * per_head * 4;
-    hipLaunchKernelGGL(states, dim3((unsigned)blocks, (unsigned)(p.nseg - 1)), dim3(DA_WAVES * WAVE), 0, stream, c);
+    hipLaunchKernelGGL(states, dim3((unsigned)blocks, (unsigned)(p.nseg - 1)), dim3(DA_WAVES * WAVE), 0, stream, r);
     int rc = check_launch("decay_attention_kernel (states)");
     if (rc) return rc;
-    const int64_t quads = c.n * c.h * per_head;
-    hipLaunchKernelGGL(decay_attention_join_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, c.seg_states, c.seg_factors,
-                       quads, per_head, p.nseg);
+    const int64_t quads = heads * per_head;
+    hipLaunchKernelGGL(decay_attention_join_kernel, dim3((unsigned)((quads + 255) / 256), (unsigned)r.roles), dim3(256), 0, stream, r, quads,
+                       per_head, p.nseg);
     rc = check_launch("decay_attention_join_kernel");
     if (rc) return rc;
   }
-  hipLaunchKernelGGL(main, dim3((unsigned)blocks, (unsigned)p.nseg), dim3(DA_WAVES * WAVE), 0, stream, c);
+  hipLaunchKernelGGL(main, dim3((unsigned)blocks, (unsigned)p.nseg), dim3(DA_WAVES * WAVE), 0, stream, r);
   return check_launch("decay_attention_kernel");
 }
 
 template <typename T, int MODE>
-static int decay_attention_tiles(const DaCore& c, const DaPlan& p, float* ws, hipStream_t s) {
+static int decay_attention_tiles(const DaRoles& c, const DaPlan& p, float* ws, hipStream_t s) {
   switch (p.nk * 8 + p.nv) {
     case 8 + 1: return decay_attention_run<T, 1, 1, MODE, false>(c, p, ws, s);
     case 8 + 2: return decay_attention_run<T, 1, 2, MODE, false>(c, p, ws, s);
@@ -1091,7 +1147,7 @@ static bool da_wide(const DaCore& c, int bytes) {
 }
 
 template <int MODE>
-static int decay_attention_bf16_tiles(const DaCore& c, const DaPlan& p, float* ws, hipStream_t s) {
+static int decay_attention_bf16_tiles(const DaRoles& c, const DaPlan& p, float* ws, hipStream_t s) {
   switch (p.nk * 8 + p.nv) {
     case 16 + 1: return decay_attention_run<__bf16, 2, 1, MODE, true>(c, p, ws, s);
     case 16 + 2: return decay_attention_run<__bf16, 2, 2, MODE, true>(c, p, ws, s);
@@ -1103,31 +1159,31 @@ static int decay_attention_bf16_tiles(const DaCore& c, const DaPlan& p, float* w
   return fail(OIGE_EINVAL, "decay_attention: no variant for %d x %d tiles", p.nk, p.nv);
 }
 
-template <typename T>
-static int decay_attention_typed(const DaCore& c, float* ws, hipStream_t s) {
-  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, false);
-  if (!da_wide(c, sizeof(T))) return decay_attention_tiles<T, ELEMS_SINGLE>(c, p, ws, s);
-  if (c.dk == 16 * p.nk && c.dv == 16 * p.nv * p.slices) return decay_attention_tiles<T, ELEMS_FULL>(c, p, ws, s);
-  return decay_attention_tiles<T, ELEMS_WIDE>(c, p, ws, s);
-}
-
-// bf16: the kernel of its own where 16-byte accesses are possible and a block of tokens spans less than 2^32 bytes.
-static int decay_attention_bf16(const DaCore& c, float* ws, hipStream_t s) {
-  const int64_t most = (((int64_t)1 << 32) - 1024) / (2 * DB_TOKENS);
-  if (!da_wide(c, 2) || c.q.st > most || c.k.st > most || c.v.st > most)
-    return decay_attention_tiles<__bf16, ELEMS_SINGLE>(c, decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, false), ws, s);
-  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, true);
-  if (c.dk == 16 * p.nk && c.dv == 16 * p.nv * p.slices) return decay_attention_bf16_tiles<ELEMS_FULL>(c, p, ws, s);
-  return decay_attention_bf16_tiles<ELEMS_WIDE>(c, p, ws, s);
-}
-
-static int decay_attention_core(const DaCore& c, int dtype, float* ws, hipStream_t s) {
-  const int64_t most = (int64_t)1 << 32;
-  OIGE_REQUIRE(c.q.st >= 0 && c.q.st < most && c.k.st >= 0 && c.k.st < most && c.v.st >= 0 && c.v.st < most,
-               "decay_attention: token strides must be below 2^32 elements and not negative");
-  if (dtype == OIGE_F32) return decay_attention_typed<float>(c, ws, s);
-  if (dtype == OIGE_F16) return decay_attention_typed<_Float16>(c, ws, s);
-  return decay_attention_bf16(c, ws, s);
+// The kernel and the accesses that suit all of the roles, whose head sizes ask for the same tiles.  bf16 tensors have a kernel of
+// their own where 16-byte accesses are possible and a block of tokens spans less than 2^32 bytes.
+static int decay_attention_core(const DaRoles& r, int dtype, float* ws, hipStream_t s) {
+  const int64_t most = (int64_t)1 << 32, most_bf16 = (most - 1024) / (2 * DB_TOKENS);
+  const int bytes = elem_bytes(dtype);
+  bool wide = true, bf16 = dtype == OIGE_BF16;
+  for (int i = 0; i < r.roles; ++i) {
+    const DaCore& c = r.c[i];
+    OIGE_REQUIRE(c.q.st >= 0 && c.q.st < most && c.k.st >= 0 && c.k.st < most && c.v.st >= 0 && c.v.st < most,
+                 "decay_attention: token strides must be below 2^32 elements and not negative");
+    wide = wide && da_wide(c, bytes);
+    bf16 = bf16 && c.q.st <= most_bf16 && c.k.st <= most_bf16 && c.v.st <= most_bf16;
+  }
+  bf16 = bf16 && wide;
+  const DaCore& c = r.c[0];
+  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, bf16, r.roles);
+  bool full = wide;
+  for (int i = 0; i < r.roles; ++i) full = full && r.c[i].dk == 16 * p.nk && r.c[i].dv == 16 * p.nv * p.slices;
+  if (bf16) return full ? decay_attention_bf16_tiles<ELEMS_FULL>(r, p, ws, s) : decay_attention_bf16_tiles<ELEMS_WIDE>(r, p, ws, s);
+  if (dtype == OIGE_BF16) return decay_attention_tiles<__bf16, ELEMS_SINGLE>(r, p, ws, s);
+  if (dtype == OIGE_F16)
+    return full ? decay_attention_tiles<_Float16, ELEMS_FULL>(r, p, ws, s)
+                : wide ? decay_attention_tiles<_Float16, ELEMS_WIDE>(r, p, ws, s) : decay_attention_tiles<_Float16, ELEMS_SINGLE>(r, p, ws, s);
+  return full ? decay_attention_tiles<float, ELEMS_FULL>(r, p, ws, s)
+              : wide ? decay_attention_tiles<float, ELEMS_WIDE>(r, p, ws, s) : decay_attention_tiles<float, ELEMS_SINGLE>(r, p, ws, s);
 }
 
 static int decay_attention_share(const float* in, void* out, const oige_decay_attention_io& io, int d, const int64_t* stride, hipStream_t s) {
@@ -1159,17 +1215,29 @@ static int decay_attention_check(const oige_decay_attention_io* io, const char* 
   return OIGE_OK;
 }
 
-static int64_t da_seg_floats(const oige_decay_attention_io& io, int dk, int dv) {
-  const int64_t f = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, false).seg_floats;
-  if (io.dtype != OIGE_BF16) return f;
-  const int64_t b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, true).seg_floats;
-  return f > b ? f : b;
+// Head sizes that ask for the same tiles in either order: the backward pass is one launch of three roles.
+static bool da_square(const oige_decay_attention_io& io) {
+  bool same = true;
+  for (int bf16 = 0; bf16 < 2; ++bf16) {
+    const DaPlan a = decay_attention_plan(1, 1, 1, io.key_dim, io.value_dim, bf16, 1), b = decay_attention_plan(1, 1, 1, io.value_dim, io.key_dim, bf16, 1);
+    same = same && a.nk == b.nk && a.nv == b.nv && a.slices == b.slices;
+  }
+  return same;
+}
+static int64_t da_seg_floats(const oige_decay_attention_io& io, int dk, int dv, int roles) {
+  const int64_t f = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, false, roles).seg_floats;
+  const int64_t b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, true, roles).seg_floats;
+  return ((f > b && io.dtype == OIGE_BF16) || io.dtype != OIGE_BF16 ? f : b) * roles;
 }
 static int64_t da_workspace(const oige_decay_attention_io& io, bool backward) {
-  if (!backward) return da_seg_floats(io, io.key_dim, io.value_dim);
-  const int64_t a = da_seg_floats(io, io.value_dim, io.key_dim), b = da_seg_floats(io, io.key_dim, io.value_dim);
-  const int64_t most = ((a > b ? a : b) + 3) / 4 * 4, d = io.key_dim > io.value_dim ? io.key_dim : io.value_dim;
-  return most + (io.heads != io.kv_heads ? io.num_envs * io.num_tokens * io.heads * d : 0);  // per query head, dv and then dk
+  if (!backward) return da_seg_floats(io, io.key_dim, io.value_dim, 1);
+  int64_t most = da_seg_floats(io, io.key_dim, io.value_dim, 3);
+  if (!da_square(io)) {
+    const int64_t a = da_seg_floats(io, io.value_dim, io.key_dim, 1), b = da_seg_floats(io, io.key_dim, io.value_dim, 1);
+    most = a > b ? a : b;
+  }
+  most = (most + 3) / 4 * 4;
+  return most + (io.heads != io.kv_heads ? io.num_envs * io.num_tokens * io.heads * (io.key_dim + io.value_dim) : 0);  // rows per query head
 }
 
 static DaCore da_core(const oige_decay_attention_io& io) {
@@ -1226,7 +1294,10 @@ int oige_decay_attention_forward(const oige_decay_attention_io* io, oige_stream_
   c.out_scale = io->scale;
   c.dk = io->key_dim;
   c.dv = io->value_dim;
-  return decay_attention_core(c, io->dtype, io->workspace, (hipStream_t)stream);
+  DaRoles r{};
+  r.c[0] = c;
+  r.roles = 1;
+  return decay_attention_core(r, io->dtype, io->workspace, (hipStream_t)stream);
 }
 
 int oige_decay_attention_backward(const oige_decay_attention_io* io, oige_stream_t stream) {
@@ -1243,62 +1314,67 @@ int oige_decay_attention_backward(const oige_decay_attention_io* io, oige_stream
   const int group = io->heads / io->kv_heads;
   const DaRows q = da_rows(io->q, io->q_stride, 1), k = da_rows(io->k, io->k_stride, group), v = da_rows(io->v, io->v_stride, group),
                d_o = da_rows(io->d_o, io->d_o_stride, 1);
-  DaCore c = da_core(*io);
-  if (io->num_tokens > 0) {  // dq_t = scale S_t do_t
-    c.q = d_o;
-    c.k = v;
-    c.v = k;
-    da_out(c, io->dq, io->dq_stride);
-    c.s_in = io->state_in;
-    c.transposed = 1;
-    c.out_scale = io->scale;
-    c.dk = io->value_dim;
-    c.dv = io->key_dim;
-    rc = decay_attention_core(c, io->dtype, io->workspace, s);
-    if (rc) return rc;
-  }
-  c = da_core(*io);
-  c.reverse = 1;
-  c.s_in = io->d_state_out;
-  c.kv_scale = io->scale;
-  // shared heads: rows per query head in fp32 behind the segments' scratch, then their sums
+  // shared heads: dk and dv per query head in fp32 behind the segments' scratch, then their sums
   const int64_t t = io->num_tokens, h = io->heads;
-  float* wide = nullptr;
+  float *wide_v = nullptr, *wide_k = nullptr;
   if (group > 1) {
-    const int64_t d = io->key_dim > io->value_dim ? io->key_dim : io->value_dim;
-    wide = io->workspace + (need - io->num_envs * t * h * d);
-    c.o_float = 1;
+    wide_v = io->workspace + (need - io->num_envs * t * h * (io->key_dim + io->value_dim));
+    wide_k = wide_v + io->num_envs * t * h * io->value_dim;
   }
-  {  // dv_t = G_t^T k_t, and the initial state's gradient
-    DaCore b = c;
-    b.q = k;
-    b.k = q;
-    b.v = d_o;
-    const int64_t rows[3] = {t * h * io->value_dim, h * io->value_dim, io->value_dim};
-    da_out(b, wide ? wide : io->dv, wide ? rows : io->dv_stride);
-    b.s_out = io->d_state_in;
-    b.dk = io->key_dim;
-    b.dv = io->value_dim;
-    rc = decay_attention_core(b, io->dtype, io->workspace, s);
-    if (rc) return rc;
-    if (wide && t > 0) rc = decay_attention_share(wide, io->dv, *io, io->value_dim, io->dv_stride, s);
-    if (rc) return rc;
+  const int64_t rows_v[3] = {t * h * io->value_dim, h * io->value_dim, io->value_dim}, rows_k[3] = {t * h * io->key_dim, h * io->key_dim, io->key_dim};
+  DaRoles r{};
+  for (int i = 0; i < 3; ++i) {
+    DaCore& c = r.c[i];
+    c = da_core(*io);
+    c.dk = i == 0 ? io->key_dim : io->value_dim;
+    c.dv = i == 0 ? io->value_dim : io->key_dim;
+    if (i < 2) {
+      c.reverse = 1;
+      c.s_in = io->d_state_out;
+      c.kv_scale = io->scale;
+      c.o_float = group > 1;
+    }
   }
-  if (t > 0) {  // dk_t = G_t v_t
-    DaCore b = c;
-    b.q = v;
-    b.k = d_o;
-    b.v = q;
-    const int64_t rows[3] = {t * h * io->key_dim, h * io->key_dim, io->key_dim};
-    da_out(b, wide ? wide : io->dk, wide ? rows : io->dk_stride);
-    b.transposed = 1;
-    b.dk = io->value_dim;
-    b.dv = io->key_dim;
-    rc = decay_attention_core(b, io->dtype, io->workspace, s);
-    if (rc) return rc;
-    if (wide) rc = decay_attention_share(wide, io->dk, *io, io->key_dim, io->dk_stride, s);
+  // dv_t = G_t^T k_t, and the initial state's gradient
+  r.c[0].q = k;
+  r.c[0].k = q;
+  r.c[0].v = d_o;
+  da_out(r.c[0], wide_v ? wide_v : io->dv, wide_v ? rows_v : io->dv_stride);
+  r.c[0].s_out = io->d_state_in;
+  // dk_t = G_t v_t
+  r.c[1].q = v;
+  r.c[1].k = d_o;
+  r.c[1].v = q;
+  da_out(r.c[1], wide_k ? wide_k : io->dk, wide_k ? rows_k : io->dk_stride);
+  r.c[1].transposed = 1;
+  // dq_t = scale S_t do_t
+  r.c[2].q = d_o;
+  r.c[2].k = v;
+  r.c[2].v = k;
+  da_out(r.c[2], io->dq, io->dq_stride);
+  r.c[2].s_in = io->state_in;
+  r.c[2].transposed = 1;
+  r.c[2].out_scale = io->scale;
+  if (t == 0) {
+    r.roles = 1;  // the state's gradient passes through
+    return decay_attention_core(r, io->dtype, io->workspace, s);
   }
-  return rc;
+  if (da_square(*io)) {
+    r.roles = 3;
+    rc = decay_attention_core(r, io->dtype, io->workspace, s);
+    if (rc) return rc;
+  } else {
+    for (int i = 0; i < 3; ++i) {
+      DaRoles one{};
+      one.c[0] = r.c[i];
+      one.roles = 1;
+      rc = decay_attention_core(one, io->dtype, io->workspace, s);
+      if (rc) return rc;
+    }
+  }
+  if (group == 1) return OIGE_OK;
+  rc = decay_attention_share(wide_v, io->dv, *io, io->value_dim, io->dv_stride, s);
+  return rc ? rc : decay_attention_share(wide_k, io->dk, *io, io->key_dim, io->dk_stride, s);
 }
 
 int oige_decay_attention_step(const oige_decay_attention_step_io* io, oige_stream_t stream) {
