@@ -69,9 +69,9 @@ __device__ __forceinline__ int64_t da_length(const DaCore& c, int64_t n) {
   return l < 0 ? 0 : (l > c.t ? c.t : l);
 }
 
-__device__ __forceinline__ bool da_reset(const DaCore& c, int64_t n, int64_t t) {
+__device__ __forceinline__ int64_t da_flag(const DaCore& c, int64_t n, int64_t t) {  // not zero: a reset
   const int64_t i = n * c.rsn + t * c.rst;
-  return c.resets_bytes == 8 ? static_cast<const int64_t*>(c.resets)[i] != 0 : static_cast<const uint8_t*>(c.resets)[i] != 0;
+  return c.resets_bytes == 8 ? static_cast<const int64_t*>(c.resets)[i] : (int64_t)static_cast<const uint8_t*>(c.resets)[i];
 }
 
 // decay^n.  Products of squares in 64 bits: exact where the result is used in 32, also for decays of 0 and above 1.
@@ -208,6 +208,12 @@ struct DaBlock {
     return head + low * st + (uint64_t)(uint32_t)row(i) * (uint32_t)st;
   }
 };
+// The flag that stands between token i of the block and the token taken in before it: its own, or in reverse the next one's (there
+// is none behind the last token: what is read then is not used).
+__device__ __forceinline__ int64_t da_block_flag(const DaCore& a, const DaBlock& b, int64_t n, int i) {
+  const int64_t t = b.low + b.row(i) + b.reverse;
+  return da_flag(a, n, t < a.t ? t : a.t - 1);
+}
 template <int TOKENS>
 __device__ __forceinline__ DaBlock da_block(const DaCore& a, int64_t p0, int64_t end, int64_t len) {
   DaBlock b;
@@ -300,7 +306,7 @@ __device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, co
   }
   if (a.s_out && w.seg == a.nseg - 1) {
     if (a.reverse && w.len > 0) {  // dS_0 = a_0 G_0
-      const bool drop = a.resets && da_reset(a, w.n, 0);
+      const bool drop = a.resets && da_flag(a, w.n, 0) != 0;
 #pragma unroll
       for (int s = 0; s < NK; ++s)
 #pragma unroll
@@ -310,18 +316,30 @@ __device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, co
   }
 }
 
-template <typename T, int NV, int MODE>
-__device__ __forceinline__ void da_store_out(const f32x4 (&acc)[NV], const DaCore& a, int64_t row, int col) {
-  float out[4 * NV];
+// O^T's tiles hold a token's columns in one lane; they leave through LDS, so that 16 lanes store one row side by side.
+template <typename T, int NV, int MODE, int LD>
+__device__ __forceinline__ void da_store_out(float* lds, const f32x4 (&acc)[NV], const DaCore& a, const DaBlock& b, int64_t head, int dv0, int c, int g) {
+  float* mine = lds + c * LD + 4 * NV * g;
 #pragma unroll
   for (int sv = 0; sv < NV; ++sv) {
-    out[sv] = acc[sv].x * a.out_scale;
-    out[NV + sv] = acc[sv].y * a.out_scale;
-    out[2 * NV + sv] = acc[sv].z * a.out_scale;
-    out[3 * NV + sv] = acc[sv].w * a.out_scale;
+    mine[sv] = acc[sv].x * a.out_scale;
+    mine[NV + sv] = acc[sv].y * a.out_scale;
+    mine[2 * NV + sv] = acc[sv].z * a.out_scale;
+    mine[3 * NV + sv] = acc[sv].w * a.out_scale;
   }
-  if (a.o_float) store_run<float, 4 * NV, MODE>(out, static_cast<float*>(a.o) + row, col, a.dv);
-  else store_run<T, 4 * NV, MODE>(out, static_cast<T*>(a.o) + row, col, a.dv);
+  wave_lds_fence();
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float out[NV];
+#pragma unroll
+    for (int sv = 0; sv < NV; ++sv) out[sv] = lds[(4 * g + r) * LD + NV * c + sv];
+    if (4 * g + r < b.L) {
+      const int64_t row = head + (b.low + b.row(4 * g + r)) * a.ot;
+      if (a.o_float) store_run<float, NV, MODE>(out, static_cast<float*>(a.o) + row, dv0 + NV * c, a.dv);
+      else store_run<T, NV, MODE>(out, static_cast<T*>(a.o) + row, dv0 + NV * c, a.dv);
+    }
+  }
+  wave_lds_fence();
 }
 
 // STATES: only the states at the segments' ends (no q, no o), for sequences cut over time.
@@ -341,29 +359,49 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
   const T* kh = static_cast<const T*>(a.k.p) + n * a.k.sn + (int64_t)(h / a.k.group) * a.k.sh;
   const T* vh = static_cast<const T*>(a.v.p) + n * a.v.sn + (int64_t)(h / a.v.group) * a.v.sh;
 
-  Run<T, 4 * NK, MODE> q_run, k1_run;
-  Run<T, NK, MODE> k2_run[4];
+  // Rows come in as 16 lanes read them side by side, 16 or less bytes each: lane (c, g) holds columns NK c .. of tokens 4 g .. 4 g + 3.
+  // That is how the state's product takes k and v; the others take q and k with a token to a lane, by way of LDS.
+  constexpr int LD = 16 * (NK > NV ? NK : NV) + 4;
+  __shared__ __align__(16) float lds_rows[DA_WAVES][DA_TOKENS * LD];
+  float* lds = lds_rows[threadIdx.x >> 6];
+  Run<T, NK, MODE> q_run[4], k_run[4];
   Run<T, NV, MODE> v_run[4];
-  bool flag = false;
-  auto issue_rows = [&](const DaBlock& b) {
-    if (!STATES) {
-      q_run.issue(b.at(qh, a.q.st, c), 4 * NK * g, a.dk);
-      k1_run.issue(b.at(kh, a.k.st, c), 4 * NK * g, a.dk);
-    }
+  int64_t flag = 0;
+  const auto issue_q = [&](const DaBlock& b) {
+    if (STATES) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) q_run[r].issue(b.at(qh, a.q.st, 4 * g + r), NK * c, a.dk);
   };
-  auto issue_columns = [&](const DaBlock& b, bool not_first) {
+  const auto issue_k = [&](const DaBlock& b) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) k_run[r].issue(b.at(kh, a.k.st, 4 * g + r), NK * c, a.dk);
+    if (a.resets) flag = da_block_flag(a, b, n, c);
+  };
+  const auto issue_v = [&](const DaBlock& b) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v_run[r].issue(b.at(vh, a.v.st, 4 * g + r), dv0 + NV * c, a.dv);
+  };
+  const auto put_rows = [&](const Run<T, NK, MODE> (&run)[4]) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      v_run[r].issue(b.at(vh, a.v.st, 4 * g + r), dv0 + NV * c, a.dv);
-      k2_run[r].issue(b.at(kh, a.k.st, 4 * g + r), NK * c, a.dk);
+      float x[NK];
+      run[r].take(x, NK * c, a.dk);
+#pragma unroll
+      for (int s = 0; s < NK; ++s) lds[(4 * g + r) * LD + NK * c + s] = x[s];
     }
-    if (a.resets) flag = (not_first || !b.reverse || c > 0) && c < b.L && da_reset(a, n, b.low + b.row(c) + b.reverse);
+    wave_lds_fence();
+  };
+  const auto get_token = [&](float (&x)[4 * NK]) {
+#pragma unroll
+    for (int e = 0; e < 4 * NK; ++e) x[e] = lds[c * LD + 4 * NK * g + e];
+    wave_lds_fence();
   };
 
   DaBlock blk = da_block<DA_TOKENS>(a, begin, end, len);
   if (begin < end) {
-    issue_rows(blk);
-    issue_columns(blk, begin > 0);
+    issue_q(blk);
+    issue_k(blk);
+    issue_v(blk);
   }
 
   f32x4 S[NK][NV];
@@ -392,16 +430,21 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
         tail_w[r] = j < L ? pw(L - 1 - j) * a.kv_scale : 0.f;
       }
     }
-    const uint32_t m = (uint32_t)(__ballot(flag) & 0xFFFFull);  // bit i: a reset in front of the block's token i
+    // bit i: a reset in front of the block's token i
+    const uint32_t m = a.resets ? (uint32_t)(__ballot(flag != 0 && c < L && !(a.reverse && p0 == 0 && c == 0)) & 0xFFFFull) : 0u;
     const bool more = p0 + DA_TOKENS < end;
     const DaBlock next = da_block<DA_TOKENS>(a, more ? p0 + DA_TOKENS : p0, end, len);  // behind the last block: the same rows once more
 
     f32x4 acc[NV];
-    float V[4][NV];
+    float V[4][NV], K2[4][NK];
     if (!STATES) {
       float Q[4 * NK], K1[4 * NK];
-      q_run.take(Q, 4 * NK * g, a.dk);
-      k1_run.take(K1, 4 * NK * g, a.dk);
+      put_rows(q_run);
+      get_token(Q);
+      issue_q(next);
+      put_rows(k_run);
+      get_token(K1);
+      issue_k(next);
       f32x4 pt = zero;
 #pragma unroll
       for (int e = 0; e < 4 * NK; ++e) pt = __builtin_amdgcn_mfma_f32_16x16x4f32(K1[e], Q[e], pt, 0, 0, 0);
@@ -449,16 +492,20 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
           for (int sv = 0; sv < NV; ++sv) acc[sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[r][sv], P[r], acc[sv], 0, 0, 0);
         da_settle();
       }
-      issue_rows(next);
-      if (c < L) da_store_out<T, NV, MODE>(acc, a, n * a.on + (blk.low + blk.row(c)) * a.ot + (int64_t)h * a.oh, dv0 + 4 * NV * g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int s = 0; s < NK; ++s) K2[r][s] = lds[(4 * g + r) * LD + NK * c + s];
+      wave_lds_fence();
+      da_store_out<T, NV, MODE, LD>(lds, acc, a, blk, n * a.on + (int64_t)h * a.oh, dv0, c, g);
     } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v_run[r].take(V[r], dv0 + NV * c, a.dv);
+      for (int r = 0; r < 4; ++r) {
+        v_run[r].take(V[r], dv0 + NV * c, a.dv);
+        k_run[r].take(K2[r], NK * c, a.dk);
+      }
     }
 
-    float K2[4][NK];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) k2_run[r].take(K2[r], NK * c, a.dk);
     // rows in front of the block's last reset, and behind the end, stay out of the state's sum altogether
     if (m || L < DA_TOKENS) {
       const int g = da_here(lane) >> 4;
@@ -482,7 +529,8 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
 #pragma unroll
         for (int sv = 0; sv < NV; ++sv) S[s][sv] = zero;
     }
-    issue_columns(next, true);
+    if (STATES) issue_k(next);
+    issue_v(next);
 #pragma unroll
     for (int s = 0; s < NK; ++s)
 #pragma unroll
@@ -603,6 +651,45 @@ __device__ __forceinline__ void db_state_part(f32x4 (&acc)[2][NV], const f32x4 (
     for (int sv = 0; sv < NV; ++sv) acc[it][sv] = from_state[it] ? acc[it][sv] * head_w[it] : zero;
 }
 
+// The result's way out, as above; two bf16 to a word.  Rows per query head of shared ones (fp32) go straight from the registers.
+template <int NV, int MODE, int LD>
+__device__ __forceinline__ void db_store_out(uint32_t* lds, const f32x4 (&acc)[2][NV], const DaCore& a, const DaBlock& b, int64_t head, int dv0, int c,
+                                             int g) {
+#pragma unroll
+  for (int it = 0; it < 2; ++it) {
+    float out[4 * NV];
+#pragma unroll
+    for (int sv = 0; sv < NV; ++sv) {
+      out[sv] = acc[it][sv].x * a.out_scale;
+      out[NV + sv] = acc[it][sv].y * a.out_scale;
+      out[2 * NV + sv] = acc[it][sv].z * a.out_scale;
+      out[3 * NV + sv] = acc[it][sv].w * a.out_scale;
+    }
+    const int i = 16 * it + c;
+    if (a.o_float) {
+      if (i < b.L) store_run<float, 4 * NV, MODE>(out, static_cast<float*>(a.o) + head + (b.low + b.row(i)) * a.ot, dv0 + 4 * NV * g, a.dv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2 * NV; ++e) lds[i * LD + 2 * NV * g + e] = db_pack(out[2 * e], out[2 * e + 1]);
+    }
+  }
+  if (a.o_float) return;
+  wave_lds_fence();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int i = (e < 4 ? 0 : 12) + 4 * g + e, col = dv0 + NV * c;
+    uint16_t* row = static_cast<uint16_t*>(a.o) + head + (b.low + b.row(i)) * a.ot;
+    if (NV == 2) {
+      const uint32_t x = lds[i * LD + c];
+      if (i < b.L && (MODE == ELEMS_FULL || col < a.dv)) *reinterpret_cast<uint32_t*>(row + col) = x;
+    } else {
+      const uint16_t x = reinterpret_cast<const uint16_t*>(lds + i * LD)[c];
+      if (i < b.L && (MODE == ELEMS_FULL || col < a.dv)) row[col] = x;
+    }
+  }
+  wave_lds_fence();
+}
+
 // Offset of token `i` of a block of L from its earliest one, in elements of less than 32 bits: `step` = the token stride times i.
 __device__ __forceinline__ uint32_t db_offset(const DaBlock& b, uint32_t step, uint32_t st) {
   const uint32_t last = (uint32_t)(b.L - 1) * st;
@@ -623,68 +710,64 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   const __bf16* kh = static_cast<const __bf16*>(a.k.p) + n * a.k.sn + (int64_t)(h / a.k.group) * a.k.sh;
   const __bf16* vh = static_cast<const __bf16*>(a.v.p) + n * a.v.sn + (int64_t)(h / a.v.group) * a.v.sh;
 
-  Bits<4 * NK, MODE> q_run[2], k1_run[2];
-  Bits<NK, MODE> k2_run[8];
+  // As in the kernel above: lane (c, g) holds columns NK c .. of tokens 4 g + {0..3} and 16 + 4 g + {0..3}, q and the first use of k
+  // take whole tokens by way of LDS.
+  constexpr int LD = 8 * NK + 4;  // in registers' words
+  __shared__ __align__(16) uint32_t lds_rows[DA_WAVES][DB_TOKENS * LD];
+  uint32_t* lds = lds_rows[threadIdx.x >> 6];
+  Bits<NK, MODE> q_run[8], k_run[8];
   Bits<NV, MODE> v_run[8];
-  bool flag = false;
+  int64_t flag = 0;
   const uint32_t qst = (uint32_t)a.q.st, kst = (uint32_t)a.k.st, vst = (uint32_t)a.v.st;
   // whole blocks: a lane's offset is the same in each, rows differ by a multiple of the token stride that the scalar base takes;
   // in reverse token i lies 31 - i rows behind the block's earliest
   const int rev = a.reverse;
-  const uint32_t q_lane = (rev ? 15 - c : c) * qst, k_lane = (rev ? 15 - c : c) * kst;
-  const uint32_t k_group = (rev ? 12 - 4 * g : 4 * g) * kst, v_group = (rev ? 12 - 4 * g : 4 * g) * vst;
-  const auto row_of = [&](int i) { return rev ? (i < 16 ? 16 : 0) : (i < 16 ? 0 : 16); };            // + 15 - c or c
-  const auto step_of = [&](int e) { return rev ? 3 - (e & 3) + (e < 4 ? 16 : 0) : (e & 3) + (e < 4 ? 0 : 16); };  // + 12 - 4 g or 4 g
-  const auto issue_rows = [&](const DaBlock& b) {
-    if (STATES) return;
-    const __bf16 *q0 = qh + b.low * a.q.st, *k0 = kh + b.low * a.k.st;
+  const uint32_t group = rev ? 12 - 4 * g : 4 * g;
+  const uint32_t q_group = group * qst, k_group = group * kst, v_group = group * vst;
+  const auto step_of = [&](int e) { return rev ? 3 - (e & 3) + (e < 4 ? 16 : 0) : (e & 3) + (e < 4 ? 0 : 16); };
+  const auto issue = [&](auto& run, const __bf16* head, int64_t st, uint32_t lane_off, const DaBlock& b, int off, int limit) {
+    const __bf16* base = head + b.low * st;
     if (b.L == DB_TOKENS) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        k1_run[i].issue(k0 + (int64_t)row_of(16 * i) * kst, k_lane, 4 * NK * g, a.dk);
-        q_run[i].issue(q0 + (int64_t)row_of(16 * i) * qst, q_lane, 4 * NK * g, a.dk);
-      }
-    } else {
-      const int c = da_here(lane) & 15;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        k1_run[i].issue(k0, db_offset(b, (c + 16 * i) * kst, kst), 4 * NK * g, a.dk);
-        q_run[i].issue(q0, db_offset(b, (c + 16 * i) * qst, qst), 4 * NK * g, a.dk);
-      }
-    }
-  };
-  const auto issue_v = [&](const DaBlock& b, bool not_first) {
-    const __bf16* v0 = vh + b.low * a.v.st;
-    if (b.L == DB_TOKENS) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v_run[e].issue(v0 + (int64_t)step_of(e) * vst, v_group, dv0 + NV * c, a.dv);
+      for (int e = 0; e < 8; ++e) run[e].issue(base + (int64_t)step_of(e) * st, lane_off, off, limit);
     } else {
       const int g = da_here(lane) >> 4;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v_run[e].issue(v0, db_offset(b, (uint32_t)(4 * g + (e < 4 ? e : 12 + e)) * vst, vst), dv0 + NV * c, a.dv);
+      for (int e = 0; e < 8; ++e) run[e].issue(base, db_offset(b, (uint32_t)(4 * g + (e < 4 ? e : 12 + e)) * (uint32_t)st, (uint32_t)st), off, limit);
     }
-    if (a.resets) {
-      const int i = da_here(lane) & 31;
-      flag = (not_first || !b.reverse || i > 0) && i < b.L && da_reset(a, n, b.low + b.row(i) + b.reverse);
-    }
+  };
+  const auto issue_q = [&](const DaBlock& b) {
+    if (!STATES) issue(q_run, qh, a.q.st, q_group, b, NK * c, a.dk);
   };
   const auto issue_k = [&](const DaBlock& b) {
-    const __bf16* k0 = kh + b.low * a.k.st;
-    if (b.L == DB_TOKENS) {
+    issue(k_run, kh, a.k.st, k_group, b, NK * c, a.dk);
+    if (a.resets) flag = da_block_flag(a, b, n, da_here(lane) & 31);
+  };
+  const auto issue_v = [&](const DaBlock& b) { issue(v_run, vh, a.v.st, v_group, b, dv0 + NV * c, a.dv); };
+  const auto lds_row = [&](int e) { return lds + ((e < 4 ? 0 : 12) + 4 * g + e) * LD; };
+  const auto put_rows = [&](const Bits<NK, MODE> (&run)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) k2_run[e].issue(k0 + (int64_t)step_of(e) * kst, k_group, NK * c, a.dk);
-    } else {
-      const int g = da_here(lane) >> 4;
+    for (int e = 0; e < 8; ++e) {
+      uint32_t x[NK / 2];
+      run[e].take(x, NK * c, a.dk);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) k2_run[e].issue(k0, db_offset(b, (uint32_t)(4 * g + (e < 4 ? e : 12 + e)) * kst, kst), NK * c, a.dk);
+      for (int i = 0; i < NK / 2; ++i) lds_row(e)[NK / 2 * c + i] = x[i];
     }
+    wave_lds_fence();
+  };
+  const auto get_tokens = [&](uint32_t (&x)[2][2 * NK]) {
+#pragma unroll
+    for (int it = 0; it < 2; ++it)
+#pragma unroll
+      for (int i = 0; i < 2 * NK; ++i) x[it][i] = lds[(16 * it + c) * LD + 2 * NK * g + i];
+    wave_lds_fence();
   };
 
   DaBlock blk = da_block<DB_TOKENS>(a, begin, end, len);
   if (begin < end) {
-    issue_rows(blk);
-    issue_v(blk, begin > 0);
+    issue_q(blk);
     issue_k(blk);
+    issue_v(blk);
   }
   f32x4 S[NK][NV];
   const f32x4 zero{0.f, 0.f, 0.f, 0.f};
@@ -720,20 +803,22 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
       for (int i = 0; i < 4; ++i) weights[i * WAVE] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
       wave_lds_fence();
     }
-    const uint32_t m = (uint32_t)__ballot(flag);  // bit i: a reset in front of the block's token i
+    // bit i: a reset in front of the block's token i
+    const uint32_t m = a.resets ? (uint32_t)__ballot(flag != 0 && (lane & 31) < L && !(rev && p0 == 0 && (lane & 31) == 0)) : 0u;
     const bool more = p0 + DB_TOKENS < end;
     const DaBlock next = da_block<DB_TOKENS>(a, more ? p0 + DB_TOKENS : p0, end, len);  // behind the last block: the same rows once more
     const uint32_t upto[2] = {(2u << c) - 1u, (0x20000u << c) - 1u};  // bits 0 .. i for token i = c, 16 + c
 
-    uint32_t V[8][Bits<NV, MODE>::REGS];
+    uint32_t V[8][Bits<NV, MODE>::REGS], K2[8][NK / 2];
     if (!STATES) {
       f32x4 acc[2][NV];
       uint32_t Q[2][2 * NK], K1[2][2 * NK];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        q_run[i].take(Q[i], 4 * NK * g, a.dk);
-        k1_run[i].take(K1[i], 4 * NK * g, a.dk);
-      }
+      put_rows(q_run);
+      get_tokens(Q);
+      issue_q(next);
+      put_rows(k_run);
+      get_tokens(K1);
+      issue_k(next);
       f32x4 pt[3] = {zero, zero, zero};  // P^T: tokens 0-15 for 0-15, 0-15 for 16-31, 16-31 for 16-31
 #pragma unroll
       for (int p = 0; p < NK / 2; ++p) {
@@ -841,20 +926,20 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
         da_settle();
       }
 #pragma unroll
-      for (int it = 0; it < 2; ++it) {
-        const int i = 16 * it + c;
-        if (i < L) da_store_out<__bf16, NV, MODE>(acc[it], a, n * a.on + (blk.low + blk.row(i)) * a.ot + (int64_t)h * a.oh, dv0 + 4 * NV * g);
-      }
-      issue_rows(next);
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < NK / 2; ++i) K2[e][i] = lds_row(e)[NK / 2 * c + i];
+      wave_lds_fence();
+      db_store_out<NV, MODE, LD>(lds, acc, a, blk, n * a.on + (int64_t)h * a.oh, dv0, c, g);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v_run[e].take(V[e], dv0 + NV * c, a.dv);
+      for (int e = 0; e < 8; ++e) {
+        v_run[e].take(V[e], dv0 + NV * c, a.dv);
+        k_run[e].take(K2[e], NK * c, a.dk);
+      }
     }
 
     __builtin_amdgcn_sched_barrier(0);
-    uint32_t K2[8][NK / 2];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) k2_run[e].take(K2[e], NK * c, a.dk);
     // rows in front of the block's last reset, and behind the end, stay out of the state's sum altogether
     if (m || L < DB_TOKENS) {
       const int g = da_here(lane) >> 4;
@@ -890,7 +975,8 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
 #pragma unroll
         for (int sv = 0; sv < NV; ++sv) S[s][sv] = zero;
     }
-    issue_v(next, true);
+    if (STATES) issue_k(next);
+    issue_v(next);
 #pragma unroll
     for (int s = 0; s < NK; ++s) {
       __builtin_amdgcn_sched_barrier(0);
@@ -905,7 +991,6 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
         S[s][sv] = db_mfma(k, vh3[sv], S[s][sv]);
       }
     }
-    issue_k(next);
     da_settle();
     blk = next;
   }
