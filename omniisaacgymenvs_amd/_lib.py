@@ -469,13 +469,14 @@ SIGNATURES = {
     "oige_episode_stats_fold_scratch": (C.c_int64, [C.c_int64]),
     "oige_observer_accumulate": (C.c_int, [C.POINTER(ObserverBatch), _P, _P, _P]),
     "oige_observer_means": (C.c_int, [_P, _P, _P, C.c_int32, C.c_int32, _P]),
-    "oige_layer_norm_forward": (C.c_int, [C.POINTER(LayerNormIo), _P]),
+    # (argument blocks of the next seven: packed bytes or byref of the Structure)
+    "oige_layer_norm_forward": (C.c_int, [_P, _P]),
     "oige_layer_norm_workspace_floats": (C.c_int64, [C.c_int64, C.c_int32]),
-    "oige_layer_norm_backward": (C.c_int, [C.POINTER(LayerNormIo), _P]),
-    "oige_decay_attention_workspace_floats": (C.c_int64, [C.POINTER(DecayAttentionIo), C.c_int32]),
-    "oige_decay_attention_forward": (C.c_int, [C.POINTER(DecayAttentionIo), _P]),
-    "oige_decay_attention_backward": (C.c_int, [C.POINTER(DecayAttentionIo), _P]),
-    "oige_decay_attention_step": (C.c_int, [C.POINTER(DecayAttentionStepIo), _P]),
+    "oige_layer_norm_backward": (C.c_int, [_P, _P]),
+    "oige_decay_attention_workspace_floats": (C.c_int64, [_P, C.c_int32]),
+    "oige_decay_attention_forward": (C.c_int, [_P, _P]),
+    "oige_decay_attention_backward": (C.c_int, [_P, _P]),
+    "oige_decay_attention_step": (C.c_int, [_P, _P]),
     "oige_stream_copy": (C.c_int, [_P, _P, C.c_int64, C.c_int32, _P]),
     "oige_dr_noise_count": (C.c_int, [C.POINTER(NoiseArgs), C.c_int64, _P]),
     "oige_dr_noise_apply": (C.c_int, [C.POINTER(NoiseArgs), C.c_int64, _P]),

@@ -239,9 +239,10 @@ __device__ __forceinline__ f32x4 da_poison(f32x4 x, f32x4 hit) {
 // What a wave works on: a slice of the state's columns of one head of one sequence, over one segment of its tokens.
 struct DaWave {
   int64_t n, nh, len, begin, end;
-  int h, seg, slice, dv0;
+  int h, seg, last, slice, dv0;  // last: the segment that the sequence ends in; those behind it only clear their rows
   bool live;
 };
+__device__ __forceinline__ int da_last_segment(const DaCore& a, int64_t len) { return len > 0 ? (int)((len - 1) / a.seg_len) : 0; }
 __device__ __forceinline__ int da_role(const DaRoles& r) { return (int)(blockIdx.x / DA_XCDS % r.roles); }
 template <int NV>
 __device__ __forceinline__ DaWave da_wave(const DaCore& a, int roles) {
@@ -257,6 +258,7 @@ __device__ __forceinline__ DaWave da_wave(const DaCore& a, int roles) {
   w.n = w.nh / a.h;
   w.dv0 = w.slice * 16 * NV;
   w.len = da_length(a, w.n);
+  w.last = da_last_segment(a, w.len);
   w.begin = (int64_t)w.seg * a.seg_len;
   w.end = w.begin + a.seg_len < w.len ? w.begin + a.seg_len : w.len;
   return w;
@@ -265,7 +267,7 @@ __device__ __forceinline__ DaWave da_wave(const DaCore& a, int roles) {
 // The state in front of the segment's first token ...
 template <int NK, int NV, int MODE, bool STATES>
 __device__ __forceinline__ void da_open(f32x4 (&S)[NK][NV], const DaCore& a, const DaWave& w, int lane) {
-  if (w.seg > 0 && !STATES) {
+  if (w.seg > 0 && w.seg <= w.last && !STATES) {
     const float* slot = a.seg_states + ((w.nh * a.nseg + w.seg) * a.slices + w.slice) * (int64_t)(NK * NV * 4 * WAVE);
 #pragma unroll
     for (int s = 0; s < NK; ++s)
@@ -304,7 +306,7 @@ __device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, co
     if (a.o_float) store_run<float, 4 * NV, MODE>(none, static_cast<float*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
     else store_run<T, 4 * NV, MODE>(none, static_cast<T*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
   }
-  if (a.s_out && w.seg == a.nseg - 1) {
+  if (a.s_out && w.seg == w.last) {
     if (a.reverse && w.len > 0) {  // dS_0 = a_0 G_0
       const bool drop = a.resets && da_flag(a, w.n, 0) != 0;
 #pragma unroll
@@ -351,7 +353,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
   const DaCore a = roles.c[da_role(roles)];  // by value: loaded in a few wide reads, not field by field
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const DaWave w = da_wave<NV>(a, roles.roles);
-  if (!w.live) return;
+  if (!w.live || (STATES && w.seg >= w.last)) return;
   const int64_t n = w.n, nh = w.nh, len = w.len, begin = w.begin, end = w.end;
   const int h = w.h, seg = w.seg, slice = w.slice, dv0 = w.dv0;
 
@@ -411,7 +413,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
   const double decay = (double)a.decay[h];
   const DaPowers pw(decay);
   bool dropped = false;  // a reset inside the segment
-  float head_w = 0.f, pair_w[4], tail_w[4], keep_hi = 0.f, keep_lo = 0.f;
+  float head_w = 0.f, pair_w[4], tail_w[4], keep_hi = 0.f, keep_lo = 0.f, keep_off = 0.f;
   const uint32_t upto = (2u << c) - 1u;  // bits 0 .. i
 
   for (int64_t p0 = begin; p0 < end; p0 += DA_TOKENS) {
@@ -421,7 +423,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
       const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
       const double keep = da_power(decay, L - first);
       keep_hi = (float)keep;
-      keep_lo = (float)(keep - (double)keep_hi);  // the rounding of decay^16 would pile up over a long memory
+      keep_lo = (float)(keep - (double)keep_hi);
       head_w = pw(c + 1 - first);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -522,6 +524,10 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) V[r][sv] *= tail_w[r];
+    // decay^tokens in 32 bits; what its rounding leaves is carried along, or it would pile up over a long memory
+    keep_off += keep_lo;
+    const float kept = keep_hi + keep_off;
+    keep_off -= kept - keep_hi;
     if (m) {  // (a state that is not finite is dropped too: cleared, not multiplied)
       dropped = true;
 #pragma unroll
@@ -535,7 +541,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     for (int s = 0; s < NK; ++s)
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) {
-        S[s][sv] = __builtin_elementwise_fma(S[s][sv], f32x4(keep_hi), S[s][sv] * keep_lo);
+        S[s][sv] *= kept;
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[s][sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(K2[r][s], V[r][sv], S[s][sv], 0, 0, 0);
       }
@@ -702,7 +708,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   const DaCore a = roles.c[da_role(roles)];  // by value: loaded in a few wide reads, not field by field
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const DaWave w = da_wave<NV>(a, roles.roles);
-  if (!w.live) return;
+  if (!w.live || (STATES && w.seg >= w.last)) return;
   const int64_t n = w.n, len = w.len, begin = w.begin, end = w.end;
   const int h = w.h, dv0 = w.dv0;
   __shared__ f32x4 lds_weights[DA_WAVES][4][WAVE];
@@ -776,7 +782,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   const double decay = (double)a.decay[h];
   const DaPowers pw(decay);
   bool dropped = false;
-  float head_w[2] = {0.f, 0.f}, keep_hi = 0.f, keep_lo = 0.f;
+  float head_w[2] = {0.f, 0.f}, keep_hi = 0.f, keep_lo = 0.f, keep_off = 0.f;
   // this lane's weights: within 16 tokens, from the first 16 to the last, and the two halves' up to the block's end
   f32x4* weights = &lds_weights[(threadIdx.x >> 6)][0][lane];
 
@@ -787,7 +793,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
       const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
       const double keep = da_power(decay, L - first);
       keep_hi = (float)keep;
-      keep_lo = (float)(keep - (double)keep_hi);  // the rounding of decay^32 would pile up over a long memory
+      keep_lo = (float)(keep - (double)keep_hi);
       head_w[0] = pw(c + 1 - first);
       head_w[1] = pw(c + 17 - first);
       float x[16];
@@ -968,6 +974,10 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
       vm3[sv] = u32x4{mid[0], mid[1], mid[2], mid[3]};
       vl3[sv] = u32x4{lo[0], lo[1], lo[2], lo[3]};
     }
+    // decay^tokens in 32 bits; what its rounding leaves is carried along, or it would pile up over a long memory
+    keep_off += keep_lo;
+    const float kept = keep_hi + keep_off;
+    keep_off -= kept - keep_hi;
     if (m) {  // (a state that is not finite is dropped too: cleared, not multiplied)
       dropped = true;
 #pragma unroll
@@ -985,7 +995,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
                             : u32x4{db_lows(K2[0][i], K2[1][i]), db_lows(K2[2][i], K2[3][i]), db_lows(K2[4][i], K2[5][i]), db_lows(K2[6][i], K2[7][i])};
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) {
-        S[s][sv] = __builtin_elementwise_fma(S[s][sv], f32x4(keep_hi), S[s][sv] * keep_lo);
+        S[s][sv] *= kept;
         S[s][sv] = db_mfma(k, vl3[sv], S[s][sv]);
         S[s][sv] = db_mfma(k, vm3[sv], S[s][sv]);
         S[s][sv] = db_mfma(k, vh3[sv], S[s][sv]);
@@ -1005,21 +1015,23 @@ __global__ __launch_bounds__(256) void decay_attention_join_kernel(const DaRoles
   const DaCore& a = roles.c[blockIdx.y];
   const float* factors = a.seg_factors;
   const int64_t nh = i / per_head, e = i % per_head;
+  const int last = da_last_segment(a, da_length(a, nh / a.h));
+  if (last == 0) return;
   f32x4* s = reinterpret_cast<f32x4*>(a.seg_states) + nh * nseg * per_head + e;
   f32x4 carry = s[0];
   constexpr int U = 8;  // ends in flight (they do not depend on the carry, but lie where it goes)
-  for (int seg0 = 1; seg0 < nseg; seg0 += U) {
+  for (int seg0 = 1; seg0 <= last; seg0 += U) {
     f32x4 end[U];
     float f[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int seg = seg0 + i < nseg - 1 ? seg0 + i : nseg - 2;  // (the last segment's own end is nobody's start)
+      const int seg = seg0 + i < last ? seg0 + i : last - 1;  // (the last segment's own end is nobody's start)
       end[i] = s[seg * per_head];
       f[i] = factors[nh * nseg + seg];
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      if (seg0 + i >= nseg) break;
+      if (seg0 + i > last) break;
       s[(seg0 + i) * per_head] = carry;
       carry = f[i] < 0.f ? end[i] : __builtin_elementwise_fma(carry, f32x4(f[i]), end[i]);
     }
@@ -1139,21 +1151,33 @@ struct DaPlan {
   int64_t seg_len, seg_floats;  // scratch: states between segments and the segments' factors
 };
 
-// Tiles per wave: 16 NK rows cover dk, 16 NV columns are a slice of dv; at most 16 tiles (64 registers) of state.
+// Tiles per wave: 16 NK rows cover dk, 16 NV columns are a slice of dv; at most 16 tiles (64 registers) of state.  Wider slices share
+// q, k and their product among more columns, narrower ones leave fewer columns empty behind dv: the width with the least
+// matrix instructions over all slices is taken.
+//
 // A call with fewer waves than the chip has SIMDs is cut over time, into pieces of 64 tokens at least: the pieces' end states first,
-// joined by one small launch, then every piece by itself.
+// joined by one small launch, then every piece by itself; the aim is two waves per SIMD, or four where the sequences' lengths
+// differ (long bf16 prompts between a quarter and all of 8192 tokens: 280 us with two, 204 us with four; equal ones no difference).
 constexpr int64_t DA_FEW_WAVES = 1024, DA_WANT_WAVES = 2048, DA_MIN_SEGMENT = 64;
 
-static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, bool bf16, int roles) {
+static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, bool bf16, int roles, bool ragged) {
   DaPlan p;
   p.nk = dk <= 16 && !bf16 ? 1 : dk <= 32 ? 2 : dk <= 64 ? 4 : 8;
-  p.nv = dv <= 16 ? 1 : (dv <= 32 || p.nk == 8 || bf16) ? 2 : 4;
+  p.nv = 1;
+  int64_t least = 0;
+  for (int nv = 1; nv <= (p.nk == 8 || bf16 ? 2 : 4); nv *= 2) {
+    const int64_t slices = (dv + 16 * nv - 1) / (16 * nv), cost = slices * (4 * p.nk + 4 * nv + 8 * p.nk * nv);
+    if (nv == 1 || cost <= least) {
+      least = cost;
+      p.nv = nv;
+    }
+  }
   p.slices = (dv + 16 * p.nv - 1) / (16 * p.nv);
   const int64_t waves = n * h * p.slices * roles;
   p.nseg = 1;
   p.seg_len = t > 0 ? t : 1;
   if (waves < DA_FEW_WAVES && t >= 2 * DA_MIN_SEGMENT) {
-    int64_t want = (DA_WANT_WAVES + waves - 1) / waves;
+    int64_t want = ((ragged ? 2 : 1) * DA_WANT_WAVES + waves - 1) / waves;
     if (want > t / DA_MIN_SEGMENT) want = t / DA_MIN_SEGMENT;
     p.seg_len = (t + want - 1) / want;
     p.seg_len = (p.seg_len + DB_TOKENS - 1) / DB_TOKENS * DB_TOKENS;
@@ -1259,7 +1283,7 @@ static int decay_attention_core(const DaRoles& r, int dtype, float* ws, hipStrea
   }
   bf16 = bf16 && wide;
   const DaCore& c = r.c[0];
-  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, bf16, r.roles);
+  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, bf16, r.roles, c.lengths != nullptr);
   bool full = wide;
   for (int i = 0; i < r.roles; ++i) full = full && r.c[i].dk == 16 * p.nk && r.c[i].dv == 16 * p.nv * p.slices;
   if (bf16) return full ? decay_attention_bf16_tiles<ELEMS_FULL>(r, p, ws, s) : decay_attention_bf16_tiles<ELEMS_WIDE>(r, p, ws, s);
@@ -1304,14 +1328,14 @@ static int decay_attention_check(const oige_decay_attention_io* io, const char* 
 static bool da_square(const oige_decay_attention_io& io) {
   bool same = true;
   for (int bf16 = 0; bf16 < 2; ++bf16) {
-    const DaPlan a = decay_attention_plan(1, 1, 1, io.key_dim, io.value_dim, bf16, 1), b = decay_attention_plan(1, 1, 1, io.value_dim, io.key_dim, bf16, 1);
+    const DaPlan a = decay_attention_plan(1, 1, 1, io.key_dim, io.value_dim, bf16, 1, false), b = decay_attention_plan(1, 1, 1, io.value_dim, io.key_dim, bf16, 1, false);
     same = same && a.nk == b.nk && a.nv == b.nv && a.slices == b.slices;
   }
   return same;
 }
 static int64_t da_seg_floats(const oige_decay_attention_io& io, int dk, int dv, int roles) {
-  const int64_t f = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, false, roles).seg_floats;
-  const int64_t b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, true, roles).seg_floats;
+  const int64_t f = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, false, roles, io.lengths != nullptr).seg_floats;
+  const int64_t b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, true, roles, io.lengths != nullptr).seg_floats;
   return ((f > b && io.dtype == OIGE_BF16) || io.dtype != OIGE_BF16 ? f : b) * roles;
 }
 static int64_t da_workspace(const oige_decay_attention_io& io, bool backward) {

@@ -16,7 +16,8 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Optional, Tuple
+from struct import Struct as _Struct
+from typing import Callable, Optional, Tuple
 
 import torch
 
@@ -26,103 +27,123 @@ MAX_HEAD_DIM = 128
 MAX_WIDTH = 16384
 
 
-def _require(cond: bool, message: str) -> None:
-    if not cond:
-        raise _lib.OigeError(message)
+_TYPES = _lib.ELEM_TYPES
+_FLAGS = (torch.bool, torch.uint8, torch.int64)
+_error = _lib.OigeError
 
 
-def _tensors(what: str, required, optional=()) -> None:
-    for (name, t), needed in [(x, True) for x in required] + [(x, False) for x in optional]:
-        _require(isinstance(t, torch.Tensor) or (t is None and not needed), f"{what}: {name} must be a tensor, got {type(t).__name__}")
+def _packer(struct) -> Callable[..., bytes]:
+    """The fields of an argument block, in order, as its bytes: one pack instead of a ctypes store per field."""
+    fmt, at = "<", 0
+    codes = {C.c_void_p: "Q", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+    for name, kind in struct._fields_:
+        count = 1
+        if issubclass(kind, C.Array):
+            kind, count = kind._type_, kind._length_
+        offset = getattr(struct, name).offset
+        fmt += f"{offset - at}x" * (offset > at) + f"{count}{codes[kind]}"
+        at = offset + getattr(struct, name).size
+    fmt += f"{C.sizeof(struct) - at}x" * (C.sizeof(struct) > at)
+    return _Struct(fmt).pack
 
 
-def _on_device(what: str, device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        _require(t.device.type == "cuda", f"{what}: {name} is on {t.device}; liboige_hip kernels need a ROCm device tensor (no CPU fallback)")
-        _require(t.device == device, f"{what}: {name} is on {t.device}, the other tensors on {device}")
+_pack_norm, _pack_attention, _pack_step = _packer(_lib.LayerNormIo), _packer(_lib.DecayAttentionIo), _packer(_lib.DecayAttentionStepIo)
 
 
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _call(fn: str, io: C.Structure, device: torch.device) -> None:
+def _needs_grad(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _tensors(what: str, required, optional=()) -> None:
+    for name, t in required:
+        if not isinstance(t, torch.Tensor):
+            raise _error(f"{what}: {name} must be a tensor, got {type(t).__name__}")
+    for name, t in optional:
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise _error(f"{what}: {name} must be a tensor, got {type(t).__name__}")
+
+
+def _on_device(what: str, device: torch.device, named) -> None:
+    if device.type != "cuda":
+        raise _error(f"{what}: tensors are on {device}; liboige_hip kernels need ROCm device tensors (no CPU fallback)")
+    for name, t in named:
+        if t is not None and t.device != device:
+            raise _error(f"{what}: {name} is on {t.device}, the other tensors on {device}")
+
+
+def _call(fn: str, block: bytes, device: torch.device) -> None:
     lib = _lib.load()
-    if device.index is not None and device.index != torch.cuda.current_device():
+    if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            rc = getattr(lib, fn)(C.byref(io), _lib.current_stream(device))
+            rc = getattr(lib, fn)(block, _lib.current_stream(device))
     else:
-        rc = getattr(lib, fn)(C.byref(io), _lib.current_stream(device))
-    _lib.check(rc, fn)
+        rc = getattr(lib, fn)(block, _lib.current_stream(device))
+    if rc:
+        _lib.check(rc, fn)
 
 
 # ------------------------------------------------------------------------------------------------ layer norm
-def _norm_io(x2: torch.Tensor, weight, bias, eps: float) -> _lib.LayerNormIo:
-    io = _lib.LayerNormIo()
-    io.x, io.weight, io.bias = x2.data_ptr(), _ptr(weight), _ptr(bias)
-    io.rows, io.width = x2.shape
-    io.x_row_stride = x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
-    io.dtype = _lib.ELEM_TYPES[x2.dtype]
-    param = weight if weight is not None else bias
-    io.weight_dtype = _lib.ELEM_TYPES[param.dtype] if param is not None else io.dtype
-    io.eps = eps
-    return io
-
-
 def _rows_of(x: torch.Tensor) -> torch.Tensor:
     """(rows, width) with a contiguous last axis: a view wherever the leading axes collapse into one stride."""
-    return _last_contiguous(x.reshape(-1, x.shape[-1]))
+    return _last_contiguous(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+
+
+def _norm_forward(x, weight, bias, eps, keep):
+    x2 = _rows_of(x)
+    rows, width = x2.shape
+    dtype = x2.dtype
+    y = torch.empty(x.shape, dtype=dtype, device=x.device)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
+    at = _ptr(stats)
+    param = weight if weight is not None else bias
+    _call("oige_layer_norm_forward", _pack_norm(
+        x2.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), at, at and at + 4 * rows, 0, 0, 0, 0, 0,
+        0, rows, x2.stride(0) if rows > 1 else width, 0, width, _TYPES[dtype], _TYPES[dtype if param is None else param.dtype], eps), x.device)
+    return y, x2, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x2 = _rows_of(x)
-        keep = any(ctx.needs_input_grad)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        io = _norm_io(x2, weight, bias, eps)
-        io.y = y.data_ptr()
-        stats = torch.empty((2, x2.shape[0]), dtype=torch.float32, device=x.device) if keep else None
-        if keep:
-            io.mean, io.rstd = stats.data_ptr(), stats.data_ptr() + 4 * x2.shape[0]
-        _call("oige_layer_norm_forward", io, x.device)
-        if keep:
-            ctx.save_for_backward(x2, weight, bias, stats)
-            ctx.eps, ctx.shape = eps, x.shape
+        y, x2, stats = _norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x2, weight, bias, stats)
+        ctx.eps, ctx.shape = eps, x.shape
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x2, weight, bias, stats = ctx.saved_tensors
-        dx, dw, db = _layer_norm_backward(x2, weight, bias, stats, dy, ctx.eps, ctx.needs_input_grad)
-        return (dx.view(ctx.shape) if dx is not None else None), dw, db, None
-
-
-def _layer_norm_backward(x2, weight, bias, stats, dy, eps, needs):
-    dy2 = _rows_of(dy)
-    rows, width = x2.shape
-    io = _norm_io(x2, weight, bias, eps)
-    io.mean, io.rstd = stats.data_ptr(), stats.data_ptr() + 4 * rows
-    io.dy, io.dy_row_stride = dy2.data_ptr(), dy2.stride(0) if rows > 1 else width
-    dx = torch.empty((rows, width), dtype=x2.dtype, device=x2.device) if needs[0] else None
-    dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if weight is not None and needs[1] else None
-    db = torch.empty_like(bias, memory_format=torch.contiguous_format) if bias is not None and needs[2] else None
-    io.dx, io.dweight, io.dbias = _ptr(dx), _ptr(dw), _ptr(db)
-    ws = None
-    if (dw is not None or db is not None) and rows:
-        size = _lib.load().oige_layer_norm_workspace_floats(rows, width)
-        ws = torch.empty(size, dtype=torch.float32, device=x2.device)
-        io.workspace, io.workspace_floats = ws.data_ptr(), size
-    if io.dx or io.dweight or io.dbias:
-        _call("oige_layer_norm_backward", io, x2.device)
-    return dx, dw, db
+        needs = ctx.needs_input_grad
+        device, dtype = x2.device, x2.dtype
+        rows, width = x2.shape
+        dy2 = _rows_of(dy)
+        dx = torch.empty((rows, width), dtype=dtype, device=device) if needs[0] else None
+        dw = torch.empty(width, dtype=weight.dtype, device=device) if needs[1] else None
+        db = torch.empty(width, dtype=bias.dtype, device=device) if needs[2] else None
+        ws, size = None, 0
+        if rows and (needs[1] or needs[2]):
+            size = _lib.load().oige_layer_norm_workspace_floats(rows, width)
+            ws = torch.empty(size, dtype=torch.float32, device=device)
+        param = weight if weight is not None else bias
+        at = stats.data_ptr()
+        _call("oige_layer_norm_backward", _pack_norm(
+            x2.data_ptr(), _ptr(weight), _ptr(bias), 0, at, at + 4 * rows, dy2.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
+            size, rows, x2.stride(0) if rows > 1 else width, dy2.stride(0) if rows > 1 else width, width,
+            _TYPES[dtype], _TYPES[dtype if param is None else param.dtype], ctx.eps), device)
+        return (dx.view(ctx.shape) if needs[0] else None), dw, db, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -132,124 +153,132 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     ``weight`` and ``bias`` are (width,) of x's type or both fp32 (either may be None); the result has x's shape and type and is
     contiguous.  Differentiable once in x, weight and bias; the parameters' gradients are sums in a fixed order."""
     _tensors("layer_norm", (("x", x),), (("weight", weight), ("bias", bias)))
-    _require(x.dtype in _lib.ELEM_TYPES, f"layer_norm: x is {x.dtype}; float32, float16 and bfloat16 are supported")
-    _require(x.dim() >= 1 and 1 <= x.shape[-1] <= MAX_WIDTH, f"layer_norm: x of shape {tuple(x.shape)} needs a last axis of 1 to {MAX_WIDTH}")
+    dtype = x.dtype
+    if dtype not in _TYPES:
+        raise _error(f"layer_norm: x is {dtype}; float32, float16 and bfloat16 are supported")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
+        raise _error(f"layer_norm: x of shape {tuple(x.shape)} needs a last axis of 1 to {MAX_WIDTH}")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None:
-            _require(p.dtype in (x.dtype, torch.float32), f"layer_norm: {name} is {p.dtype}, expected {x.dtype} or float32")
-            _require(tuple(p.shape) == (x.shape[-1],), f"layer_norm: {name} has shape {tuple(p.shape)}, expected {(x.shape[-1],)}")
-    if weight is not None and bias is not None:
-        _require(weight.dtype == bias.dtype, f"layer_norm: weight is {weight.dtype} and bias {bias.dtype}; they need one type")
-    _require(math.isfinite(eps) and eps >= 0, f"layer_norm: eps = {eps}")
-    _on_device("layer_norm", x.device, x=x, weight=weight, bias=bias)
-    return _LayerNorm.apply(x, None if weight is None else _last_contiguous(weight), None if bias is None else _last_contiguous(bias), float(eps))
+            if p.dtype is not dtype and p.dtype is not torch.float32:
+                raise _error(f"layer_norm: {name} is {p.dtype}, expected {dtype} or torch.float32")
+            if p.dim() != 1 or p.shape[0] != x.shape[-1]:
+                raise _error(f"layer_norm: {name} has shape {tuple(p.shape)}, expected {(x.shape[-1],)}")
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
+        raise _error(f"layer_norm: weight is {weight.dtype} and bias {bias.dtype}; they need one type")
+    eps = float(eps)
+    if not (math.isfinite(eps) and eps >= 0):
+        raise _error(f"layer_norm: eps = {eps}")
+    _on_device("layer_norm", x.device, (("weight", weight), ("bias", bias)))
+    weight = None if weight is None else _last_contiguous(weight)
+    bias = None if bias is None else _last_contiguous(bias)
+    if _needs_grad(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return _norm_forward(x, weight, bias, eps, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ decay attention
-def _like(x: torch.Tensor, heads: int, d: int, dtype=None) -> torch.Tensor:
+def _like(x: torch.Tensor, heads: int, d: int) -> torch.Tensor:
     """(N, T, heads, d), in memory in x's order of the first two axes (a rollout stored time first stays so)."""
     n, t = x.shape[:2]
     if n > 1 and t > 1 and x.stride(0) < x.stride(1):
-        return torch.empty((t, n, heads, d), dtype=dtype or x.dtype, device=x.device).transpose(0, 1)
-    return torch.empty((n, t, heads, d), dtype=dtype or x.dtype, device=x.device)
+        return torch.empty((t, n, heads, d), dtype=x.dtype, device=x.device).transpose(0, 1)
+    return torch.empty((n, t, heads, d), dtype=x.dtype, device=x.device)
 
 
-def _check_flags(what, resets, shape):
-    if resets is None:
-        return
-    _require(resets.dtype in (torch.bool, torch.uint8, torch.int64), f"{what}: resets is {resets.dtype}; bool, uint8 and int64 are supported")
-    _require(tuple(resets.shape) == shape, f"{what}: resets has shape {tuple(resets.shape)}, expected {shape}")
-
-
-def _check_heads(what, q, k, v, decay, state, lead):
-    """Shapes and types of the tensors both forms share; ``lead`` = the axes in front of (heads, d)."""
-    _require(q.dtype in _lib.ELEM_TYPES, f"{what}: q is {q.dtype}; float32, float16 and bfloat16 are supported")
-    nl = len(lead)
+def _check_heads(what, q, k, v, decay, state, resets, lead):
+    """Shapes and types of the tensors both forms share; ``lead`` = the number of axes in front of (heads, d)."""
+    dtype = q.dtype
+    if dtype not in _TYPES:
+        raise _error(f"{what}: q is {dtype}; float32, float16 and bfloat16 are supported")
     for name, t in (("q", q), ("k", k), ("v", v)):
-        _require(t.dim() == nl + 2, f"{what}: {name} has {t.dim()} axes, expected {lead + ('heads', 'd')}")
-        _require(t.dtype == q.dtype, f"{what}: {name} is {t.dtype}, q is {q.dtype}")
-        _require(t.shape[:nl] == q.shape[:nl], f"{what}: {name} has shape {tuple(t.shape)}, q {tuple(q.shape)}")
-        _require(1 <= t.shape[-1] <= MAX_HEAD_DIM, f"{what}: head size {t.shape[-1]} of {name} (1 to {MAX_HEAD_DIM})")
-    h, hk = q.shape[nl], k.shape[nl]
-    _require(v.shape[nl] == hk and k.shape[-1] == q.shape[-1], f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match")
-    _require(h >= 1 and hk >= 1 and h % hk == 0, f"{what}: {h} heads over {hk} key / value heads")
-    _require(decay.dtype == torch.float32 and tuple(decay.shape) == (h,), f"{what}: decay must be float32 of shape {(h,)}, got {decay.dtype} {tuple(decay.shape)}")
-    _require(not decay.requires_grad, f"{what}: decay is a constant of the head, it has no gradient")
-    if state is not None:
-        want = (q.shape[0], h, q.shape[-1], v.shape[-1])
-        _require(state.dtype == torch.float32 and tuple(state.shape) == want,
-                 f"{what}: state must be float32 of shape {want}, got {state.dtype} {tuple(state.shape)}")
-
-
-def _attention_io(q, k, v, decay, state, resets, lengths, scale) -> _lib.DecayAttentionIo:
-    io = _lib.DecayAttentionIo()
-    io.q, io.k, io.v, io.decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr()
-    io.q_stride[:], io.k_stride[:], io.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    io.state_in = _ptr(state)
+        if t.dim() != lead + 2:
+            raise _error(f"{what}: {name} has {t.dim()} axes, expected {('N', 'T')[:lead] + ('heads', 'd')}")
+        if t.dtype is not dtype:
+            raise _error(f"{what}: {name} is {t.dtype}, q is {dtype}")
+        if not 1 <= t.shape[-1] <= MAX_HEAD_DIM:
+            raise _error(f"{what}: head size {t.shape[-1]} of {name} (1 to {MAX_HEAD_DIM})")
+    qs, ks, vs = q.shape, k.shape, v.shape
+    for name, shape in (("k", ks), ("v", vs)):
+        if shape[:lead] != qs[:lead]:
+            raise _error(f"{what}: {name} has shape {tuple(shape)}, q {tuple(qs)}")
+    h, hk = qs[lead], ks[lead]
+    if vs[lead] != hk or ks[-1] != qs[-1]:
+        raise _error(f"{what}: q {tuple(qs)}, k {tuple(ks)}, v {tuple(vs)} do not match")
+    if h < 1 or hk < 1 or h % hk:
+        raise _error(f"{what}: {h} heads over {hk} key / value heads")
+    if decay.dtype is not torch.float32 or decay.dim() != 1 or decay.shape[0] != h:
+        raise _error(f"{what}: decay must be float32 of shape {(h,)}, got {decay.dtype} {tuple(decay.shape)}")
+    if decay.requires_grad:
+        raise _error(f"{what}: decay is a constant of the head, it has no gradient")
+    if state is not None and (state.dtype is not torch.float32 or state.shape != (qs[0], h, qs[-1], vs[-1])):
+        raise _error(f"{what}: state must be float32 of shape {(qs[0], h, qs[-1], vs[-1])}, got {state.dtype} {tuple(state.shape)}")
     if resets is not None:
-        io.resets, io.resets_bytes, io.resets_stride[:] = resets.data_ptr(), resets.element_size(), resets.stride()
-    if lengths is not None:
-        io.lengths, io.lengths_bytes = lengths.data_ptr(), lengths.element_size()
-    io.num_envs, io.num_tokens, io.heads, io.key_dim = q.shape
-    io.kv_heads, io.value_dim = v.shape[2], v.shape[3]
-    io.dtype, io.scale = _lib.ELEM_TYPES[q.dtype], scale
-    return io
+        if resets.dtype not in _FLAGS:
+            raise _error(f"{what}: resets is {resets.dtype}; bool, uint8 and int64 are supported")
+        if resets.shape != qs[:lead]:
+            raise _error(f"{what}: resets has shape {tuple(resets.shape)}, expected {tuple(qs[:lead])}")
 
 
-def _workspace(io: _lib.DecayAttentionIo, backward: bool, device) -> Optional[torch.Tensor]:
-    size = _lib.load().oige_decay_attention_workspace_floats(C.byref(io), int(backward))
-    if size < 0:
-        _lib.check(int(size), "oige_decay_attention_workspace_floats")
-    if size == 0:
-        return None
-    ws = torch.empty(size, dtype=torch.float32, device=device)
-    io.workspace, io.workspace_floats = ws.data_ptr(), size
-    return ws
+_NO3, _NO2 = (0, 0, 0), (0, 0)
+
+
+def _attention(fn, q, k, v, decay, state, resets, lengths, scale, o=None, state_out=None, d_o=None, d_state=None, dq=None, dk=None, dv=None,
+               d_state_in=None):
+    """Fill the argument block, give the call its workspace and make it."""
+    n, t, h, key_dim = q.shape
+    stride = lambda x: _NO3 if x is None else x.stride()[:3]
+
+    def block(ws, size):
+        return _pack_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(o), decay.data_ptr(), _ptr(state), _ptr(state_out), _ptr(resets), _ptr(lengths),
+            _ptr(d_o), _ptr(d_state), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(d_state_in), ws, size,
+            *stride(q), *stride(k), *stride(v), *stride(o), *stride(d_o), *stride(dq), *stride(dk), *stride(dv),
+            *(_NO2 if resets is None else resets.stride()), n, t, h, v.shape[2], key_dim, v.shape[3], _TYPES[q.dtype],
+            0 if resets is None else resets.element_size(), 0 if lengths is None else lengths.element_size(), scale)
+
+    call = block(0, 0)
+    size = _lib.load().oige_decay_attention_workspace_floats(call, o is None)
+    if size:
+        if size < 0:
+            _lib.check(int(size), "oige_decay_attention_workspace_floats")
+        ws = torch.empty(size, dtype=torch.float32, device=q.device)
+        call = block(ws.data_ptr(), size)
+    _call(fn, call, q.device)
+
+
+def _attention_forward(q, k, v, state, decay, resets, lengths, scale, return_state):
+    n, t, h, dk = q.shape
+    dv = v.shape[3]
+    o = _like(q, h, dv)
+    state_out = torch.empty((n, h, dk, dv), dtype=torch.float32, device=q.device) if return_state else None
+    if n and (t or return_state):
+        _attention("oige_decay_attention_forward", q, k, v, decay, state, resets, lengths, scale, o=o, state_out=state_out)
+    return o, state_out
 
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, state, decay, resets, lengths, scale, return_state):
         ctx.set_materialize_grads(False)
-        n, t, h, dk = q.shape
-        dv = v.shape[3]
-        io = _attention_io(q, k, v, decay, state, resets, lengths, scale)
-        o = _like(q, h, dv)
-        io.o, io.o_stride[:] = o.data_ptr(), o.stride()[:3]
-        state_out = torch.empty((n, h, dk, dv), dtype=torch.float32, device=q.device) if return_state else None
-        io.state_out = _ptr(state_out)
-        if n and (t or return_state):
-            ws = _workspace(io, False, q.device)  # noqa: F841 (kept alive over the launch)
-            _call("oige_decay_attention_forward", io, q.device)
-        if any(ctx.needs_input_grad):
-            ctx.save_for_backward(q, k, v, state, decay, resets, lengths)
-            ctx.scale = scale
-        return o, state_out
+        ctx.save_for_backward(q, k, v, state, decay, resets, lengths)
+        ctx.scale = scale
+        return _attention_forward(q, k, v, state, decay, resets, lengths, scale, return_state)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_state):
         q, k, v, state, decay, resets, lengths = ctx.saved_tensors
-        return (*_decay_attention_backward(q, k, v, decay, state, resets, lengths, ctx.scale, d_o, d_state,
-                                           state is not None and ctx.needs_input_grad[3]), None, None, None, None, None)
-
-
-def _decay_attention_backward(q, k, v, decay, state, resets, lengths, scale, d_o, d_state, state_grad):
-    n, t, h, dk = q.shape
-    hk, dv = v.shape[2:]
-    d_o = q.new_zeros((n, t, h, dv)) if d_o is None else _last_contiguous(d_o)
-    d_state = None if d_state is None else d_state.contiguous()
-    io = _attention_io(q, k, v, decay, state, resets, lengths, scale)
-    io.d_o, io.d_o_stride[:], io.d_state_out = d_o.data_ptr(), d_o.stride()[:3], _ptr(d_state)
-    dq, dk_, dv_ = _like(q, h, dk), _like(k, hk, dk), _like(v, hk, dv)
-    io.dq, io.dk, io.dv = dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr()
-    io.dq_stride[:], io.dk_stride[:], io.dv_stride[:] = dq.stride()[:3], dk_.stride()[:3], dv_.stride()[:3]
-    ds = torch.empty_like(state) if state_grad else None
-    io.d_state_in = _ptr(ds)
-    if n and (t or state_grad):
-        ws = _workspace(io, True, q.device)  # noqa: F841
-        _call("oige_decay_attention_backward", io, q.device)
-    return dq, dk_, dv_, ds
+        n, t, h, dk = q.shape
+        hk, dv = v.shape[2:]
+        d_o = q.new_zeros((n, t, h, dv)) if d_o is None else _last_contiguous(d_o)
+        d_state = None if d_state is None else d_state.contiguous()
+        dq, dk_, dv_ = _like(q, h, dk), _like(k, hk, dk), _like(v, hk, dv)
+        ds = torch.empty_like(state) if ctx.needs_input_grad[3] else None
+        if n and (t or ds is not None):
+            _attention("oige_decay_attention_backward", q, k, v, decay, state, resets, lengths, ctx.scale, d_o=d_o, d_state=d_state, dq=dq,
+                       dk=dk_, dv=dv_, d_state_in=ds)
+        return dq, dk_, dv_, ds, None, None, None, None, None
 
 
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, state: Optional[torch.Tensor] = None,
@@ -265,23 +294,23 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     ``state`` (N, heads, key_dim, value_dim) float32 is S before the first token (None: zeros).  A reset clears the state before
     its token is taken in: the flag belongs to the first token of an episode.  ``lengths`` (N,) int32 / int64 ends sequence n
     before token lengths[n] (clamped to 0 .. T); rows behind the end are zero in the result and in the gradients and may hold
-    anything.  ``scale`` defaults to key_dim ** -0.5.
+    anything.  ``scale`` defaults to key_dim ** -0.5.  An infinite or NaN value makes the results that depend on it NaN or
+    infinite, and no others.
 
     Returns ``(o, state)``: o (N, T, heads, value_dim) of q's type, and S behind every sequence's last token (None with
     ``return_state=False``).  Differentiable once in q, k, v and state; the backward pass recomputes the states."""
     what = "decay_attention"
     _tensors(what, (("q", q), ("k", k), ("v", v), ("decay", decay)), (("state", state), ("resets", resets), ("lengths", lengths)))
-    _require(q.dim() == 4, f"{what}: q has {q.dim()} axes, expected (N, T, heads, key_dim)")
-    _check_heads(what, q, k, v, decay, state, ("N", "T"))
-    _check_flags(what, resets, tuple(q.shape[:2]))
-    if lengths is not None:
-        _require(lengths.dtype in (torch.int32, torch.int64) and tuple(lengths.shape) == (q.shape[0],),
-                 f"{what}: lengths must be int32 or int64 of shape {(q.shape[0],)}, got {lengths.dtype} {tuple(lengths.shape)}")
+    _check_heads(what, q, k, v, decay, state, resets, 2)
+    if lengths is not None and (lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != q.shape[:1]):
+        raise _error(f"{what}: lengths must be int32 or int64 of shape {(q.shape[0],)}, got {lengths.dtype} {tuple(lengths.shape)}")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    _require(math.isfinite(scale), f"{what}: scale = {scale}")
-    _on_device(what, q.device, q=q, k=k, v=v, decay=decay, state=state, resets=resets, lengths=lengths)
-    return _DecayAttention.apply(_last_contiguous(q), _last_contiguous(k), _last_contiguous(v), None if state is None else state.contiguous(),
-                                 decay.contiguous(), resets, None if lengths is None else lengths.contiguous(), scale, bool(return_state))
+    if not math.isfinite(scale):
+        raise _error(f"{what}: scale = {scale}")
+    _on_device(what, q.device, (("k", k), ("v", v), ("decay", decay), ("state", state), ("resets", resets), ("lengths", lengths)))
+    args = (_last_contiguous(q), _last_contiguous(k), _last_contiguous(v), None if state is None else state.contiguous(), decay.contiguous(),
+            resets, None if lengths is None else lengths.contiguous(), scale, bool(return_state))
+    return _DecayAttention.apply(*args) if _needs_grad(q, k, v, state) else _attention_forward(*args)
 
 
 def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
@@ -291,27 +320,26 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, deca
     is a task's ``reset_buf`` as it is after ``env.step``: flagged envs start from an empty state.  Not differentiable."""
     what = "decay_attention_step"
     _tensors(what, (("q", q), ("k", k), ("v", v), ("decay", decay), ("state", state)), (("resets", resets),))
-    _require(q.dim() == 3, f"{what}: q has {q.dim()} axes, expected (N, heads, key_dim)")
-    _check_heads(what, q, k, v, decay, state, ("N",))
-    _check_flags(what, resets, (q.shape[0],))
-    _require(state.is_contiguous(), f"{what}: state is updated in place and must be contiguous")
-    _require(not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad)),
-             f"{what}: updates the state in place and has no gradient; use decay_attention, or torch.no_grad()")
+    _check_heads(what, q, k, v, decay, state, resets, 1)
+    if not state.is_contiguous():
+        raise _error(f"{what}: state is updated in place and must be contiguous")
+    if _needs_grad(q, k, v, state):
+        raise _error(f"{what}: updates the state in place and has no gradient; use decay_attention, or torch.no_grad()")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    _require(math.isfinite(scale), f"{what}: scale = {scale}")
-    _on_device(what, q.device, q=q, k=k, v=v, decay=decay, state=state, resets=resets)
+    if not math.isfinite(scale):
+        raise _error(f"{what}: scale = {scale}")
+    device = q.device
+    _on_device(what, device, (("k", k), ("v", v), ("decay", decay), ("state", state), ("resets", resets)))
     q, k, v, decay = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v), decay.contiguous()
     n, h, dk = q.shape
-    o = torch.empty((n, h, v.shape[2]), dtype=q.dtype, device=q.device)
-    io = _lib.DecayAttentionStepIo()
-    io.q, io.k, io.v, io.o, io.state, io.decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), state.data_ptr(), decay.data_ptr()
-    io.q_stride[:], io.k_stride[:], io.v_stride[:] = q.stride()[:2], k.stride()[:2], v.stride()[:2]
-    if resets is not None:
-        io.resets, io.resets_bytes, io.resets_stride = resets.data_ptr(), resets.element_size(), resets.stride(0)
-    io.num_envs, io.heads, io.kv_heads, io.key_dim, io.value_dim = n, h, k.shape[1], dk, v.shape[2]
-    io.dtype, io.scale = _lib.ELEM_TYPES[q.dtype], scale
+    hk, dv = v.shape[1:]
+    o = torch.empty((n, h, dv), dtype=q.dtype, device=device)
     if n:
-        _call("oige_decay_attention_step", io, q.device)
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        _call("oige_decay_attention_step", _pack_step(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), state.data_ptr(), decay.data_ptr(), _ptr(resets),
+            qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], 0 if resets is None else resets.stride(0), n, h, hk, dk, dv, _TYPES[q.dtype],
+            0 if resets is None else resets.element_size(), scale, 0), device)
         if not state.is_inference():
             torch.autograd.graph.increment_version(state)  # a graph that saved the state must not be run backward any more
     return o
