@@ -18,11 +18,27 @@ constexpr int LN_MAX_THREADS = 1024;
 constexpr int LN_MAX_WIDTH = 16384;
 constexpr int LN_LDS_COLS = 2048;  // most columns of a wave row: 64 lanes x 4 pieces x 8 elements
 
-// Sum over the lanes that share a row: `lanes` (a power of two) neighbours of a wave, or the workgroup.
+// x + x of another lane, the lane found by the data path itself (no LDS round trip).
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
+}
+// Sum over `lanes` (a power of two) neighbours, in all of them: pairs and fours by permutation, then mirrored halves of 8 and 16
+// (their lanes hold equal sums by then), then two exchanges across 16 and 32 lanes.
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  if (lanes > 1) v = add_dpp<0xB1>(v);    // quad_perm 1 0 3 2
+  if (lanes > 2) v = add_dpp<0x4E>(v);    // quad_perm 2 3 0 1
+  if (lanes > 4) v = add_dpp<0x141>(v);   // row_half_mirror
+  if (lanes > 8) v = add_dpp<0x140>(v);   // row_mirror
+  if (lanes > 16) v += __shfl_xor(v, 16, WAVE);
+  if (lanes > 32) v += __shfl_xor(v, 32, WAVE);
+  return v;
+}
+
+// Sum over the lanes that share a row: `lanes` neighbours of a wave, or the workgroup.
 template <bool BLOCK>
 __device__ __forceinline__ float row_sum(float v, int lanes, float* lds) {
-  const int top = BLOCK ? WAVE : lanes;
-  for (int off = top / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, WAVE);
+  v = lanes_sum(v, BLOCK ? WAVE : lanes);
   if (BLOCK) {
     const int w = threadIdx.x >> 6, waves = blockDim.x >> 6;
     __syncthreads();  // the last sum's readers are done
@@ -36,11 +52,8 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float* lds) {
 
 template <bool BLOCK>
 __device__ __forceinline__ float2 row_sum2(float2 v, int lanes, float* lds) {
-  const int top = BLOCK ? WAVE : lanes;
-  for (int off = top / 2; off > 0; off >>= 1) {
-    v.x += __shfl_xor(v.x, off, WAVE);
-    v.y += __shfl_xor(v.y, off, WAVE);
-  }
+  v.x = lanes_sum(v.x, BLOCK ? WAVE : lanes);
+  v.y = lanes_sum(v.y, BLOCK ? WAVE : lanes);
   if (BLOCK) {
     const int w = threadIdx.x >> 6, waves = blockDim.x >> 6;
     __syncthreads();
@@ -60,6 +73,7 @@ __device__ __forceinline__ float2 row_sum2(float2 v, int lanes, float* lds) {
 
 template <typename T, int VEC, int K, bool BLOCK>
 __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_norm_forward_kernel(const oige_layer_norm_io a, int lanes) {
+  constexpr int MODE = VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE;
   __shared__ float lds[2 * LN_MAX_THREADS / WAVE];
   const int l = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
   const int rows_per_block = BLOCK ? 1 : LN_THREADS / lanes;
@@ -75,12 +89,21 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
       w[k][e] = a.weight && col < width ? load_elem(a.weight, col, a.weight_dtype) : 1.f;
       b[k][e] = a.bias && col < width ? load_elem(a.bias, col, a.weight_dtype) : 0.f;
     }
-  for (int64_t row = (int64_t)blockIdx.x * rows_per_block + sub; row < a.rows; row += (int64_t)gridDim.x * rows_per_block) {
-    const T* xr = static_cast<const T*>(a.x) + row * a.x_row_stride;
+  // the next row is on its way while this one is summed
+  const int64_t first = (int64_t)blockIdx.x * rows_per_block + sub, step = (int64_t)gridDim.x * rows_per_block;
+  Run<T, VEC, MODE> run[K];
+  if (first < a.rows) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) run[k].issue(static_cast<const T*>(a.x) + first * a.x_row_stride, (k * lanes + l) * VEC, width);
+  }
+  for (int64_t row = first; row < a.rows; row += step) {
     float x[K][VEC];
     float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) load_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(x[k], xr, (k * lanes + l) * VEC, width);
+    for (int k = 0; k < K; ++k) run[k].take(x[k], (k * lanes + l) * VEC, width);
+    const T* next = static_cast<const T*>(a.x) + (row + step < a.rows ? row + step : row) * a.x_row_stride;
+#pragma unroll
+    for (int k = 0; k < K; ++k) run[k].issue(next, (k * lanes + l) * VEC, width);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -101,7 +124,7 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
       float y[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) y[e] = fmaf(x[k][e] * rstd, w[k][e], b[k][e]);
-      store_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(y, yr, (k * lanes + l) * VEC, width);
+      store_run<T, VEC, MODE>(y, yr, (k * lanes + l) * VEC, width);
     }
     if (a.mean && l == 0) {
       a.mean[row] = mean;
@@ -112,6 +135,7 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
 
 template <typename T, int VEC, int K, bool BLOCK>
 __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_norm_backward_kernel(const oige_layer_norm_io a, int lanes) {
+  constexpr int MODE = VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE;
   __shared__ float lds[2 * LN_MAX_THREADS / WAVE];
   __shared__ float cols[BLOCK ? 1 : LN_THREADS / WAVE * LN_LDS_COLS];
   const int l = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
@@ -128,16 +152,28 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
       w[k][e] = a.weight && col < width ? load_elem(a.weight, col, a.weight_dtype) : 1.f;
       dw[k][e] = db[k][e] = 0.f;
     }
-  for (int64_t row = (int64_t)blockIdx.x * rows_per_block + sub; row < a.rows; row += (int64_t)gridDim.x * rows_per_block) {
-    const T* xr = static_cast<const T*>(a.x) + row * a.x_row_stride;
-    const T* dyr = static_cast<const T*>(a.dy) + row * a.dy_row_stride;
+  const int64_t first = (int64_t)blockIdx.x * rows_per_block + sub, step = (int64_t)gridDim.x * rows_per_block;
+  Run<T, VEC, MODE> x_run[K], g_run[K];
+  float next_mean = 0.f, next_rstd = 0.f;
+  const auto issue = [&](int64_t row) {  // one row ahead, as above
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      x_run[k].issue(static_cast<const T*>(a.x) + row * a.x_row_stride, (k * lanes + l) * VEC, width);
+      g_run[k].issue(static_cast<const T*>(a.dy) + row * a.dy_row_stride, (k * lanes + l) * VEC, width);
+    }
+    next_mean = a.mean[row];
+    next_rstd = a.rstd[row];
+  };
+  if (first < a.rows) issue(first);
+  for (int64_t row = first; row < a.rows; row += step) {
     float x[K][VEC], g[K][VEC];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      load_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(x[k], xr, (k * lanes + l) * VEC, width);
-      load_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(g[k], dyr, (k * lanes + l) * VEC, width);
+      x_run[k].take(x[k], (k * lanes + l) * VEC, width);
+      g_run[k].take(g[k], (k * lanes + l) * VEC, width);
     }
-    const float mean = a.mean[row], rstd = a.rstd[row];
+    const float mean = next_mean, rstd = next_rstd;
+    issue(row + step < a.rows ? row + step : row);
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -159,7 +195,7 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
         float d[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d[e] = rstd * (g[k][e] - fmaf(x[k][e], mgx, mg));
-        store_run<T, VEC, VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE>(d, dxr, (k * lanes + l) * VEC, width);
+        store_run<T, VEC, MODE>(d, dxr, (k * lanes + l) * VEC, width);
       }
     }
   }
@@ -209,8 +245,19 @@ __global__ __launch_bounds__(LN_FOLD * LN_FOLD) void layer_norm_fold_kernel(cons
   const int c = threadIdx.x % LN_FOLD, s = threadIdx.x / LN_FOLD;
   const int64_t col = (int64_t)blockIdx.x * LN_FOLD + c, cols = 2 * (int64_t)a.width;
   float v = 0.f;
-  if (col < cols)
-    for (int i = s; i < parts; i += LN_FOLD) v += a.workspace[i * cols + col];
+  if (col < cols) {
+    constexpr int U = 8;  // partial rows in flight
+    for (int i0 = s; i0 < parts; i0 += U * LN_FOLD) {
+      float p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * LN_FOLD;
+        p[u] = a.workspace[(i < parts ? i : s) * cols + col];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) v += i0 + u * LN_FOLD < parts ? p[u] : 0.f;
+    }
+  }
   lds[s][c] = v;
   __syncthreads();
   if (s == 0 && col < cols) {
@@ -244,7 +291,11 @@ static LnShape layer_norm_shape(int width, int vec) {
   return s;
 }
 
-constexpr int64_t LN_MAX_BLOCKS = 2048, LN_MAX_PARTS = 1024;  // forward: 8 workgroups per CU; backward: one partial row each
+// Workgroups walk rows, so that weights stay in registers and the next row is on its way behind this one's sums.  Forward: 4 per CU
+// with 16-byte accesses (262144 x 1024 bf16: 225 us, 238 with 8 per CU, 635 with a workgroup for every 4 rows), 8 with single
+// elements, which have a quarter of the bytes in flight (65536 x 211 fp32: 21.2 us, 22.8 with 4).  Backward: 4 per CU, one partial
+// row of the parameters' gradients each (65536 x 512 bf16: 37 us, 40 with 2, 43 with 8).
+constexpr int64_t LN_MAX_BLOCKS = 1024, LN_MAX_BLOCKS_SINGLE = 2048, LN_MAX_PARTS = 1024;
 
 static int64_t layer_norm_blocks(int64_t rows, const LnShape& s, int64_t most) {
   const int64_t per = s.block ? 1 : LN_THREADS / s.lanes;
@@ -321,7 +372,7 @@ int oige_layer_norm_forward(const oige_layer_norm_io* io, oige_stream_t stream) 
   OIGE_REQUIRE((io->mean == nullptr) == (io->rstd == nullptr), "layer_norm_forward: mean and rstd are kept together or not at all");
   const bool wide = layer_norm_wide(*io, false);
   const LnShape s = layer_norm_shape(io->width, wide ? 16 / elem_bytes(io->dtype) : 1);
-  return layer_norm_dispatch<false>(*io, wide, s, layer_norm_blocks(io->rows, s, LN_MAX_BLOCKS), (hipStream_t)stream);
+  return layer_norm_dispatch<false>(*io, wide, s, layer_norm_blocks(io->rows, s, wide ? LN_MAX_BLOCKS : LN_MAX_BLOCKS_SINGLE), (hipStream_t)stream);
 }
 
 int64_t oige_layer_norm_workspace_floats(int64_t rows, int32_t width) {
