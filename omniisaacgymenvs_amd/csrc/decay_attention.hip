@@ -77,6 +77,7 @@ __device__ __forceinline__ int64_t da_flag(const DaCore& c, int64_t n, int64_t t
 // decay^n.  Products of squares in 64 bits: exact where the result is used in 32, also for decays of 0 and above 1.
 __device__ __forceinline__ double da_power(double decay, int64_t n) {
   double r = 1.0, sq = decay;
+#pragma unroll 1
   for (; n > 0; n >>= 1) {
     if (n & 1) r *= sq;
     sq *= sq;
@@ -84,14 +85,16 @@ __device__ __forceinline__ double da_power(double decay, int64_t n) {
   return r;
 }
 struct DaPowers {  // decay^n for n in 0 .. 32 without a loop, within 5 roundings
+  double d16, d32;
   float p1, p2, p4, p8, p16, p32;
   __device__ __forceinline__ explicit DaPowers(double d) : p1((float)d), p2((float)(d * d)) {
     const double d4 = (d * d) * (d * d);
     p4 = (float)d4;
     p8 = (float)(d4 * d4);
-    const double d16 = (d4 * d4) * (d4 * d4);
+    d16 = (d4 * d4) * (d4 * d4);
+    d32 = d16 * d16;
     p16 = (float)d16;
-    p32 = (float)(d16 * d16);
+    p32 = (float)d32;
   }
   __device__ __forceinline__ float operator()(int n) const {
     float r = (n & 1) ? p1 : 1.f;
@@ -105,14 +108,24 @@ struct DaPowers {  // decay^n for n in 0 .. 32 without a loop, within 5 rounding
 
 // This wave's piece of a state matrix in memory: tile (s, sv), register r, lane (c, g) holds dk = NK (4 g + r) + s,
 // dv = dv0 + NV c + sv.
+// Row `row + lane_row` of a matrix of `width` columns from column `col` on.  Whole tiles: the scalar unit takes the row's part that
+// all lanes share, a lane adds 32 bits.  Else row 0 stands in for rows behind the end.
+template <int MODE>
+__device__ __forceinline__ const float* da_state_row(const float* p, int row, int lane_row, int height, int width) {
+  if (MODE == ELEMS_FULL)
+    return reinterpret_cast<const float*>(reinterpret_cast<const char*>(p + row * width) + (uint32_t)(lane_row * width) * 4u);
+  const int d = row + lane_row;
+  return p + (d < height ? d : 0) * width;
+}
+
 template <int NK, int NV, int MODE>
 __device__ __forceinline__ void da_load_state(f32x4 (&S)[NK][NV], const float* p, const DaCore& a, int dv0, int c, int g) {
   if (a.transposed) {
 #pragma unroll
     for (int sv = 0; sv < NV; ++sv) {
-      const int d = dv0 + NV * c + sv;
+      const bool in = MODE == ELEMS_FULL || dv0 + NV * c + sv < a.dv;
       float x[4 * NK];
-      load_run<float, 4 * NK, MODE>(x, p + (int64_t)(d < a.dv ? d : 0) * a.dk, 4 * NK * g, d < a.dv ? a.dk : 0);
+      load_run<float, 4 * NK, MODE>(x, da_state_row<MODE>(p, dv0 + sv, NV * c, a.dv, a.dk), 4 * NK * g, in ? a.dk : 0);
 #pragma unroll
       for (int s = 0; s < NK; ++s) S[s][sv] = f32x4{x[s], x[NK + s], x[2 * NK + s], x[3 * NK + s]};
     }
@@ -123,8 +136,8 @@ __device__ __forceinline__ void da_load_state(f32x4 (&S)[NK][NV], const float* p
       float x[4][NV];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int d = NK * (4 * g + r) + s;
-        load_run<float, NV, MODE>(x[r], p + (int64_t)(d < a.dk ? d : 0) * a.dv, dv0 + NV * c, d < a.dk ? a.dv : 0);
+        const bool in = MODE == ELEMS_FULL || NK * (4 * g + r) + s < a.dk;
+        load_run<float, NV, MODE>(x[r], da_state_row<MODE>(p, NK * r + s, NK * 4 * g, a.dk, a.dv), dv0 + NV * c, in ? a.dv : 0);
       }
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) S[s][sv] = f32x4{x[0][sv], x[1][sv], x[2][sv], x[3][sv]};
@@ -137,7 +150,6 @@ __device__ __forceinline__ void da_store_state(const f32x4 (&S)[NK][NV], float* 
   if (a.transposed) {
 #pragma unroll
     for (int sv = 0; sv < NV; ++sv) {
-      const int d = dv0 + NV * c + sv;
       float x[4 * NK];
 #pragma unroll
       for (int s = 0; s < NK; ++s) {
@@ -146,7 +158,8 @@ __device__ __forceinline__ void da_store_state(const f32x4 (&S)[NK][NV], float* 
         x[2 * NK + s] = S[s][sv].z;
         x[3 * NK + s] = S[s][sv].w;
       }
-      if (d < a.dv) store_run<float, 4 * NK, MODE>(x, p + (int64_t)d * a.dk, 4 * NK * g, a.dk);
+      if (MODE == ELEMS_FULL || dv0 + NV * c + sv < a.dv)
+        store_run<float, 4 * NK, MODE>(x, const_cast<float*>(da_state_row<MODE>(p, dv0 + sv, NV * c, a.dv, a.dk)), 4 * NK * g, a.dk);
     }
   } else {
 #pragma unroll
@@ -160,10 +173,9 @@ __device__ __forceinline__ void da_store_state(const f32x4 (&S)[NK][NV], float* 
         x[3][sv] = S[s][sv].w;
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = NK * (4 * g + r) + s;
-        if (d < a.dk) store_run<float, NV, MODE>(x[r], p + (int64_t)d * a.dv, dv0 + NV * c, a.dv);
-      }
+      for (int r = 0; r < 4; ++r)
+        if (MODE == ELEMS_FULL || NK * (4 * g + r) + s < a.dk)
+          store_run<float, NV, MODE>(x[r], const_cast<float*>(da_state_row<MODE>(p, NK * r + s, NK * 4 * g, a.dk, a.dv)), dv0 + NV * c, a.dv);
     }
   }
 }
@@ -244,18 +256,25 @@ struct DaWave {
 };
 __device__ __forceinline__ int da_last_segment(const DaCore& a, int64_t len) { return len > 0 ? (int)((len - 1) / a.seg_len) : 0; }
 __device__ __forceinline__ int da_role(const DaRoles& r) { return (int)(blockIdx.x / DA_XCDS % r.roles); }
+// The role's fields once more, read behind the loop: what only its end needs stays out of the scalar registers until then.
+__device__ __forceinline__ const DaCore& da_again(const DaRoles& r) {
+  int role = da_role(r);
+  asm volatile("" : "+s"(role));
+  return r.c[role];
+}
 template <int NV>
 __device__ __forceinline__ DaWave da_wave(const DaCore& a, int roles) {
   DaWave w{};
-  const int64_t block = (int64_t)(blockIdx.x / DA_XCDS / roles) * DA_XCDS + blockIdx.x % DA_XCDS;
-  const int64_t u = block * DA_WAVES + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  w.live = u < a.n * a.h * a.slices;
+  const uint32_t block = blockIdx.x / DA_XCDS / (uint32_t)roles * DA_XCDS + blockIdx.x % DA_XCDS;
+  const uint32_t u = block * DA_WAVES + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));  // below 2^31: checked on the host
+  const uint32_t nh = u / (uint32_t)a.slices, n = nh / (uint32_t)a.h;
+  w.live = n < (uint32_t)a.n;
   if (!w.live) return w;
   w.seg = blockIdx.y;
-  w.slice = (int)(u % a.slices);
-  w.nh = u / a.slices;
-  w.h = (int)(w.nh % a.h);
-  w.n = w.nh / a.h;
+  w.slice = (int)(u - nh * (uint32_t)a.slices);
+  w.nh = nh;
+  w.h = (int)(nh - n * (uint32_t)a.h);
+  w.n = n;
   w.dv0 = w.slice * 16 * NV;
   w.len = da_length(a, w.n);
   w.last = da_last_segment(a, w.len);
@@ -383,6 +402,10 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
 #pragma unroll
     for (int r = 0; r < 4; ++r) v_run[r].issue(b.at(vh, a.v.st, 4 * g + r), dv0 + NV * c, a.dv);
   };
+  const auto forget = [&](auto& run) {
+#pragma unroll
+    for (auto& x : run) x.forget();
+  };
   const auto put_rows = [&](const Run<T, NK, MODE> (&run)[4]) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -421,7 +444,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     if (p0 == begin || p0 == DA_TOKENS || L < DA_TOKENS) {
       const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
       const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
-      const double keep = da_power(decay, L - first);
+      const double keep = L - first == DA_TOKENS ? pw.d16 : da_power(decay, L - first);
       keep_hi = (float)keep;
       keep_lo = (float)(keep - (double)keep_hi);
       head_w = pw(c + 1 - first);
@@ -435,7 +458,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     // bit i: a reset in front of the block's token i
     const uint32_t m = a.resets ? (uint32_t)(__ballot(flag != 0 && c < L && !(a.reverse && p0 == 0 && c == 0)) & 0xFFFFull) : 0u;
     const bool more = p0 + DA_TOKENS < end;
-    const DaBlock next = da_block<DA_TOKENS>(a, more ? p0 + DA_TOKENS : p0, end, len);  // behind the last block: the same rows once more
+    const DaBlock next = da_block<DA_TOKENS>(a, more ? p0 + DA_TOKENS : p0, end, len);
 
     f32x4 acc[NV];
     float V[4][NV], K2[4][NK];
@@ -443,10 +466,12 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
       float Q[4 * NK], K1[4 * NK];
       put_rows(q_run);
       get_token(Q);
-      issue_q(next);
+      if (more) issue_q(next);
+      else forget(q_run);
       put_rows(k_run);
       get_token(K1);
-      issue_k(next);
+      if (more) issue_k(next);
+      else forget(k_run);
       f32x4 pt = zero;
 #pragma unroll
       for (int e = 0; e < 4 * NK; ++e) pt = __builtin_amdgcn_mfma_f32_16x16x4f32(K1[e], Q[e], pt, 0, 0, 0);
@@ -535,8 +560,12 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
 #pragma unroll
         for (int sv = 0; sv < NV; ++sv) S[s][sv] = zero;
     }
-    if (STATES) issue_k(next);
-    issue_v(next);
+    if (STATES) {
+      if (more) issue_k(next);
+      else forget(k_run);
+    }
+    if (more) issue_v(next);
+    else forget(v_run);
 #pragma unroll
     for (int s = 0; s < NK; ++s)
 #pragma unroll
@@ -548,7 +577,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     da_settle();
     blk = next;
   }
-  da_close<T, NK, NV, MODE, STATES>(S, a, w, lane, decay, dropped);
+  da_close<T, NK, NV, MODE, STATES>(S, da_again(roles), w, lane, decay, dropped);
 }
 
 // ---------------------------------------------------------------- the same for bf16 tensors
@@ -628,7 +657,6 @@ __device__ __forceinline__ void db_state_part(f32x4 (&acc)[2][NV], const f32x4 (
     for (int sv = 0; sv < NV; ++sv) acc[it][sv] = zero;
 #pragma unroll
   for (int p = 0; p < NK / 2; ++p) {
-    __builtin_amdgcn_sched_barrier(0);
     u32x4 q[2];
 #pragma unroll
     for (int it = 0; it < 2; ++it) {
@@ -720,7 +748,9 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   // take whole tokens by way of LDS.
   constexpr int LD = 8 * NK + 4;  // in registers' words
   __shared__ __align__(16) uint32_t lds_rows[DA_WAVES][DB_TOKENS * LD];
-  uint32_t* lds = lds_rows[threadIdx.x >> 6];
+  constexpr int LD_OUT = 8 * NV + 4;
+  __shared__ __align__(16) uint32_t lds_out[DA_WAVES][DB_TOKENS * LD_OUT];
+  uint32_t *lds = lds_rows[threadIdx.x >> 6], *out = lds_out[threadIdx.x >> 6];
   Bits<NK, MODE> q_run[8], k_run[8];
   Bits<NV, MODE> v_run[8];
   int64_t flag = 0;
@@ -740,6 +770,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
       const int g = da_here(lane) >> 4;
 #pragma unroll
       for (int e = 0; e < 8; ++e) run[e].issue(base, db_offset(b, (uint32_t)(4 * g + (e < 4 ? e : 12 + e)) * (uint32_t)st, (uint32_t)st), off, limit);
+      asm volatile("" ::: "memory");  // as above: merged, both branches' loads would go through addresses in vector registers
     }
   };
   const auto issue_q = [&](const DaBlock& b) {
@@ -750,6 +781,10 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
     if (a.resets) flag = da_block_flag(a, b, n, da_here(lane) & 31);
   };
   const auto issue_v = [&](const DaBlock& b) { issue(v_run, vh, a.v.st, v_group, b, dv0 + NV * c, a.dv); };
+  const auto forget = [&](auto& run) {
+#pragma unroll
+    for (auto& x : run) x.run.forget();
+  };
   const auto lds_row = [&](int e) { return lds + ((e < 4 ? 0 : 12) + 4 * g + e) * LD; };
   const auto put_rows = [&](const Bits<NK, MODE> (&run)[8]) {
 #pragma unroll
@@ -791,7 +826,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
     if (p0 == begin || p0 == DB_TOKENS || L < DB_TOKENS) {
       const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
       const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
-      const double keep = da_power(decay, L - first);
+      const double keep = L - first == DB_TOKENS ? pw.d32 : da_power(decay, L - first);
       keep_hi = (float)keep;
       keep_lo = (float)(keep - (double)keep_hi);
       head_w[0] = pw(c + 1 - first);
@@ -812,19 +847,17 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
     // bit i: a reset in front of the block's token i
     const uint32_t m = a.resets ? (uint32_t)__ballot(flag != 0 && (lane & 31) < L && !(rev && p0 == 0 && (lane & 31) == 0)) : 0u;
     const bool more = p0 + DB_TOKENS < end;
-    const DaBlock next = da_block<DB_TOKENS>(a, more ? p0 + DB_TOKENS : p0, end, len);  // behind the last block: the same rows once more
+    const DaBlock next = da_block<DB_TOKENS>(a, more ? p0 + DB_TOKENS : p0, end, len);
     const uint32_t upto[2] = {(2u << c) - 1u, (0x20000u << c) - 1u};  // bits 0 .. i for token i = c, 16 + c
 
-    uint32_t V[8][Bits<NV, MODE>::REGS], K2[8][NK / 2];
+    uint32_t V[8][Bits<NV, MODE>::REGS], K2[STATES ? 8 : 1][NK / 2];  // k stays in LDS where it went there
     if (!STATES) {
       f32x4 acc[2][NV];
       uint32_t Q[2][2 * NK], K1[2][2 * NK];
       put_rows(q_run);
       get_tokens(Q);
-      issue_q(next);
       put_rows(k_run);
       get_tokens(K1);
-      issue_k(next);
       f32x4 pt[3] = {zero, zero, zero};  // P^T: tokens 0-15 for 0-15, 0-15 for 16-31, 16-31 for 16-31
 #pragma unroll
       for (int p = 0; p < NK / 2; ++p) {
@@ -838,11 +871,13 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
         pt[1] = db_mfma(k[0], q[1], pt[1]);
         pt[2] = db_mfma(k[1], q[1], pt[2]);
       }
-      __builtin_amdgcn_sched_barrier(0);
+        if (more) issue_k(next);
+      else forget(k_run);
       const bool from_state[2] = {!(m & upto[0]), !(m & upto[1])};
       db_state_part<NK, NV>(acc, S, Q, from_state, head_w);
-      __builtin_amdgcn_sched_barrier(0);
-      // a masked product may be infinite or NaN: selected away, not multiplied
+      if (more) issue_q(next);
+      else forget(q_run);
+        // a masked product may be infinite or NaN: selected away, not multiplied
       const f32x4 w0 = weights[0], w1 = weights[WAVE];
       const float pair_w[4] = {w0.x, w0.y, w0.z, w0.w}, cross_w[4] = {w1.x, w1.y, w1.z, w1.w};
       float P[3][4] = {{pt[0].x, pt[0].y, pt[0].z, pt[0].w}, {pt[1].x, pt[1].y, pt[1].z, pt[1].w}, {pt[2].x, pt[2].y, pt[2].z, pt[2].w}};
@@ -931,21 +966,15 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
         }
         da_settle();
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int i = 0; i < NK / 2; ++i) K2[e][i] = lds_row(e)[NK / 2 * c + i];
-      wave_lds_fence();
-      db_store_out<NV, MODE, LD>(lds, acc, a, blk, n * a.on + (int64_t)h * a.oh, dv0, c, g);
+      db_store_out<NV, MODE, LD_OUT>(out, acc, a, blk, n * a.on + (int64_t)h * a.oh, dv0, c, g);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v_run[e].take(V[e], dv0 + NV * c, a.dv);
-        k_run[e].take(K2[e], NK * c, a.dk);
+        if constexpr (STATES) k_run[e].take(K2[e], NK * c, a.dk);
       }
     }
 
-    __builtin_amdgcn_sched_barrier(0);
     // rows in front of the block's last reset, and behind the end, stay out of the state's sum altogether
     if (m || L < DB_TOKENS) {
       const int g = da_here(lane) >> 4;
@@ -953,11 +982,17 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
       for (int e = 0; e < 8; ++e) {
         const int j = (e < 4 ? 0 : 12) + 4 * g + e;
         const bool in = j < L && !(m & ~((2u << j) - 1u));
+        if constexpr (STATES) {
 #pragma unroll
-        for (int i = 0; i < NK / 2; ++i) K2[e][i] = in ? K2[e][i] : 0u;
+          for (int i = 0; i < NK / 2; ++i) K2[e][i] = in ? K2[e][i] : 0u;
+        } else if (!in) {
+#pragma unroll
+          for (int i = 0; i < NK / 2; ++i) lds_row(e)[NK / 2 * c + i] = 0u;
+        }
 #pragma unroll
         for (int i = 0; i < Bits<NV, MODE>::REGS; ++i) V[e][i] = in ? V[e][i] : 0u;
       }
+      wave_lds_fence();
     }
     u32x4 vh3[NV], vm3[NV], vl3[NV];
     const f32x4 w2 = weights[2 * WAVE], w3 = weights[3 * WAVE];
@@ -985,14 +1020,26 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
 #pragma unroll
         for (int sv = 0; sv < NV; ++sv) S[s][sv] = zero;
     }
-    if (STATES) issue_k(next);
-    issue_v(next);
+    if (STATES) {
+      if (more) issue_k(next);
+      else forget(k_run);
+    }
+    if (more) issue_v(next);
+    else forget(v_run);
+    uint32_t kk[8];
 #pragma unroll
     for (int s = 0; s < NK; ++s) {
-      __builtin_amdgcn_sched_barrier(0);
-      const int i = s / 2;
-      const u32x4 k = s & 1 ? u32x4{db_highs(K2[0][i], K2[1][i]), db_highs(K2[2][i], K2[3][i]), db_highs(K2[4][i], K2[5][i]), db_highs(K2[6][i], K2[7][i])}
-                            : u32x4{db_lows(K2[0][i], K2[1][i]), db_lows(K2[2][i], K2[3][i]), db_lows(K2[4][i], K2[5][i]), db_lows(K2[6][i], K2[7][i])};
+        const int i = s / 2;
+      if (!(s & 1)) {
+        if constexpr (NK == 8 && !STATES) __builtin_amdgcn_sched_barrier(0);  // or all of k is read at once, into registers there are not
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (STATES) kk[e] = K2[e][i];
+          else kk[e] = lds_row(e)[NK / 2 * c + i];
+        }
+      }
+      const u32x4 k = s & 1 ? u32x4{db_highs(kk[0], kk[1]), db_highs(kk[2], kk[3]), db_highs(kk[4], kk[5]), db_highs(kk[6], kk[7])}
+                            : u32x4{db_lows(kk[0], kk[1]), db_lows(kk[2], kk[3]), db_lows(kk[4], kk[5]), db_lows(kk[6], kk[7])};
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) {
         S[s][sv] *= kept;
@@ -1001,10 +1048,11 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
         S[s][sv] = db_mfma(k, vh3[sv], S[s][sv]);
       }
     }
+    wave_lds_fence();
     da_settle();
     blk = next;
   }
-  da_close<__bf16, NK, NV, MODE, STATES>(S, a, w, lane, decay, dropped);
+  da_close<__bf16, NK, NV, MODE, STATES>(S, da_again(roles), w, lane, decay, dropped);
 }
 
 // The states in front of every segment from those at the segments' ends (in place, register order): carry = factor carry + end.
@@ -1192,7 +1240,8 @@ static int decay_attention_run(const DaRoles& in, const DaPlan& p, float* worksp
   DaRoles r = in;
   const int64_t heads = r.c[0].n * r.c[0].h, units = heads * p.slices, groups = ((units + DA_WAVES - 1) / DA_WAVES + DA_XCDS - 1) / DA_XCDS;
   const int64_t blocks = groups * DA_XCDS * r.roles, per_head = (int64_t)p.slices * NK * NV * WAVE;  // the last in 16-byte quads
-  OIGE_REQUIRE(blocks < ((int64_t)1 << 31), "decay_attention: %lld sequences x heads are too many for one launch", (long long)heads);
+  OIGE_REQUIRE(groups * DA_XCDS * DA_WAVES < ((int64_t)1 << 31) && blocks < ((int64_t)1 << 31),
+               "decay_attention: %lld sequences x heads are too many for one launch", (long long)heads);
   for (int i = 0; i < r.roles; ++i) {
     DaCore& c = r.c[i];
     c.slices = p.slices;

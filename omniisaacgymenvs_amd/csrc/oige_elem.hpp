@@ -56,6 +56,27 @@ struct Run {
     for (int b = 0; b < CNT / W; ++b)
       x[b] = *reinterpret_cast<const Pack<T, W>*>(row + (MODE == ELEMS_FULL || off + b * W < limit ? off + b * W : 0));
   }
+  // Nothing was asked for: the registers hold no value (without this the last one would be kept for a round that does not come).
+  __device__ __forceinline__ void forget() {
+    constexpr int BYTES = W * (int)sizeof(T);
+    typedef uint32_t words __attribute__((ext_vector_type(BYTES < 8 ? 2 : BYTES / 4)));
+#pragma unroll
+    for (int b = 0; b < CNT / W; ++b) {
+      if constexpr (BYTES >= 8) {
+        words w;
+        asm volatile("" : "=v"(w));
+        x[b] = __builtin_bit_cast(Pack<T, W>, w);
+      } else if constexpr (BYTES == 4) {
+        uint32_t w;
+        asm volatile("" : "=v"(w));
+        x[b] = __builtin_bit_cast(Pack<T, W>, w);
+      } else {
+        uint16_t w;
+        asm volatile("" : "=v"(w));
+        x[b] = __builtin_bit_cast(Pack<T, W>, w);
+      }
+    }
+  }
   __device__ __forceinline__ void take(float (&out)[CNT], int off, int limit) const {
 #pragma unroll
     for (int b = 0; b < CNT / W; ++b)
