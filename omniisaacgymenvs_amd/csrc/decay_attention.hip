@@ -633,18 +633,12 @@ struct Bits {
 #pragma unroll
     for (int i = 0; i < REGS; ++i) {
       const int e = CNT == 1 ? 0 : 2 * i;
-      const bool ok0 = MODE == ELEMS_FULL || off + e / W * W < limit, ok1 = MODE == ELEMS_FULL || off + (e + 1) / W * W < limit;
-      const uint32_t lo = run.x[e / W].v[e % W];
-      const uint32_t hi = CNT == 1 ? 0u : (uint32_t)run.x[(e + 1) / W].v[(e + 1) % W];
-      out[i] = (ok0 ? lo : 0u) | (CNT == 1 || !ok1 ? 0u : hi << 16);
+      const uint32_t lo = run.x[e / W].v[e % W], hi = CNT == 1 ? 0u : (uint32_t)run.x[(e + 1) / W].v[(e + 1) % W];
+      out[i] = lo | hi << 16;
+      if (MODE != ELEMS_FULL) out[i] &= bits_if(off + e / W * W < limit);  // (a pair lies in one piece)
     }
   }
 };
-// element e of a row held that way, paired over two rows
-template <int E>
-__device__ __forceinline__ uint32_t db_pair(uint32_t x, uint32_t y) {
-  return E & 1 ? db_highs(x, y) : db_lows(x, y);
-}
 
 // O^T's part from the state: for both halves of the block's tokens, the state's hi and lo parts against q.
 template <int NK, int NV>

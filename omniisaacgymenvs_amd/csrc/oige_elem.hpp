@@ -32,6 +32,15 @@ __device__ __forceinline__ void store_elem(void* p, int64_t i, float x, int dtyp
 // ELEMS_SINGLE: element by element.
 constexpr int ELEMS_FULL = 0, ELEMS_WIDE = 1, ELEMS_SINGLE = 2;
 
+// All bits where `in`, none elsewhere, as a value the compiler knows nothing about: an AND with it stays one instruction, where a
+// select between a loaded value and zero has become a branch around the load.
+__device__ __forceinline__ uint32_t bits_if(bool in) {
+  uint32_t m = in ? 0xFFFFFFFFu : 0u;
+  asm("" : "+v"(m));
+  return m;
+}
+__device__ __forceinline__ float and_bits(float x, uint32_t m) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & m); }
+
 // CNT consecutive elements from `off` of a row of `limit`, as floats; elements behind the limit read as 0.  A piece behind the end
 // re-reads the row's first one (no load inside a conditional block).
 template <typename T, int CNT, int MODE>
@@ -41,8 +50,9 @@ __device__ __forceinline__ void load_run(float (&out)[CNT], const T* row, int of
   for (int b = 0; b < CNT; b += W) {
     const bool ok = MODE == ELEMS_FULL || off + b < limit;
     const Pack<T, W> x = *reinterpret_cast<const Pack<T, W>*>(row + (ok ? off + b : 0));
+    const uint32_t in = MODE == ELEMS_FULL ? 0u : bits_if(ok);
 #pragma unroll
-    for (int e = 0; e < W; ++e) out[b + e] = ok ? (float)x.v[e] : 0.f;
+    for (int e = 0; e < W; ++e) out[b + e] = MODE == ELEMS_FULL ? (float)x.v[e] : and_bits((float)x.v[e], in);
   }
 }
 
@@ -79,9 +89,11 @@ struct Run {
   }
   __device__ __forceinline__ void take(float (&out)[CNT], int off, int limit) const {
 #pragma unroll
-    for (int b = 0; b < CNT / W; ++b)
+    for (int b = 0; b < CNT / W; ++b) {
+      const uint32_t in = MODE == ELEMS_FULL ? 0u : bits_if(off + b * W < limit);
 #pragma unroll
-      for (int e = 0; e < W; ++e) out[b * W + e] = MODE == ELEMS_FULL || off + b * W < limit ? (float)x[b].v[e] : 0.f;
+      for (int e = 0; e < W; ++e) out[b * W + e] = MODE == ELEMS_FULL ? (float)x[b].v[e] : and_bits((float)x[b].v[e], in);
+    }
   }
 };
 
