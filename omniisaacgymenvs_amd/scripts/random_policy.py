@@ -2,11 +2,13 @@
 registry, drive ``VecEnvRLGames.step`` with uniform random actions and print frames per second.
 
     python -m omniisaacgymenvs_amd.scripts.random_policy task=Ant num_envs=4096 [--cfg-dir <reference>/cfg]
-                                                         [--frames 2000] [--graph]
+                                                         [--frames 2000] [--graph] [--policy memory]
 
 Arguments of the form ``key=value`` are hydra-style overrides.  With ``--cfg-dir`` the reference's own YAML files are
 read (utils/hydra_cfg.py); without it the tables of utils/config.py stand in for them.  ``--graph`` replays the wrapper's
-whole step as one HIP graph (``VecEnvRLGames.capture_step``); ``--drop-resets`` leaves the synthetic views' setters out
+whole step as one HIP graph (``VecEnvRLGames.capture_step``); ``--policy memory`` takes the actions from a randomly initialised
+policy with a memory (utils/rlgames/memory_policy.py) that reads the observations and the reset flags, instead of drawing
+them; ``--drop-resets`` leaves the synthetic views' setters out
 (at small sizes their torch scatters, stand-ins for PhysX's, cost more than the task math).  The physics step between the two task calls is the
 synthetic world's (state stays as loaded), so the number printed is the rate of the task math and the wrapper alone.
 """
@@ -22,6 +24,7 @@ import torch
 from omniisaacgymenvs_amd.envs.vec_env_rlgames import VecEnvRLGames
 from omniisaacgymenvs_amd.utils import hydra_cfg
 from omniisaacgymenvs_amd.utils.config import global_config, task_config
+from omniisaacgymenvs_amd.utils.rlgames.memory_policy import MemoryPolicy
 from omniisaacgymenvs_amd.utils.seed import set_seed
 from omniisaacgymenvs_amd.utils.task_util import initialize_task
 
@@ -42,13 +45,15 @@ def compose(cfg_dir: Optional[str], overrides: List[str]) -> Dict[str, Any]:
     return cfg
 
 
-def run(cfg: Dict[str, Any], frames: int, graph: bool = False, report_every: float = 1.0, drop_resets: bool = False
-        ) -> Dict[str, float]:
+def run(cfg: Dict[str, Any], frames: int, graph: bool = False, report_every: float = 1.0, drop_resets: bool = False,
+        policy: str = "uniform") -> Dict[str, float]:
+    if policy not in ("uniform", "memory"):
+        raise ValueError(f"policy {policy!r}: uniform or memory")
     env = VecEnvRLGames(headless=cfg.get("headless", True), sim_device=cfg.get("device_id", 0),
                         enable_livestream=cfg.get("enable_livestream", False))
     cfg["seed"] = set_seed(cfg.get("seed", 42), torch_deterministic=cfg.get("torch_deterministic", False))
     task = initialize_task(cfg, env)
-    env.reset()
+    obs = env.reset()["obs"]
     high, low = float(env.action_space.high[0]), float(env.action_space.low[0])
     shape = (env.num_envs, env.action_space.shape[0])
     actions = torch.empty(shape, device=task.rl_device)
@@ -59,14 +64,20 @@ def run(cfg: Dict[str, Any], frames: int, graph: bool = False, report_every: flo
         if not drop_resets:
             task.set_reset_scatter("device")
         env.capture_step(actions)
+    net = state = resets = None
+    if policy == "memory":
+        net = MemoryPolicy(obs.shape[-1], shape[1]).to(task.rl_device)
+        state = net.initial_state(env.num_envs)  # empty: nothing has been reset against it yet
     num_frames, total, prev = 0, 0, time.time()
     t0 = time.perf_counter()
     while total < frames and env.world.is_playing():
-        actions.uniform_(low, high)
-        if graph:
-            env.replay_step()
-        else:
-            env.step(actions)
+        if net is None:
+            actions.uniform_(low, high)
+        else:  # means in (-1, 1) over the action space
+            mu, _ = net.step(obs, state, resets)
+            torch.add(mu * (0.5 * (high - low)), 0.5 * (high + low), out=actions)
+        out = env.replay_step() if graph else env.step(actions)
+        obs, resets = out[0]["obs"], out[2]
         num_frames += 1
         total += 1
         if time.time() - prev >= report_every:
@@ -88,9 +99,11 @@ def main(argv: Optional[List[str]] = None) -> int:
     ap.add_argument("--drop-resets", action="store_true",
                     help="do not scatter reset rows into the synthetic views (their setters emulate PhysX's, outside the path)")
     ap.add_argument("overrides", nargs="*", help="hydra-style key=value items, e.g. task=Ant num_envs=4096")
+    ap.add_argument("--policy", choices=("uniform", "memory"), default="uniform",
+                    help="uniform random actions (default), or a randomly initialised policy with a memory")
     args = ap.parse_args(argv)
     cfg = compose(args.cfg_dir, args.overrides)
-    run(cfg, args.frames, graph=args.graph, drop_resets=args.drop_resets)
+    run(cfg, args.frames, graph=args.graph, drop_resets=args.drop_resets, policy=args.policy)
     return 0
 
 

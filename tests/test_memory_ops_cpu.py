@@ -174,3 +174,35 @@ def test_abi_decay_attention_step_refuses():
     _fail(fn(C.byref(io), None), "null decay")
     io.decay = 16
     _fail(fn(C.byref(io), None), "null q")
+
+
+def test_packed_argument_blocks_match_the_structures():
+    from omniisaacgymenvs_amd.utils.rlgames import memory_ops as m
+
+    for struct, pack in ((_lib.LayerNormIo, m._pack_norm), (_lib.DecayAttentionIo, m._pack_attention), (_lib.DecayAttentionStepIo, m._pack_step)):
+        count = sum(kind._length_ if issubclass(kind, C.Array) else 1 for _, kind in struct._fields_)
+        block = pack(*range(1, count + 1))
+        assert len(block) == C.sizeof(struct)
+        got = []
+        for name, _ in struct._fields_:
+            v = getattr(struct.from_buffer_copy(block), name)
+            got += list(v) if isinstance(v, C.Array) else [v]
+        assert [int(x) for x in got] == list(range(1, count + 1))
+
+
+def test_policy_refuses():
+    from omniisaacgymenvs_amd.scripts import random_policy
+    from omniisaacgymenvs_amd.utils.rlgames.memory_policy import MemoryPolicy
+
+    with pytest.raises(ValueError, match="not a multiple"):
+        MemoryPolicy(10, 2, width=30, heads=4)
+    with pytest.raises(ValueError, match="uniform or memory"):
+        random_policy.run({}, frames=1, policy="lstm")
+    with pytest.raises(SystemExit):
+        random_policy.main(["task=Ant", "--policy", "lstm"])
+    policy = MemoryPolicy(10, 2, width=32, heads=4, layers=2)
+    assert policy.initial_state(5).shape == (2, 5, 4, 8, 8)
+    with pytest.raises(_lib.OigeError, match="no CPU fallback"):
+        policy.step(torch.zeros(5, 10), policy.initial_state(5))
+    with pytest.raises(_lib.OigeError, match="no CPU fallback"):
+        policy(torch.zeros(5, 3, 10))
