@@ -1296,7 +1296,7 @@ int oige_layer_norm_backward(const oige_layer_norm_io* io, oige_stream_t stream)
 /* Linear attention with a decay per head over sequences of tokens:
  *     S_t = a_t S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t,   a_t = decay[h], 0 where resets flags token t
  * Tensors are (N, T, heads, d) with element strides for the first three axes (the last one is contiguous); heads a multiple of
- * kv_heads; head sizes 1 .. 128.  Tokens from lengths[n] on (clamped to 0 .. T) are not part of sequence n: they are not read
+ * kv_heads; head sizes 1 .. 128; T below 2^30.  Tokens from lengths[n] on (clamped to 0 .. T) are not part of sequence n: they are not read
  * into anything, their rows of o and of the gradients are zero.  An infinite or NaN value reaches only the rows whose
  * tokens see it.  States are fp32, contiguous (N, heads, key_dim, value_dim).                                             */
 typedef struct oige_decay_attention_io {

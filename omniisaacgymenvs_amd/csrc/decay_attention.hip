@@ -46,8 +46,9 @@ struct DaCore {
   const void* resets;
   const void* lengths;
   int64_t rsn, rst;  // element strides of resets
-  int64_t n, t, seg_len;
+  int64_t n;
   float out_scale, kv_scale;
+  int t, seg_len;  // tokens: below 2^30
   int h, dk, dv, slices, nseg;
   int resets_bytes, lengths_bytes;
   int reverse;     // walk from the last token to the first; the first one taken in is not preceded by a decay, the state is multiplied once more at the end
@@ -63,13 +64,13 @@ struct DaRoles {
   int roles;
 };
 
-__device__ __forceinline__ int64_t da_length(const DaCore& c, int64_t n) {
+__device__ __forceinline__ int da_length(const DaCore& c, int64_t n) {
   if (!c.lengths) return c.t;
   const int64_t l = c.lengths_bytes == 8 ? static_cast<const int64_t*>(c.lengths)[n] : static_cast<const int32_t*>(c.lengths)[n];
-  return l < 0 ? 0 : (l > c.t ? c.t : l);
+  return l < 0 ? 0 : (l > c.t ? c.t : (int)l);
 }
 
-__device__ __forceinline__ int64_t da_flag(const DaCore& c, int64_t n, int64_t t) {  // not zero: a reset
+__device__ __forceinline__ int64_t da_flag(const DaCore& c, int64_t n, int t) {  // not zero: a reset
   const int64_t i = n * c.rsn + t * c.rst;
   return c.resets_bytes == 8 ? static_cast<const int64_t*>(c.resets)[i] : (int64_t)static_cast<const uint8_t*>(c.resets)[i];
 }
@@ -209,27 +210,26 @@ __device__ __forceinline__ void da_settle() { asm volatile("s_nop 15" ::: "memor
 // One block's rows of the operands.  Rows behind the block's L tokens re-read its last one; `low` is the earliest of its tokens
 // in memory, and in reverse the block's first token is the latest.
 struct DaBlock {
-  int64_t low;
-  int L, reverse;
+  int low, L, reverse;
   __device__ __forceinline__ int row(int i) const {
     const int r = i < L ? i : L - 1;
     return reverse ? L - 1 - r : r;
   }
   template <typename T>
   __device__ __forceinline__ const T* at(const T* head, int64_t st, int i) const {  // row * stride in 32 x 32 bits: checked on the host
-    return head + low * st + (uint64_t)(uint32_t)row(i) * (uint32_t)st;
+    return head + (int64_t)low * st + (uint64_t)(uint32_t)row(i) * (uint32_t)st;
   }
 };
 // The flag that stands between token i of the block and the token taken in before it: its own, or in reverse the next one's (there
 // is none behind the last token: what is read then is not used).
 __device__ __forceinline__ int64_t da_block_flag(const DaCore& a, const DaBlock& b, int64_t n, int i) {
-  const int64_t t = b.low + b.row(i) + b.reverse;
+  const int t = b.low + b.row(i) + b.reverse;
   return da_flag(a, n, t < a.t ? t : a.t - 1);
 }
 template <int TOKENS>
-__device__ __forceinline__ DaBlock da_block(const DaCore& a, int64_t p0, int64_t end, int64_t len) {
+__device__ __forceinline__ DaBlock da_block(const DaCore& a, int p0, int end, int len) {
   DaBlock b;
-  b.L = end - p0 < TOKENS ? (int)(end - p0) : TOKENS;
+  b.L = end - p0 < TOKENS ? end - p0 : TOKENS;
   b.reverse = a.reverse;
   b.low = a.reverse ? len - p0 - b.L : p0;
   return b;
@@ -250,11 +250,11 @@ __device__ __forceinline__ f32x4 da_poison(f32x4 x, f32x4 hit) {
 
 // What a wave works on: a slice of the state's columns of one head of one sequence, over one segment of its tokens.
 struct DaWave {
-  int64_t n, nh, len, begin, end;
-  int h, seg, last, slice, dv0;  // last: the segment that the sequence ends in; those behind it only clear their rows
+  int64_t n, nh;
+  int len, begin, end, h, seg, last, slice, dv0;  // last: the segment that the sequence ends in; those behind it only clear their rows
   bool live;
 };
-__device__ __forceinline__ int da_last_segment(const DaCore& a, int64_t len) { return len > 0 ? (int)((len - 1) / a.seg_len) : 0; }
+__device__ __forceinline__ int da_last_segment(const DaCore& a, int len) { return len > 0 ? (len - 1) / a.seg_len : 0; }
 __device__ __forceinline__ int da_role(const DaRoles& r) { return (int)(blockIdx.x / DA_XCDS % r.roles); }
 // The role's fields once more, read behind the loop: what only its end needs stays out of the scalar registers until then.
 __device__ __forceinline__ const DaCore& da_again(const DaRoles& r) {
@@ -278,7 +278,7 @@ __device__ __forceinline__ DaWave da_wave(const DaCore& a, int roles) {
   w.dv0 = w.slice * 16 * NV;
   w.len = da_length(a, w.n);
   w.last = da_last_segment(a, w.len);
-  w.begin = (int64_t)w.seg * a.seg_len;
+  w.begin = w.seg * a.seg_len;
   w.end = w.begin + a.seg_len < w.len ? w.begin + a.seg_len : w.len;
   return w;
 }
@@ -313,14 +313,14 @@ __device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, co
 #pragma unroll
       for (int sv = 0; sv < NV; ++sv) *reinterpret_cast<f32x4*>(slot + ((s * NV + sv) * WAVE + lane) * 4) = S[s][sv];
     if (w.slice == 0 && lane == 0) {
-      const int64_t count = (w.end > w.begin ? w.end - w.begin : 0) - (a.reverse && w.seg == 0 && w.end > 0 ? 1 : 0);
+      const int count = (w.end > w.begin ? w.end - w.begin : 0) - (a.reverse && w.seg == 0 && w.end > 0 ? 1 : 0);
       a.seg_factors[w.nh * a.nseg + w.seg] = dropped ? -1.f : (float)da_power(decay, count);
     }
     return;
   }
-  const int64_t stop = w.begin + a.seg_len < a.t ? w.begin + a.seg_len : a.t;
-  for (int64_t t = (w.begin > w.len ? w.begin : w.len) + c; t < stop; t += 16) {
-    const int64_t row = w.n * a.on + t * a.ot + (int64_t)w.h * a.oh;
+  const int stop = w.begin + a.seg_len < a.t ? w.begin + a.seg_len : a.t;
+  for (int t = (w.begin > w.len ? w.begin : w.len) + c; t < stop; t += 16) {
+    const int64_t row = w.n * a.on + (int64_t)t * a.ot + (int64_t)w.h * a.oh;
     const float none[4 * NV] = {};
     if (a.o_float) store_run<float, 4 * NV, MODE>(none, static_cast<float*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
     else store_run<T, 4 * NV, MODE>(none, static_cast<T*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
@@ -355,7 +355,7 @@ __device__ __forceinline__ void da_store_out(float* lds, const f32x4 (&acc)[NV],
 #pragma unroll
     for (int sv = 0; sv < NV; ++sv) out[sv] = lds[(4 * g + r) * LD + NV * c + sv];
     if (4 * g + r < b.L) {
-      const int64_t row = head + (b.low + b.row(4 * g + r)) * a.ot;
+      const int64_t row = head + (int64_t)(b.low + b.row(4 * g + r)) * a.ot;
       if (a.o_float) store_run<float, NV, MODE>(out, static_cast<float*>(a.o) + row, dv0 + NV * c, a.dv);
       else store_run<T, NV, MODE>(out, static_cast<T*>(a.o) + row, dv0 + NV * c, a.dv);
     }
@@ -373,7 +373,8 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const DaWave w = da_wave<NV>(a, roles.roles);
   if (!w.live || (STATES && w.seg >= w.last)) return;
-  const int64_t n = w.n, nh = w.nh, len = w.len, begin = w.begin, end = w.end;
+  const int64_t n = w.n;
+  const int len = w.len, begin = w.begin, end = w.end;
   const int h = w.h, seg = w.seg, slice = w.slice, dv0 = w.dv0;
 
   const T* qh = static_cast<const T*>(a.q.p) + n * a.q.sn + (int64_t)(h / a.q.group) * a.q.sh;
@@ -439,7 +440,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
   float head_w = 0.f, pair_w[4], tail_w[4], keep_hi = 0.f, keep_lo = 0.f, keep_off = 0.f;
   const uint32_t upto = (2u << c) - 1u;  // bits 0 .. i
 
-  for (int64_t p0 = begin; p0 < end; p0 += DA_TOKENS) {
+  for (int p0 = begin; p0 < end; p0 += DA_TOKENS) {
     const int L = blk.L;
     if (p0 == begin || p0 == DA_TOKENS || L < DA_TOKENS) {
       const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
@@ -591,6 +592,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 constexpr int DB_TOKENS = 32;
 
 __device__ __forceinline__ f32x4 db_mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -695,7 +697,7 @@ __device__ __forceinline__ void db_store_out(uint32_t* lds, const f32x4 (&acc)[2
     }
     const int i = 16 * it + c;
     if (a.o_float) {
-      if (i < b.L) store_run<float, 4 * NV, MODE>(out, static_cast<float*>(a.o) + head + (b.low + b.row(i)) * a.ot, dv0 + 4 * NV * g, a.dv);
+      if (i < b.L) store_run<float, 4 * NV, MODE>(out, static_cast<float*>(a.o) + head + (int64_t)(b.low + b.row(i)) * a.ot, dv0 + 4 * NV * g, a.dv);
     } else {
 #pragma unroll
       for (int e = 0; e < 2 * NV; ++e) lds[i * LD + 2 * NV * g + e] = db_pack(out[2 * e], out[2 * e + 1]);
@@ -703,16 +705,31 @@ __device__ __forceinline__ void db_store_out(uint32_t* lds, const f32x4 (&acc)[2
   }
   if (a.o_float) return;
   wave_lds_fence();
+  // what lane (c, g) stores of token e: NV elements, one word or half of one
+  const auto put = [&](uint16_t* at, int e) {
+    const int i = (e < 4 ? 0 : 12) + 4 * g + e;
+    if (NV == 2) *reinterpret_cast<uint32_t*>(at) = lds[i * LD + c];
+    else *at = reinterpret_cast<const uint16_t*>(lds + i * LD)[c];
+  };
+  const int col = dv0 + NV * c;
+  const bool in = MODE == ELEMS_FULL || col < a.dv;
+  uint16_t* first = static_cast<uint16_t*>(a.o) + head + (int64_t)b.low * a.ot;
+  if (b.L == DB_TOKENS) {  // as with the loads: 32 bits from the lane, the rest from the scalar unit
+    const uint32_t off = 2u * ((uint32_t)(b.reverse ? 12 - 4 * g : 4 * g) * (uint32_t)a.ot + (uint32_t)col);
+    if (in) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int i = (e < 4 ? 0 : 12) + 4 * g + e, col = dv0 + NV * c;
-    uint16_t* row = static_cast<uint16_t*>(a.o) + head + (b.low + b.row(i)) * a.ot;
-    if (NV == 2) {
-      const uint32_t x = lds[i * LD + c];
-      if (i < b.L && (MODE == ELEMS_FULL || col < a.dv)) *reinterpret_cast<uint32_t*>(row + col) = x;
-    } else {
-      const uint16_t x = reinterpret_cast<const uint16_t*>(lds + i * LD)[c];
-      if (i < b.L && (MODE == ELEMS_FULL || col < a.dv)) row[col] = x;
+      for (int e = 0; e < 8; ++e) {
+        const int step = b.reverse ? 3 - (e & 3) + (e < 4 ? 16 : 0) : (e & 3) + (e < 4 ? 0 : 16);
+        put(reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(first + (int64_t)step * a.ot) + off), e);
+      }
+    }
+    asm volatile("" ::: "memory");  // (keeps the branches' ends apart)
+  } else {
+    const int g0 = da_here(lane_id()) >> 4;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = (e < 4 ? 0 : 12) + 4 * g0 + e;
+      if (in && i < b.L) put(first + (int64_t)b.row(i) * a.ot + col, e);
     }
   }
   wave_lds_fence();
@@ -731,7 +748,8 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const DaWave w = da_wave<NV>(a, roles.roles);
   if (!w.live || (STATES && w.seg >= w.last)) return;
-  const int64_t n = w.n, len = w.len, begin = w.begin, end = w.end;
+  const int64_t n = w.n;
+  const int len = w.len, begin = w.begin, end = w.end;
   const int h = w.h, dv0 = w.dv0;
   __shared__ f32x4 lds_weights[DA_WAVES][4][WAVE];
   const __bf16* qh = static_cast<const __bf16*>(a.q.p) + n * a.q.sn + (int64_t)(h / a.q.group) * a.q.sh;
@@ -756,7 +774,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   const uint32_t q_group = group * qst, k_group = group * kst, v_group = group * vst;
   const auto step_of = [&](int e) { return rev ? 3 - (e & 3) + (e < 4 ? 16 : 0) : (e & 3) + (e < 4 ? 0 : 16); };
   const auto issue = [&](auto& run, const __bf16* head, int64_t st, uint32_t lane_off, const DaBlock& b, int off, int limit) {
-    const __bf16* base = head + b.low * st;
+    const __bf16* base = head + (int64_t)b.low * st;
     if (b.L == DB_TOKENS) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) run[e].issue(base + (int64_t)step_of(e) * st, lane_off, off, limit);
@@ -815,7 +833,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   // this lane's weights: within 16 tokens, from the first 16 to the last, and the two halves' up to the block's end
   f32x4* weights = &lds_weights[(threadIdx.x >> 6)][0][lane];
 
-  for (int64_t p0 = begin; p0 < end; p0 += DB_TOKENS) {
+  for (int p0 = begin; p0 < end; p0 += DB_TOKENS) {
     const int L = blk.L;
     if (p0 == begin || p0 == DB_TOKENS || L < DB_TOKENS) {
       const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
@@ -905,13 +923,14 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
         hi[1] = u32x4{x[4], x[6], x[8], x[10]};
         lo[1] = u32x4{x[5], x[7], x[9], x[11]};
       }
-      bool odd = false;  // infinite or NaN
+      u16x2 top = {0, 0};  // the largest magnitudes' bits
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v_run[e].take(V[e], dv0 + NV * c, a.dv);
 #pragma unroll
-        for (int i = 0; i < Bits<NV, MODE>::REGS; ++i) odd |= (V[e][i] & 0x7F80u) == 0x7F80u || (V[e][i] & 0x7F800000u) == 0x7F800000u;
+        for (int i = 0; i < Bits<NV, MODE>::REGS; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, V[e][i] & 0x7FFF7FFFu));
       }
+      const bool odd = top.x >= 0x7F80 || top.y >= 0x7F80;  // infinite or NaN
       if (__any(odd)) {
         // An infinite or NaN value: where a token sees it the result is NaN, everywhere else (its weight is zero) it is left out.
         const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
@@ -1240,7 +1259,7 @@ static int decay_attention_run(const DaRoles& in, const DaPlan& p, float* worksp
     DaCore& c = r.c[i];
     c.slices = p.slices;
     c.nseg = p.nseg;
-    c.seg_len = p.seg_len;
+    c.seg_len = (int)p.seg_len;
     if (p.nseg > 1) {
       c.seg_states = workspace + i * p.seg_floats;
       c.seg_factors = c.seg_states + heads * p.nseg * per_head * 4;
@@ -1322,7 +1341,7 @@ static int decay_attention_core(const DaRoles& r, int dtype, float* ws, hipStrea
     OIGE_REQUIRE(c.q.st >= 0 && c.q.st < most && c.k.st >= 0 && c.k.st < most && c.v.st >= 0 && c.v.st < most,
                  "decay_attention: token strides must be below 2^32 elements and not negative");
     wide = wide && da_wide(c, bytes);
-    bf16 = bf16 && c.q.st <= most_bf16 && c.k.st <= most_bf16 && c.v.st <= most_bf16;
+    bf16 = bf16 && c.q.st <= most_bf16 && c.k.st <= most_bf16 && c.v.st <= most_bf16 && c.ot <= most_bf16;
   }
   bf16 = bf16 && wide;
   const DaCore& c = r.c[0];
@@ -1355,7 +1374,7 @@ static int decay_attention_share(const float* in, void* out, const oige_decay_at
 static int decay_attention_check(const oige_decay_attention_io* io, const char* what) {
   OIGE_REQUIRE(io != nullptr, "%s: null io", what);
   OIGE_REQUIRE(elem_bytes(io->dtype), "%s: dtype must be OIGE_F32, OIGE_F16 or OIGE_BF16", what);
-  OIGE_REQUIRE(io->num_envs >= 0 && io->num_tokens >= 0 && io->num_tokens < ((int64_t)1 << 31), "%s: %lld sequences of %lld tokens", what,
+  OIGE_REQUIRE(io->num_envs >= 0 && io->num_tokens >= 0 && io->num_tokens < ((int64_t)1 << 30), "%s: %lld sequences of %lld tokens", what,
                (long long)io->num_envs, (long long)io->num_tokens);
   OIGE_REQUIRE(io->heads >= 1 && io->kv_heads >= 1 && io->heads % io->kv_heads == 0, "%s: %d heads over %d key / value heads", what, io->heads,
                io->kv_heads);
@@ -1400,7 +1419,7 @@ static DaCore da_core(const oige_decay_attention_io& io) {
   c.rsn = io.resets_stride[0];
   c.rst = io.resets_stride[1];
   c.n = io.num_envs;
-  c.t = io.num_tokens;
+  c.t = (int)io.num_tokens;
   c.h = io.heads;
   c.resets_bytes = io.resets_bytes;
   c.lengths_bytes = io.lengths_bytes;
