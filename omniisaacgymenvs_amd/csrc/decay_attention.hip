@@ -343,10 +343,10 @@ __device__ __forceinline__ void da_store_out(float* lds, const f32x4 (&acc)[NV],
   float* mine = lds + c * LD + 4 * NV * g;
 #pragma unroll
   for (int sv = 0; sv < NV; ++sv) {
-    mine[sv] = acc[sv].x * a.out_scale;
-    mine[NV + sv] = acc[sv].y * a.out_scale;
-    mine[2 * NV + sv] = acc[sv].z * a.out_scale;
-    mine[3 * NV + sv] = acc[sv].w * a.out_scale;
+    mine[sv] = acc[sv].x;
+    mine[NV + sv] = acc[sv].y;
+    mine[2 * NV + sv] = acc[sv].z;
+    mine[3 * NV + sv] = acc[sv].w;
   }
   wave_lds_fence();
 #pragma unroll
@@ -442,17 +442,17 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
 
   for (int p0 = begin; p0 < end; p0 += DA_TOKENS) {
     const int L = blk.L;
-    if (p0 == begin || p0 == DA_TOKENS || L < DA_TOKENS) {
+    if (p0 == begin || (a.reverse && p0 == DA_TOKENS) || L < DA_TOKENS) {
       const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
       const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
       const double keep = L - first == DA_TOKENS ? pw.d16 : da_power(decay, L - first);
       keep_hi = (float)keep;
       keep_lo = (float)(keep - (double)keep_hi);
-      head_w = pw(c + 1 - first);
+      head_w = pw(c + 1 - first) * a.out_scale;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = 4 * g + r;
-        pair_w[r] = j <= c ? pw(c - j) * a.kv_scale : 0.f;
+        pair_w[r] = j <= c ? pw(c - j) * a.kv_scale * a.out_scale : 0.f;
         tail_w[r] = j < L ? pw(L - 1 - j) * a.kv_scale : 0.f;
       }
     }
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
 //   S Q, P V     the 32-bit factor as a sum of two bf16 numbers (hi + lo; what is left out is at most 2^-18 of it), two products
 //   K^T (w V)    w V as a sum of three (at most 2^-27 of it is left out): the state stays a 32-bit sum
 // The operand that a product sums over lies packed along registers, eight to a lane: for tokens, lane group g holds 4 g + {0..3} and
-// 16 + 4 g + {0..3}, as K Q^T leaves them; for dk, the four rows of two neighbouring tiles, as the state keeps them.
+// 16 + 4 g + {0..3}, as K Q^T leaves them; for dk, the four rows of two neighbouring tiles side by side, as q's words hold them.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -642,6 +642,24 @@ struct Bits {
   }
 };
 
+// The scalar part of the addresses of a whole block's rows: lane group 0's in the order 0 .. 3, 16 .. 19, or in reverse, where
+// token i lies 31 - i rows behind the block's earliest, 19 .. 16, 3 .. 0.  CHAIN: each from the one before, where eight addresses
+// per tensor computed ahead of the loop are more than the scalar registers hold (52 of them went to vector registers; the kernel
+// that only makes states has room: 42 us against 50 with the chain, 64 sequences of 8192 tokens at most, 128 x 128).
+template <bool CHAIN>
+struct DbWalk {
+  const char* p;
+  int step;  // bytes; 16 of them are below 2^31: checked on the host
+  __device__ __forceinline__ DbWalk(const char* base, int64_t st, int reverse)
+      : p(base + (reverse ? 19 * 2 * st : 0)), step(reverse ? -2 * (int)st : 2 * (int)st) {}
+  __device__ __forceinline__ const char* at(int e) {  // e: 0, 1, .. 7
+    if (!CHAIN) return p + (e < 4 ? e : 12 + e) * (int64_t)step;
+    if (e > 0) p += e == 4 ? 13 * (int64_t)step : (int64_t)step;
+    asm volatile("" : "+s"(p));
+    return p;
+  }
+};
+
 // O^T's part from the state: for both halves of the block's tokens, the state's hi and lo parts against q.
 template <int NK, int NV>
 __device__ __forceinline__ void db_state_part(f32x4 (&acc)[2][NV], const f32x4 (&S)[NK][NV], const uint32_t (&Q)[2][2 * NK],
@@ -655,24 +673,21 @@ __device__ __forceinline__ void db_state_part(f32x4 (&acc)[2][NV], const f32x4 (
   for (int p = 0; p < NK / 2; ++p) {
     u32x4 q[2];
 #pragma unroll
-    for (int it = 0; it < 2; ++it) {
-      const uint32_t x0 = Q[it][p], x1 = Q[it][NK / 2 + p], x2 = Q[it][NK + p], x3 = Q[it][3 * NK / 2 + p];
-      q[it] = u32x4{db_lows(x0, x1), db_lows(x2, x3), db_highs(x0, x1), db_highs(x2, x3)};
-    }
+    for (int it = 0; it < 2; ++it)
+      q[it] = u32x4{Q[it][p], Q[it][NK / 2 + p], Q[it][NK + p], Q[it][3 * NK / 2 + p]};
 #pragma unroll
     for (int sv = 0; sv < NV; ++sv) {
       const f32x4 s0 = S[2 * p][sv], s1 = S[2 * p + 1][sv];
       uint32_t hi[4], lo[4];
-      db_split(s0.x, s0.y, hi[0], lo[0]);
-      db_split(s0.z, s0.w, hi[1], lo[1]);
-      db_split(s1.x, s1.y, hi[2], lo[2]);
-      db_split(s1.z, s1.w, hi[3], lo[3]);
+      db_split(s0.x, s1.x, hi[0], lo[0]);
+      db_split(s0.y, s1.y, hi[1], lo[1]);
+      db_split(s0.z, s1.z, hi[2], lo[2]);
+      db_split(s0.w, s1.w, hi[3], lo[3]);
       const u32x4 h{hi[0], hi[1], hi[2], hi[3]}, l{lo[0], lo[1], lo[2], lo[3]};
 #pragma unroll
-      for (int it = 0; it < 2; ++it) {
-        acc[it][sv] = db_mfma(l, q[it], acc[it][sv]);
-        acc[it][sv] = db_mfma(h, q[it], acc[it][sv]);
-      }
+      for (int it = 0; it < 2; ++it) acc[it][sv] = db_mfma(l, q[it], acc[it][sv]);
+#pragma unroll
+      for (int it = 0; it < 2; ++it) acc[it][sv] = db_mfma(h, q[it], acc[it][sv]);
     }
   }
 #pragma unroll
@@ -690,10 +705,10 @@ __device__ __forceinline__ void db_store_out(uint32_t* lds, const f32x4 (&acc)[2
     float out[4 * NV];
 #pragma unroll
     for (int sv = 0; sv < NV; ++sv) {
-      out[sv] = acc[it][sv].x * a.out_scale;
-      out[NV + sv] = acc[it][sv].y * a.out_scale;
-      out[2 * NV + sv] = acc[it][sv].z * a.out_scale;
-      out[3 * NV + sv] = acc[it][sv].w * a.out_scale;
+      out[sv] = acc[it][sv].x;
+      out[NV + sv] = acc[it][sv].y;
+      out[2 * NV + sv] = acc[it][sv].z;
+      out[3 * NV + sv] = acc[it][sv].w;
     }
     const int i = 16 * it + c;
     if (a.o_float) {
@@ -705,10 +720,11 @@ __device__ __forceinline__ void db_store_out(uint32_t* lds, const f32x4 (&acc)[2
   }
   if (a.o_float) return;
   wave_lds_fence();
-  // what lane (c, g) stores of token e: NV elements, one word or half of one
+  // what lane (c, g) stores of token e: NV elements, two words, one or half of one
   const auto put = [&](uint16_t* at, int e) {
     const int i = (e < 4 ? 0 : 12) + 4 * g + e;
-    if (NV == 2) *reinterpret_cast<uint32_t*>(at) = lds[i * LD + c];
+    if (NV == 4) *reinterpret_cast<Pack<uint32_t, 2>*>(at) = *reinterpret_cast<const Pack<uint32_t, 2>*>(lds + i * LD + 2 * c);
+    else if (NV == 2) *reinterpret_cast<uint32_t*>(at) = lds[i * LD + c];
     else *at = reinterpret_cast<const uint16_t*>(lds + i * LD)[c];
   };
   const int col = dv0 + NV * c;
@@ -716,12 +732,10 @@ __device__ __forceinline__ void db_store_out(uint32_t* lds, const f32x4 (&acc)[2
   uint16_t* first = static_cast<uint16_t*>(a.o) + head + (int64_t)b.low * a.ot;
   if (b.L == DB_TOKENS) {  // as with the loads: 32 bits from the lane, the rest from the scalar unit
     const uint32_t off = 2u * ((uint32_t)(b.reverse ? 12 - 4 * g : 4 * g) * (uint32_t)a.ot + (uint32_t)col);
+    DbWalk<true> walk(reinterpret_cast<const char*>(first), a.ot, b.reverse);
     if (in) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int step = b.reverse ? 3 - (e & 3) + (e < 4 ? 16 : 0) : (e & 3) + (e < 4 ? 0 : 16);
-        put(reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(first + (int64_t)step * a.ot) + off), e);
-      }
+      for (int e = 0; e < 8; ++e) put(reinterpret_cast<uint16_t*>(const_cast<char*>(walk.at(e)) + off), e);
     }
     asm volatile("" ::: "memory");  // (keeps the branches' ends apart)
   } else {
@@ -767,17 +781,16 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   Bits<NV, MODE> v_run[8];
   int64_t flag = 0;
   const uint32_t qst = (uint32_t)a.q.st, kst = (uint32_t)a.k.st, vst = (uint32_t)a.v.st;
-  // whole blocks: a lane's offset is the same in each, rows differ by a multiple of the token stride that the scalar base takes;
-  // in reverse token i lies 31 - i rows behind the block's earliest
+  // whole blocks: a lane's offset is the same in each, rows differ by a multiple of the token stride that the scalar base takes
   const int rev = a.reverse;
   const uint32_t group = rev ? 12 - 4 * g : 4 * g;
   const uint32_t q_group = group * qst, k_group = group * kst, v_group = group * vst;
-  const auto step_of = [&](int e) { return rev ? 3 - (e & 3) + (e < 4 ? 16 : 0) : (e & 3) + (e < 4 ? 0 : 16); };
   const auto issue = [&](auto& run, const __bf16* head, int64_t st, uint32_t lane_off, const DaBlock& b, int off, int limit) {
     const __bf16* base = head + (int64_t)b.low * st;
     if (b.L == DB_TOKENS) {
+      DbWalk<!STATES> walk(reinterpret_cast<const char*>(base), st, rev);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) run[e].issue(base + (int64_t)step_of(e) * st, lane_off, off, limit);
+      for (int e = 0; e < 8; ++e) run[e].issue(reinterpret_cast<const __bf16*>(walk.at(e)), lane_off, off, limit);
     } else {
       const int g = da_here(lane) >> 4;
 #pragma unroll
@@ -835,20 +848,20 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
 
   for (int p0 = begin; p0 < end; p0 += DB_TOKENS) {
     const int L = blk.L;
-    if (p0 == begin || p0 == DB_TOKENS || L < DB_TOKENS) {
+    if (p0 == begin || (rev && p0 == DB_TOKENS) || L < DB_TOKENS) {
       const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
       const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
       const double keep = L - first == DB_TOKENS ? pw.d32 : da_power(decay, L - first);
       keep_hi = (float)keep;
       keep_lo = (float)(keep - (double)keep_hi);
-      head_w[0] = pw(c + 1 - first);
-      head_w[1] = pw(c + 17 - first);
+      head_w[0] = pw(c + 1 - first) * a.out_scale;
+      head_w[1] = pw(c + 17 - first) * a.out_scale;
       float x[16];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = 4 * g + r;
-        x[r] = j <= c ? pw(c - j) * a.kv_scale : 0.f;
-        x[4 + r] = pw(16 + c - j) * a.kv_scale;
+        x[r] = j <= c ? pw(c - j) * a.kv_scale * a.out_scale : 0.f;
+        x[4 + r] = pw(16 + c - j) * a.kv_scale * a.out_scale;
         x[8 + r] = j < L ? pw(L - 1 - j) * a.kv_scale : 0.f;
         x[12 + r] = j + 16 < L ? pw(L - 17 - j) * a.kv_scale : 0.f;
       }
@@ -966,17 +979,19 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
         }
         da_settle();
       } else {
+        u32x4 v[NV];
 #pragma unroll
         for (int sv = 0; sv < NV; ++sv) {
           const int i = sv / 2;
-          const u32x4 v = sv & 1 ? u32x4{db_highs(V[0][i], V[1][i]), db_highs(V[2][i], V[3][i]), db_highs(V[4][i], V[5][i]), db_highs(V[6][i], V[7][i])}
-                                 : u32x4{db_lows(V[0][i], V[1][i]), db_lows(V[2][i], V[3][i]), db_lows(V[4][i], V[5][i]), db_lows(V[6][i], V[7][i])};
-#pragma unroll
-          for (int it = 0; it < 2; ++it) {
-            acc[it][sv] = db_mfma(v, lo[it], acc[it][sv]);
-            acc[it][sv] = db_mfma(v, hi[it], acc[it][sv]);
-          }
+          v[sv] = sv & 1 ? u32x4{db_highs(V[0][i], V[1][i]), db_highs(V[2][i], V[3][i]), db_highs(V[4][i], V[5][i]), db_highs(V[6][i], V[7][i])}
+                         : u32x4{db_lows(V[0][i], V[1][i]), db_lows(V[2][i], V[3][i]), db_lows(V[4][i], V[5][i]), db_lows(V[6][i], V[7][i])};
         }
+#pragma unroll
+        for (int part = 0; part < 2; ++part)  // (no product waits for the one just in front of it)
+#pragma unroll
+          for (int sv = 0; sv < NV; ++sv)
+#pragma unroll
+            for (int it = 0; it < 2; ++it) acc[it][sv] = db_mfma(v[sv], part ? hi[it] : lo[it], acc[it][sv]);
         da_settle();
       }
       db_store_out<NV, MODE, LD_OUT>(out, acc, a, blk, n * a.on + (int64_t)h * a.oh, dv0, c, g);
@@ -1054,12 +1069,11 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
       const u32x4 k = s & 1 ? u32x4{db_highs(kk[0], kk[1]), db_highs(kk[2], kk[3]), db_highs(kk[4], kk[5]), db_highs(kk[6], kk[7])}
                             : u32x4{db_lows(kk[0], kk[1]), db_lows(kk[2], kk[3]), db_lows(kk[4], kk[5]), db_lows(kk[6], kk[7])};
 #pragma unroll
-      for (int sv = 0; sv < NV; ++sv) {
-        S[s][sv] *= kept;
-        S[s][sv] = db_mfma(k, vl3[sv], S[s][sv]);
-        S[s][sv] = db_mfma(k, vm3[sv], S[s][sv]);
-        S[s][sv] = db_mfma(k, vh3[sv], S[s][sv]);
-      }
+      for (int sv = 0; sv < NV; ++sv) S[s][sv] *= kept;
+#pragma unroll
+      for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) S[s][sv] = db_mfma(k, part == 0 ? vl3[sv] : part == 1 ? vm3[sv] : vh3[sv], S[s][sv]);
     }
     wave_lds_fence();
     da_settle();
@@ -1213,21 +1227,26 @@ struct DaPlan {
 };
 
 // Tiles per wave: 16 NK rows cover dk, 16 NV columns are a slice of dv; at most 16 tiles (64 registers) of state.  Wider slices share
-// q, k and their product among more columns, narrower ones leave fewer columns empty behind dv: the width with the least
-// matrix instructions over all slices is taken.
+// q, k and their product among more columns (bf16, 64 x 64, 512 tokens of 4096 heads: 251 us with four tiles, 313 with two), narrower
+// ones leave fewer columns empty behind dv: the width with the least matrix instructions over all slices is taken.  Calls that
+// neither fill the chip nor have many tokens to a wave take narrower ones: the chain of one wave's blocks is what lasts (fp32,
+// 64 x 64, 128 tokens of 256 heads: 38 us with four tiles, 31 with two, 22 with one; with 2048 tokens four are the best).
 //
 // A call with fewer waves than the chip has SIMDs is cut over time, into pieces of 64 tokens at least: the pieces' end states first,
 // joined by one small launch, then every piece by itself; the aim is two waves per SIMD, or four where the sequences' lengths
-// differ (long bf16 prompts between a quarter and all of 8192 tokens: 280 us with two, 204 us with four; equal ones no difference).
-constexpr int64_t DA_FEW_WAVES = 1024, DA_WANT_WAVES = 2048, DA_MIN_SEGMENT = 64;
+// differ (long bf16 prompts between a quarter and all of 8192 tokens: 280 us with two, 204 us with four; equal ones no difference),
+// and not one more, which would run alone behind the others.
+constexpr int64_t DA_FEW_WAVES = 1024, DA_WANT_WAVES = 2048, DA_MIN_SEGMENT = 64, DA_WIDE_TOKENS = 12288;
 
 static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, bool bf16, int roles, bool ragged) {
   DaPlan p;
   p.nk = dk <= 16 && !bf16 ? 1 : dk <= 32 ? 2 : dk <= 64 ? 4 : 8;
   p.nv = 1;
   int64_t least = 0;
-  for (int nv = 1; nv <= (p.nk == 8 || bf16 ? 2 : 4); nv *= 2) {
+  for (int nv = 1; nv <= (p.nk == 8 ? 2 : 4); nv *= 2) {
     const int64_t slices = (dv + 16 * nv - 1) / (16 * nv), cost = slices * (4 * p.nk + 4 * nv + 8 * p.nk * nv);
+    const int64_t waves = n * h * slices * roles;  // (n and h are in the products the launch checks; t is below 2^30)
+    if (nv > 1 && waves < DA_FEW_WAVES && waves * t < DA_WIDE_TOKENS * nv * nv) break;
     if (nv == 1 || cost <= least) {
       least = cost;
       p.nv = nv;
@@ -1238,7 +1257,7 @@ static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, 
   p.nseg = 1;
   p.seg_len = t > 0 ? t : 1;
   if (waves < DA_FEW_WAVES && t >= 2 * DA_MIN_SEGMENT) {
-    int64_t want = ((ragged ? 2 : 1) * DA_WANT_WAVES + waves - 1) / waves;
+    int64_t want = (ragged ? 2 : 1) * DA_WANT_WAVES / waves;
     if (want > t / DA_MIN_SEGMENT) want = t / DA_MIN_SEGMENT;
     p.seg_len = (t + want - 1) / want;
     p.seg_len = (p.seg_len + DB_TOKENS - 1) / DB_TOKENS * DB_TOKENS;
@@ -1322,8 +1341,10 @@ static int decay_attention_bf16_tiles(const DaRoles& c, const DaPlan& p, float* 
   switch (p.nk * 8 + p.nv) {
     case 16 + 1: return decay_attention_run<__bf16, 2, 1, MODE, true>(c, p, ws, s);
     case 16 + 2: return decay_attention_run<__bf16, 2, 2, MODE, true>(c, p, ws, s);
+    case 16 + 4: return decay_attention_run<__bf16, 2, 4, MODE, true>(c, p, ws, s);
     case 32 + 1: return decay_attention_run<__bf16, 4, 1, MODE, true>(c, p, ws, s);
     case 32 + 2: return decay_attention_run<__bf16, 4, 2, MODE, true>(c, p, ws, s);
+    case 32 + 4: return decay_attention_run<__bf16, 4, 4, MODE, true>(c, p, ws, s);
     case 64 + 1: return decay_attention_run<__bf16, 8, 1, MODE, true>(c, p, ws, s);
     case 64 + 2: return decay_attention_run<__bf16, 8, 2, MODE, true>(c, p, ws, s);
   }
@@ -1390,7 +1411,9 @@ static int decay_attention_check(const oige_decay_attention_io* io, const char* 
 static bool da_square(const oige_decay_attention_io& io) {
   bool same = true;
   for (int bf16 = 0; bf16 < 2; ++bf16) {
-    const DaPlan a = decay_attention_plan(1, 1, 1, io.key_dim, io.value_dim, bf16, 1, false), b = decay_attention_plan(1, 1, 1, io.value_dim, io.key_dim, bf16, 1, false);
+    const bool ragged = io.lengths != nullptr;
+    const DaPlan a = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, io.key_dim, io.value_dim, bf16, 3, ragged);
+    const DaPlan b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, io.value_dim, io.key_dim, bf16, 3, ragged);
     same = same && a.nk == b.nk && a.nv == b.nv && a.slices == b.slices;
   }
   return same;

@@ -220,6 +220,16 @@ def test_decay_attention_lengths_are_clamped_and_empty_sequences_pass_the_state_
     assert o.shape == (0, 5, 2, 8) and state.shape == (0, 2, 16, 8)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, t, h, hk, dk, dv", [
+    (256, 37, 4, 2, 64, 64), (512, 20, 2, 2, 32, 64), (512, 35, 2, 1, 24, 56), (1024, 18, 1, 1, 16, 30), (1024, 34, 1, 1, 40, 32),
+    (1, 6300, 2, 2, 128, 120), (4, 1500, 16, 16, 32, 64)])
+def test_decay_attention_wide_slices_of_many_sequences(n, t, h, hk, dk, dv, dtype):
+    """Enough sequences, or tokens, for up to 64 columns of the state to a wave."""
+    kw, d_o, d_state = _attention_inputs(n, t, h, hk, dk, dv, dtype, 21, resets=0.04, ragged=n > 1)
+    _check_attention(kw, d_o, d_state)
+
+
 @pytest.mark.parametrize("decay", [0.0, 1.0, 1.01, 1e-30, 0.5])
 def test_decay_attention_extreme_decays(decay):
     kw, d_o, d_state = _attention_inputs(2, 150, 1, 1, 16, 16, torch.float32, 14, resets=0.02, decay=[decay])
