@@ -1233,7 +1233,9 @@ struct DaPlan {
 // 64 x 64, 128 tokens of 256 heads: 38 us with four tiles, 31 with two, 22 with one; with 2048 tokens four are the best).
 //
 // A call with fewer waves than the chip has SIMDs is cut over time, into pieces of 64 tokens at least: the pieces' end states first,
-// joined by one small launch, then every piece by itself; the aim is two waves per SIMD, or four where the sequences' lengths
+// joined by one small launch, then every piece by itself.  Two launches more cost about 10 us: below 192 tokens (256 in bf16) the
+// call stays whole (64 heads of 64 x 64, bf16: 128 tokens 18 us cut and 14 whole, 384 tokens 24 cut and 30 whole; fp32: 128 tokens
+// 21 and 19, 192 tokens 23 and 27).  The aim is two waves per SIMD, or four where the sequences' lengths
 // differ (long bf16 prompts between a quarter and all of 8192 tokens: 280 us with two, 204 us with four; equal ones no difference),
 // and not one more, which would run alone behind the others.
 constexpr int64_t DA_FEW_WAVES = 1024, DA_WANT_WAVES = 2048, DA_MIN_SEGMENT = 64, DA_WIDE_TOKENS = 12288;
@@ -1256,7 +1258,7 @@ static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, 
   const int64_t waves = n * h * p.slices * roles;
   p.nseg = 1;
   p.seg_len = t > 0 ? t : 1;
-  if (waves < DA_FEW_WAVES && t >= 2 * DA_MIN_SEGMENT) {
+  if (waves < DA_FEW_WAVES && t >= (bf16 ? 4 : 3) * DA_MIN_SEGMENT) {
     int64_t want = (ragged ? 2 : 1) * DA_WANT_WAVES / waves;
     if (want > t / DA_MIN_SEGMENT) want = t / DA_MIN_SEGMENT;
     p.seg_len = (t + want - 1) / want;
