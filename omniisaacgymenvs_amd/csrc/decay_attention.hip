@@ -1113,19 +1113,37 @@ __global__ __launch_bounds__(256) void decay_attention_join_kernel(const DaRoles
   }
 }
 
-// Gradients of shared key / value heads: the sum over the query heads that share one, from fp32 rows (N, T, H, d) -> T.
-template <typename T>
-__global__ __launch_bounds__(256) void decay_attention_share_kernel(const float* __restrict__ in, T* __restrict__ out, int64_t n, int64_t t,
-                                                                    int hk, int group, int d, int64_t on, int64_t ot, int64_t oh) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n * t * hk * d) return;
-  const int e = (int)(i % d);
-  const int64_t r = i / d;  // (n, t, hk)
-  const int head = (int)(r % hk);
-  const int64_t nt = r / hk;
-  float v = 0.f;
-  for (int k = 0; k < group; ++k) v += in[((r * group) + k) * d + e];
-  out[(nt / t) * on + (nt % t) * ot + head * oh + e] = (T)v;
+// Gradients of shared key / value heads: the sum over the query heads that share one, from fp32 rows (N, T, H, d) -> T, of k's and
+// v's heads in one launch.  Bound by the fp32 rows' read (mostly from the caches that they were just written through).  A thread
+// adds up VEC columns; the 64-bit divisions that find its row are the workgroup's, once: with one element and its own divisions
+// to a thread, 64 x 512 tokens of 8 heads over 2, 64 x 64 in bf16, took 2 x 23 us; now 23 us, 6.4 TB/s.
+struct DaShare {
+  const float* in;
+  void* out;
+  int64_t on, ot, oh;
+  int d;
+};
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void decay_attention_share_kernel(const DaShare of_k, const DaShare of_v, int64_t rows, int t, int hk, int group) {
+  const DaShare a = blockIdx.y ? of_v : of_k;
+  const int per = a.d / VEC, each = 256 / per, mine = (int)threadIdx.x / per, e = ((int)threadIdx.x - mine * per) * VEC;
+  const int64_t first = (int64_t)blockIdx.x * each;  // rows (n, t, hk)
+  if (mine >= each || first + mine >= rows) return;
+  const int64_t first_nt = first / hk, first_n = first_nt / t;
+  const int head_raw = (int)(first - first_nt * hk) + mine, t_raw = (int)(first_nt - first_n * t) + head_raw / hk;
+  const int head = head_raw % hk, n_more = t_raw / t;
+  const float* in = a.in + ((first + mine) * group) * a.d + e;
+  float v[VEC] = {};
+#pragma unroll 4
+  for (int k = 0; k < group; ++k) {
+    const Pack<float, VEC> x = *reinterpret_cast<const Pack<float, VEC>*>(in + k * a.d);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] += x.v[i];
+  }
+  Pack<T, VEC> y;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) y.v[i] = (T)v[i];
+  *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.out) + (first_n + n_more) * a.on + (int64_t)(t_raw - n_more * t) * a.ot + head * a.oh + e) = y;
 }
 
 // ---------------------------------------------------------------- one token per sequence, the state updated in place
@@ -1380,13 +1398,23 @@ static int decay_attention_core(const DaRoles& r, int dtype, float* ws, hipStrea
               : wide ? decay_attention_tiles<float, ELEMS_WIDE>(r, p, ws, s) : decay_attention_tiles<float, ELEMS_SINGLE>(r, p, ws, s);
 }
 
-static int decay_attention_share(const float* in, void* out, const oige_decay_attention_io& io, int d, const int64_t* stride, hipStream_t s) {
-  const int64_t total = io.num_envs * io.num_tokens * io.kv_heads * d, blocks = (total + 255) / 256;
+static int decay_attention_share(const float* in_k, const float* in_v, const oige_decay_attention_io& io, hipStream_t s) {
+  const int64_t *sk = io.dk_stride, *sv = io.dv_stride;
+  const DaShare k{in_k, io.dk, sk[0], sk[1], sk[2], io.key_dim}, v{in_v, io.dv, sv[0], sv[1], sv[2], io.value_dim};
+  bool wide = true;  // four columns to a thread
+  for (const DaShare& x : {k, v})
+    wide = wide && x.d % 4 == 0 && x.on % 4 == 0 && x.ot % 4 == 0 && x.oh % 4 == 0 && aligned16(x.in) && aligned16(x.out);
+  const int64_t rows = io.num_envs * io.num_tokens * io.kv_heads;
+  const int d = io.key_dim > io.value_dim ? io.key_dim : io.value_dim, each = 256 / (wide ? d / 4 : d);
+  const int64_t blocks = (rows + each - 1) / each;
   OIGE_REQUIRE(blocks < ((int64_t)1 << 31), "decay_attention_backward: too many key / value rows for one launch");
-  const int group = io.heads / io.kv_heads;
-#define OIGE_SHARE(T)                                                                                                                        \
-  hipLaunchKernelGGL((decay_attention_share_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, in, static_cast<T*>(out), io.num_envs,       \
-                     io.num_tokens, (int)io.kv_heads, group, d, stride[0], stride[1], stride[2])
+  const dim3 grid((unsigned)blocks, 2);
+  const int t = (int)io.num_tokens, hk = (int)io.kv_heads, group = io.heads / io.kv_heads;
+#define OIGE_SHARE(T)                                                                                                                    \
+  do {                                                                                                                                   \
+    if (wide) hipLaunchKernelGGL((decay_attention_share_kernel<T, 4>), grid, dim3(256), 0, s, k, v, rows, t, hk, group);                 \
+    else hipLaunchKernelGGL((decay_attention_share_kernel<T, 1>), grid, dim3(256), 0, s, k, v, rows, t, hk, group);                      \
+  } while (0)
   if (io.dtype == OIGE_F32) OIGE_SHARE(float);
   else if (io.dtype == OIGE_F16) OIGE_SHARE(_Float16);
   else OIGE_SHARE(__bf16);
@@ -1569,8 +1597,7 @@ int oige_decay_attention_backward(const oige_decay_attention_io* io, oige_stream
     }
   }
   if (group == 1) return OIGE_OK;
-  rc = decay_attention_share(wide_v, io->dv, *io, io->value_dim, io->dv_stride, s);
-  return rc ? rc : decay_attention_share(wide_k, io->dk, *io, io->key_dim, io->dk_stride, s);
+  return decay_attention_share(wide_k, wide_v, *io, s);
 }
 
 int oige_decay_attention_step(const oige_decay_attention_step_io* io, oige_stream_t stream) {

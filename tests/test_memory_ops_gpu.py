@@ -230,6 +230,14 @@ def test_decay_attention_wide_slices_of_many_sequences(n, t, h, hk, dk, dv, dtyp
     _check_attention(kw, d_o, d_state)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, t, h, hk, dk, dv", [(5, 7, 6, 3, 20, 12), (9, 1, 10, 5, 8, 128), (2, 50, 14, 2, 7, 9), (3, 70, 4, 1, 4, 6)])
+def test_decay_attention_shared_heads(n, t, h, hk, dk, dv, dtype):
+    """Sums over query heads whose rows end inside a workgroup's."""
+    kw, d_o, d_state = _attention_inputs(n, t, h, hk, dk, dv, dtype, 22, resets=0.1)
+    _check_attention(kw, d_o, d_state)
+
+
 @pytest.mark.parametrize("decay", [0.0, 1.0, 1.01, 1e-30, 0.5])
 def test_decay_attention_extreme_decays(decay):
     kw, d_o, d_state = _attention_inputs(2, 150, 1, 1, 16, 16, torch.float32, 14, resets=0.02, decay=[decay])
