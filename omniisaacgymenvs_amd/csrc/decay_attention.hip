@@ -8,15 +8,27 @@
 // so the backward pass is the forward recurrence with exchanged roles: dq reads (do, v, k) over S^T, dv reads (k, q, do) over G and
 // dk reads (v, do, q) over G^T, the last two from the last token to the first.  One kernel serves all four.
 //
-// A wave owns one sequence, one head and 16 NV columns of the state, which it keeps in registers as the accumulator tiles of
-// v_mfma_f32_16x16x4_f32 while it walks the tokens in blocks of 16:
-//   P  = (Q K^T) o decay^(i-j)                  16 x 16, only j <= i with no reset in (j, i]
+// A wave owns one sequence, one head and 16 NV columns of the state, which it keeps in registers as the accumulator tiles of the
+// matrix instructions while it walks the tokens in blocks of B = 16 (fp32, fp16) or 32 (bf16):
+//   P  = (Q K^T) o decay^(i-j)                  B x B, only j <= i with no reset in (j, i]
 //   O  = P V + decay^(i+1) Q S
-//   S <- decay^16 S + (decay^(15-j) K)^T V
-// Every product is a 32-bit matrix instruction on operands widened from the tensors' type, so no intermediate is rounded to
-// fewer bits.  The transposed forms are taken (P^T = K Q^T, O^T = V^T P^T + S^T Q^T): P^T and S then come out of one product in the very
-// register layout the next one takes them in, and nothing goes through LDS.  The order of the dk (dv) columns over tiles is
-// the kernel's own: tile s, row m holds dk = NK m + s, so that every lane's operand elements are neighbours in memory.
+//   S <- decay^B S + (decay^(B-1-j) K)^T V
+// The transposed forms are taken (P^T = K Q^T, O^T = V^T P^T + S^T Q^T): P^T and S then come out of one product in the very register
+// layout the next one takes them in.  The order of the dk (dv) columns over tiles is the kernel's own: tile s, row m holds
+// dk = NK m + s, so that every lane's operand elements are neighbours in memory.  Only rows go through LDS: they come in and leave as
+// 16 lanes read and write them side by side, and turn there into a token to a lane (64 tokens of 4096 time-major rollouts, whose
+// rows lie 4 MiB apart: 338 us, 2032 us with every lane reading a row of its own).
+//
+// Two kernels: v_mfma_f32_16x16x4_f32 on operands widened to fp32, which rounds nothing to fewer bits, and for bf16 tensors
+// v_mfma_f32_16x16x32_bf16 with the 32-bit factors split into bf16 numbers.  What bounds them:
+//   short sequences: HBM, for q, k, v, o and the states.  4096 environments x 4 heads x 16 tokens, 64 x 64, fp32: forward 170 us
+//     (805 MB, 4.7 TB/s; the copy rate is 5.4), backward 350 us (1.27 GB once, 3.6 TB/s).  Of the 28
+//     thousand cycles of a backward wave 17 pass until its first rows and its state are there; the three roles read them once from
+//     HBM and three times from the L2.
+//   long ones: the chain of a wave's blocks.  A bf16 block of 32 tokens with 64 x 64 of state is 100 matrix and 800 ordinary
+//     instructions and takes a wave 10.7 thousand cycles (state's part 3.4, state's update 2.2, rows through LDS 1.8, P V 1.0, loads
+//     and weights the rest): dependent instructions follow each other after 8 cycles, not 4, and two waves are all that a SIMD's
+//     registers hold.  2 sequences x 16 heads x 4096 tokens: forward 49 us (states 16, join 8, main 25), backward 90 (28, 11, 51).
 #include "oige_elem.hpp"
 
 namespace oige {
@@ -254,7 +266,14 @@ struct DaWave {
   int len, begin, end, h, seg, last, slice, dv0;  // last: the segment that the sequence ends in; those behind it only clear their rows
   bool live;
 };
-__device__ __forceinline__ int da_last_segment(const DaCore& a, int len) { return len > 0 ? (len - 1) / a.seg_len : 0; }
+// A sequence's tokens are cut evenly over all segments where the lengths differ, into pieces of DA_MIN_SEGMENT at least.
+constexpr int DA_MIN_SEGMENT = 64;
+__device__ __forceinline__ int da_segment(const DaCore& a, int len) {
+  if (!a.lengths || a.nseg == 1) return a.seg_len;
+  const int each = (int)(((uint32_t)(len + a.nseg - 1) / (uint32_t)a.nseg + 31u) & ~31u);
+  return each > DA_MIN_SEGMENT ? each : DA_MIN_SEGMENT;
+}
+__device__ __forceinline__ int da_last_segment(const DaCore& a, int len) { return len > 0 ? (int)((uint32_t)(len - 1) / (uint32_t)da_segment(a, len)) : 0; }
 __device__ __forceinline__ int da_role(const DaRoles& r) { return (int)(blockIdx.x / DA_XCDS % r.roles); }
 // The role's fields once more, read behind the loop: what only its end needs stays out of the scalar registers until then.
 __device__ __forceinline__ const DaCore& da_again(const DaRoles& r) {
@@ -277,9 +296,10 @@ __device__ __forceinline__ DaWave da_wave(const DaCore& a, int roles) {
   w.n = n;
   w.dv0 = w.slice * 16 * NV;
   w.len = da_length(a, w.n);
-  w.last = da_last_segment(a, w.len);
-  w.begin = w.seg * a.seg_len;
-  w.end = w.begin + a.seg_len < w.len ? w.begin + a.seg_len : w.len;
+  const int each = da_segment(a, w.len);
+  w.last = w.len > 0 ? (int)((uint32_t)(w.len - 1) / (uint32_t)each) : 0;
+  w.begin = w.seg * each;
+  w.end = w.begin + each < w.len ? w.begin + each : w.len;
   return w;
 }
 
@@ -302,7 +322,7 @@ __device__ __forceinline__ void da_open(f32x4 (&S)[NK][NV], const DaCore& a, con
   }
 }
 
-// ... and what becomes of the one behind its last; rows behind the sequence's end inside this segment's stretch are cleared.
+// ... and what becomes of the one behind its last; of the rows behind the sequence's end this segment's share (of all rows) is cleared.
 template <typename T, int NK, int NV, int MODE, bool STATES>
 __device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, const DaWave& w, int lane, double decay, bool dropped) {
   const int c = lane & 15, g = lane >> 4;
@@ -318,8 +338,8 @@ __device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, co
     }
     return;
   }
-  const int stop = w.begin + a.seg_len < a.t ? w.begin + a.seg_len : a.t;
-  for (int t = (w.begin > w.len ? w.begin : w.len) + c; t < stop; t += 16) {
+  const int start = w.seg * a.seg_len, stop = start + a.seg_len < a.t ? start + a.seg_len : a.t;
+  for (int t = (start > w.len ? start : w.len) + c; t < stop; t += 16) {
     const int64_t row = w.n * a.on + (int64_t)t * a.ot + (int64_t)w.h * a.oh;
     const float none[4 * NV] = {};
     if (a.o_float) store_run<float, 4 * NV, MODE>(none, static_cast<float*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
@@ -364,6 +384,9 @@ __device__ __forceinline__ void da_store_out(float* lds, const f32x4 (&acc)[NV],
 }
 
 // STATES: only the states at the segments' ends (no q, no o), for sequences cut over time.
+//
+// Rollouts of 16 tokens as above: 169 us forward and 352 backward with two waves per SIMD and 64 columns; 182 and 369 with three waves
+// and nothing asked for ahead; 228 and 244 us forward with 32 and 16 columns.
 //
 // The next block's rows are asked for as soon as the registers of this block's are free: q and the first copy of k behind the
 // products that read them, the other copy and v at the end, so that their way from memory runs beside the matrix instructions.
@@ -1083,7 +1106,9 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
 }
 
 // The states in front of every segment from those at the segments' ends (in place, register order): carry = factor carry + end.
-// Segment 0's end already holds the initial state.  A thread owns four floats of one (sequence, head) over all segments.
+// Segment 0's end already holds the initial state.  A thread owns four floats of one (sequence, head) over all segments, eight of
+// them in flight.  It moves the states once each way (64 heads' 128 x 128 over 8 segments, 2 x 34 MB: 11 us; 32 heads' 64 x 64
+// over 32 segments, 2 x 17 MB: 8 us), mostly from and to the caches; 16 in flight are no faster.
 __global__ __launch_bounds__(256) void decay_attention_join_kernel(const DaRoles roles, int64_t quads, int64_t per_head, int nseg) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= quads) return;
@@ -1149,7 +1174,8 @@ __global__ __launch_bounds__(256) void decay_attention_share_kernel(const DaShar
 // ---------------------------------------------------------------- one token per sequence, the state updated in place
 // Bound by the state's one read and one write (8 bytes per entry).  A wave (or a workgroup of four, for states of more than
 // 8 KiB) owns one (sequence, head): lanes take 16-byte pieces of the state's rows, update them where they are and add
-// q's product up over the rows they hold, then over the lanes and waves that share a column.
+// q's product up over the rows they hold, then over the lanes and waves that share a column.  4096 environments x 4 heads, 64 x 64: 100 us,
+// 5.3 TB/s; 1024 x 16 heads, 128 x 128: 413 us, 5.2 TB/s; one environment: 4 us, a launch's latency.
 struct DaStep {
   const void *q, *k, *v;
   void* o;
@@ -1253,12 +1279,12 @@ struct DaPlan {
 // A call with fewer waves than the chip has SIMDs is cut over time, into pieces of 64 tokens at least: the pieces' end states first,
 // joined by one small launch, then every piece by itself.  Two launches more cost about 10 us: below 192 tokens (256 in bf16) the
 // call stays whole (64 heads of 64 x 64, bf16: 128 tokens 18 us cut and 14 whole, 384 tokens 24 cut and 30 whole; fp32: 128 tokens
-// 21 and 19, 192 tokens 23 and 27).  The aim is two waves per SIMD, or four where the sequences' lengths
-// differ (long bf16 prompts between a quarter and all of 8192 tokens: 280 us with two, 204 us with four; equal ones no difference),
-// and not one more, which would run alone behind the others.
-constexpr int64_t DA_FEW_WAVES = 1024, DA_WANT_WAVES = 2048, DA_MIN_SEGMENT = 64, DA_WIDE_TOKENS = 12288;
+// 21 and 19, 192 tokens 23 and 27).  The aim is two waves per SIMD, and not one more, which would run alone behind the others.
+// Where lengths differ every sequence's own tokens are cut evenly (bf16 prompts between a quarter and all of 8192 tokens, 4 x 16 heads
+// of 128 x 128, mean of eight draws: 231 us; 252 with pieces of the same length in all, 247 with twice as many of them).
+constexpr int64_t DA_FEW_WAVES = 1024, DA_WANT_WAVES = 2048, DA_WIDE_TOKENS = 12288;
 
-static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, bool bf16, int roles, bool ragged) {
+static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, bool bf16, int roles) {
   DaPlan p;
   p.nk = dk <= 16 && !bf16 ? 1 : dk <= 32 ? 2 : dk <= 64 ? 4 : 8;
   p.nv = 1;
@@ -1277,7 +1303,7 @@ static DaPlan decay_attention_plan(int64_t n, int64_t t, int h, int dk, int dv, 
   p.nseg = 1;
   p.seg_len = t > 0 ? t : 1;
   if (waves < DA_FEW_WAVES && t >= (bf16 ? 4 : 3) * DA_MIN_SEGMENT) {
-    int64_t want = (ragged ? 2 : 1) * DA_WANT_WAVES / waves;
+    int64_t want = DA_WANT_WAVES / waves;
     if (want > t / DA_MIN_SEGMENT) want = t / DA_MIN_SEGMENT;
     p.seg_len = (t + want - 1) / want;
     p.seg_len = (p.seg_len + DB_TOKENS - 1) / DB_TOKENS * DB_TOKENS;
@@ -1386,7 +1412,7 @@ static int decay_attention_core(const DaRoles& r, int dtype, float* ws, hipStrea
   }
   bf16 = bf16 && wide;
   const DaCore& c = r.c[0];
-  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, bf16, r.roles, c.lengths != nullptr);
+  const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, bf16, r.roles);
   bool full = wide;
   for (int i = 0; i < r.roles; ++i) full = full && r.c[i].dk == 16 * p.nk && r.c[i].dv == 16 * p.nv * p.slices;
   if (bf16) return full ? decay_attention_bf16_tiles<ELEMS_FULL>(r, p, ws, s) : decay_attention_bf16_tiles<ELEMS_WIDE>(r, p, ws, s);
@@ -1441,16 +1467,15 @@ static int decay_attention_check(const oige_decay_attention_io* io, const char* 
 static bool da_square(const oige_decay_attention_io& io) {
   bool same = true;
   for (int bf16 = 0; bf16 < 2; ++bf16) {
-    const bool ragged = io.lengths != nullptr;
-    const DaPlan a = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, io.key_dim, io.value_dim, bf16, 3, ragged);
-    const DaPlan b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, io.value_dim, io.key_dim, bf16, 3, ragged);
+    const DaPlan a = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, io.key_dim, io.value_dim, bf16, 3);
+    const DaPlan b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, io.value_dim, io.key_dim, bf16, 3);
     same = same && a.nk == b.nk && a.nv == b.nv && a.slices == b.slices;
   }
   return same;
 }
 static int64_t da_seg_floats(const oige_decay_attention_io& io, int dk, int dv, int roles) {
-  const int64_t f = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, false, roles, io.lengths != nullptr).seg_floats;
-  const int64_t b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, true, roles, io.lengths != nullptr).seg_floats;
+  const int64_t f = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, false, roles).seg_floats;
+  const int64_t b = decay_attention_plan(io.num_envs, io.num_tokens, io.heads, dk, dv, true, roles).seg_floats;
   return ((f > b && io.dtype == OIGE_BF16) || io.dtype != OIGE_BF16 ? f : b) * roles;
 }
 static int64_t da_workspace(const oige_decay_attention_io& io, bool backward) {

@@ -9,6 +9,9 @@
 // ones take a workgroup (reductions through LDS).  The weight's and the bias's gradients are kept per lane in registers over
 // all rows a workgroup walks, written as one partial row per workgroup and added up by a second launch in a fixed order
 // (no atomics: the result does not depend on scheduling).
+//
+// Forward 262144 x 1024 bf16: 222 us, 4.8 TB/s (the copy rate is 5.4; without the next row in flight 268 us); 65536 x 211 fp32: 21 us;
+// one row: 5 us, a launch's latency.  Forward + backward 65536 x 512 bf16: 32 + 37 us, and 4 for the partial rows' sum.
 #include "oige_elem.hpp"
 
 namespace oige {
