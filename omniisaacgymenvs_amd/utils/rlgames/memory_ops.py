@@ -221,6 +221,7 @@ def _check_heads(what, q, k, v, decay, state, resets, lead):
 
 
 _NO3, _NO2 = (0, 0, 0), (0, 0)
+_workspace_floats: dict = {}  # by sizes, type and direction, which is all that the size depends on
 
 
 def _attention(fn, q, k, v, decay, state, resets, lengths, scale, o=None, state_out=None, d_o=None, d_state=None, dq=None, dk=None, dv=None,
@@ -237,14 +238,17 @@ def _attention(fn, q, k, v, decay, state, resets, lengths, scale, o=None, state_
             *(_NO2 if resets is None else resets.stride()), n, t, h, v.shape[2], key_dim, v.shape[3], _TYPES[q.dtype],
             0 if resets is None else resets.element_size(), 0 if lengths is None else lengths.element_size(), scale)
 
-    call = block(0, 0)
-    size = _lib.load().oige_decay_attention_workspace_floats(call, o is None)
-    if size:
+    key = (n, t, h, v.shape[2], key_dim, v.shape[3], q.dtype, o is None)
+    size = _workspace_floats.get(key)
+    if size is None:
+        size = _lib.load().oige_decay_attention_workspace_floats(block(0, 0), o is None)
         if size < 0:
             _lib.check(int(size), "oige_decay_attention_workspace_floats")
-        ws = torch.empty(size, dtype=torch.float32, device=q.device)
-        call = block(ws.data_ptr(), size)
-    _call(fn, call, q.device)
+        if len(_workspace_floats) >= 1024:
+            _workspace_floats.clear()
+        _workspace_floats[key] = size
+    ws = torch.empty(size, dtype=torch.float32, device=q.device) if size else None
+    _call(fn, block(_ptr(ws), size), q.device)
 
 
 def _attention_forward(q, k, v, state, decay, resets, lengths, scale, return_state):
