@@ -121,6 +121,10 @@ struct DaPowers {  // decay^n for n in 0 .. 32 without a loop, within 5 rounding
 
 // This wave's piece of a state matrix in memory: tile (s, sv), register r, lane (c, g) holds dk = NK (4 g + r) + s,
 // dv = dv0 + NV c + sv.
+//
+// ELEMS_LOOSE: rows that start on no boundary, or head sizes of no whole vectors.  A group of NK (NV) neighbouring columns that
+// reaches across the end is moved forward to end with the row.  What a state's row or column holds twice by that is
+// computed twice, to the same bits, and stored twice; only q's doubles are cleared, so that sums over dk count every column once.
 // Row `row + lane_row` of a matrix of `width` columns from column `col` on.  Whole tiles: the scalar unit takes the row's part that
 // all lanes share, a lane adds 32 bits.  Else row 0 stands in for rows behind the end.
 template <int MODE>
@@ -133,6 +137,32 @@ __device__ __forceinline__ const float* da_state_row(const float* p, int row, in
 
 template <int NK, int NV, int MODE>
 __device__ __forceinline__ void da_load_state(f32x4 (&S)[NK][NV], const float* p, const DaCore& a, int dv0, int c, int g) {
+  if (MODE == ELEMS_LOOSE) {
+    const int v0 = run_start<NV, MODE>(dv0 + NV * c, a.dv);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k0 = run_start<NK, MODE>(NK * (4 * g + r), a.dk);
+      if (a.transposed) {
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) {
+          float x[NK];
+          load_run<float, NK, MODE>(x, p + (v0 + sv) * a.dk, k0, a.dk);
+#pragma unroll
+          for (int s = 0; s < NK; ++s) S[s][sv][r] = x[s];
+        }
+        asm volatile("" ::: "memory");
+      } else {
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+          float x[NV];
+          load_run<float, NV, MODE>(x, p + (k0 + s) * a.dv, v0, a.dv);
+#pragma unroll
+          for (int sv = 0; sv < NV; ++sv) S[s][sv][r] = x[sv];
+        }
+      }
+    }
+    return;
+  }
   if (a.transposed) {
 #pragma unroll
     for (int sv = 0; sv < NV; ++sv) {
@@ -160,6 +190,31 @@ __device__ __forceinline__ void da_load_state(f32x4 (&S)[NK][NV], const float* p
 
 template <int NK, int NV, int MODE>
 __device__ __forceinline__ void da_store_state(const f32x4 (&S)[NK][NV], float* p, const DaCore& a, int dv0, int c, int g) {
+  if (MODE == ELEMS_LOOSE) {
+    const int v0 = run_start<NV, MODE>(dv0 + NV * c, a.dv);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k0 = run_start<NK, MODE>(NK * (4 * g + r), a.dk);
+      if (a.transposed) {
+#pragma unroll
+        for (int sv = 0; sv < NV; ++sv) {
+          float x[NK];
+#pragma unroll
+          for (int s = 0; s < NK; ++s) x[s] = S[s][sv][r];
+          store_run<float, NK, MODE>(x, p + (v0 + sv) * a.dk, k0, a.dk);
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+          float x[NV];
+#pragma unroll
+          for (int sv = 0; sv < NV; ++sv) x[sv] = S[s][sv][r];
+          store_run<float, NV, MODE>(x, p + (k0 + s) * a.dv, v0, a.dv);
+        }
+      }
+    }
+    return;
+  }
   if (a.transposed) {
 #pragma unroll
     for (int sv = 0; sv < NV; ++sv) {
@@ -303,6 +358,22 @@ __device__ __forceinline__ DaWave da_wave(const DaCore& a, int roles) {
   return w;
 }
 
+// Four neighbouring groups of NV columns of a result's row, from `off` on.
+template <typename T, int NV, int MODE>
+__device__ __forceinline__ void da_store_groups(const float (&x)[4 * NV], T* row, int off, int limit) {
+  if (MODE != ELEMS_LOOSE) {
+    store_run<T, 4 * NV, MODE>(x, row, off, limit);
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float y[NV];
+#pragma unroll
+    for (int sv = 0; sv < NV; ++sv) y[sv] = x[NV * r + sv];
+    store_run<T, NV, MODE>(y, row, off + NV * r, limit);
+  }
+}
+
 // The state in front of the segment's first token ...
 template <int NK, int NV, int MODE, bool STATES>
 __device__ __forceinline__ void da_open(f32x4 (&S)[NK][NV], const DaCore& a, const DaWave& w, int lane) {
@@ -342,8 +413,8 @@ __device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, co
   for (int t = (start > w.len ? start : w.len) + c; t < stop; t += 16) {
     const int64_t row = w.n * a.on + (int64_t)t * a.ot + (int64_t)w.h * a.oh;
     const float none[4 * NV] = {};
-    if (a.o_float) store_run<float, 4 * NV, MODE>(none, static_cast<float*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
-    else store_run<T, 4 * NV, MODE>(none, static_cast<T*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
+    if (a.o_float) da_store_groups<float, NV, MODE>(none, static_cast<float*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
+    else da_store_groups<T, NV, MODE>(none, static_cast<T*>(a.o) + row, w.dv0 + 4 * NV * g, a.dv);
   }
   if (a.s_out && w.seg == w.last) {
     if (a.reverse && w.len > 0) {  // dS_0 = a_0 G_0
@@ -430,13 +501,19 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
 #pragma unroll
     for (auto& x : run) x.forget();
   };
-  const auto put_rows = [&](const Run<T, NK, MODE> (&run)[4]) {
+  const auto put_rows = [&](const Run<T, NK, MODE> (&run)[4], bool once) {  // once: columns held twice are cleared the second time
+    uint32_t in[NK];
+    if (MODE == ELEMS_LOOSE) {
+      const int off = NK * (da_here(lane) & 15), twice = off - run_start<NK, MODE>(off, a.dk);
+#pragma unroll
+      for (int s = 0; s < NK; ++s) in[s] = bits_if(s >= twice);
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float x[NK];
       run[r].take(x, NK * c, a.dk);
 #pragma unroll
-      for (int s = 0; s < NK; ++s) lds[(4 * g + r) * LD + NK * c + s] = x[s];
+      for (int s = 0; s < NK; ++s) lds[(4 * g + r) * LD + NK * c + s] = MODE == ELEMS_LOOSE && once ? and_bits(x[s], in[s]) : x[s];
     }
     wave_lds_fence();
   };
@@ -488,11 +565,11 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     float V[4][NV], K2[4][NK];
     if (!STATES) {
       float Q[4 * NK], K1[4 * NK];
-      put_rows(q_run);
+      put_rows(q_run, true);
       get_token(Q);
       if (more) issue_q(next);
       else forget(q_run);
-      put_rows(k_run);
+      put_rows(k_run, false);
       get_token(K1);
       if (more) issue_k(next);
       else forget(k_run);
@@ -649,8 +726,13 @@ struct Bits {
     constexpr int W = Run<uint16_t, CNT, MODE>::W;
 #pragma unroll
     for (int b = 0; b < CNT / W; ++b) {
-      const uint32_t at = 2u * (row + (uint32_t)(MODE == ELEMS_FULL || off + b * W < limit ? off + b * W : 0));
-      run.x[b] = *reinterpret_cast<const Pack<uint16_t, W>*>(reinterpret_cast<const char*>(base) + at);
+      if (MODE == ELEMS_LOOSE) {
+        const uint32_t at = 2u * (row + (uint32_t)(run_start<CNT, MODE>(off, limit) + b * W));
+        run.x[b] = __builtin_bit_cast(Pack<uint16_t, W>, *reinterpret_cast<const Loose<uint16_t, W>*>(reinterpret_cast<const char*>(base) + at));
+      } else {
+        const uint32_t at = 2u * (row + (uint32_t)(MODE == ELEMS_FULL || off + b * W < limit ? off + b * W : 0));
+        run.x[b] = *reinterpret_cast<const Pack<uint16_t, W>*>(reinterpret_cast<const char*>(base) + at);
+      }
     }
   }
   __device__ __forceinline__ void take(uint32_t (&out)[REGS], int off, int limit) const {
@@ -660,7 +742,7 @@ struct Bits {
       const int e = CNT == 1 ? 0 : 2 * i;
       const uint32_t lo = run.x[e / W].v[e % W], hi = CNT == 1 ? 0u : (uint32_t)run.x[(e + 1) / W].v[(e + 1) % W];
       out[i] = lo | hi << 16;
-      if (MODE != ELEMS_FULL) out[i] &= bits_if(off + e / W * W < limit);  // (a pair lies in one piece)
+      if (MODE == ELEMS_WIDE) out[i] &= bits_if(off + e / W * W < limit);  // (a pair lies in one piece)
     }
   }
 };
@@ -735,7 +817,7 @@ __device__ __forceinline__ void db_store_out(uint32_t* lds, const f32x4 (&acc)[2
     }
     const int i = 16 * it + c;
     if (a.o_float) {
-      if (i < b.L) store_run<float, 4 * NV, MODE>(out, static_cast<float*>(a.o) + head + (int64_t)(b.low + b.row(i)) * a.ot, dv0 + 4 * NV * g, a.dv);
+      if (i < b.L) da_store_groups<float, NV, MODE>(out, static_cast<float*>(a.o) + head + (int64_t)(b.low + b.row(i)) * a.ot, dv0 + 4 * NV * g, a.dv);
     } else {
 #pragma unroll
       for (int e = 0; e < 2 * NV; ++e) lds[i * LD + 2 * NV * g + e] = db_pack(out[2 * e], out[2 * e + 1]);
@@ -746,12 +828,13 @@ __device__ __forceinline__ void db_store_out(uint32_t* lds, const f32x4 (&acc)[2
   // what lane (c, g) stores of token e: NV elements, two words, one or half of one
   const auto put = [&](uint16_t* at, int e) {
     const int i = (e < 4 ? 0 : 12) + 4 * g + e;
-    if (NV == 4) *reinterpret_cast<Pack<uint32_t, 2>*>(at) = *reinterpret_cast<const Pack<uint32_t, 2>*>(lds + i * LD + 2 * c);
+    if (MODE == ELEMS_LOOSE && NV > 1) *reinterpret_cast<Loose<uint16_t, NV>*>(at) = *reinterpret_cast<const Loose<uint16_t, NV>*>(lds + i * LD + NV / 2 * c);
+    else if (NV == 4) *reinterpret_cast<Pack<uint32_t, 2>*>(at) = *reinterpret_cast<const Pack<uint32_t, 2>*>(lds + i * LD + 2 * c);
     else if (NV == 2) *reinterpret_cast<uint32_t*>(at) = lds[i * LD + c];
     else *at = reinterpret_cast<const uint16_t*>(lds + i * LD)[c];
   };
-  const int col = dv0 + NV * c;
-  const bool in = MODE == ELEMS_FULL || col < a.dv;
+  const int col = run_start<NV, MODE>(dv0 + NV * c, a.dv);
+  const bool in = MODE != ELEMS_WIDE || col < a.dv;
   uint16_t* first = static_cast<uint16_t*>(a.o) + head + (int64_t)b.low * a.ot;
   if (b.L == DB_TOKENS) {  // as with the loads: 32 bits from the lane, the rest from the scalar unit
     const uint32_t off = 2u * ((uint32_t)(b.reverse ? 12 - 4 * g : 4 * g) * (uint32_t)a.ot + (uint32_t)col);
@@ -834,13 +917,19 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
     for (auto& x : run) x.run.forget();
   };
   const auto lds_row = [&](int e) { return lds + ((e < 4 ? 0 : 12) + 4 * g + e) * LD; };
-  const auto put_rows = [&](const Bits<NK, MODE> (&run)[8]) {
+  const auto put_rows = [&](const Bits<NK, MODE> (&run)[8], bool once) {  // once: columns held twice are cleared the second time
+    uint32_t in[NK / 2];
+    if (MODE == ELEMS_LOOSE) {
+      const int off = NK * (da_here(lane) & 15), twice = off - run_start<NK, MODE>(off, a.dk);
+#pragma unroll
+      for (int i = 0; i < NK / 2; ++i) in[i] = twice <= 2 * i ? 0xFFFFFFFFu : twice == 2 * i + 1 ? 0xFFFF0000u : 0u;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       uint32_t x[NK / 2];
       run[e].take(x, NK * c, a.dk);
 #pragma unroll
-      for (int i = 0; i < NK / 2; ++i) lds_row(e)[NK / 2 * c + i] = x[i];
+      for (int i = 0; i < NK / 2; ++i) lds_row(e)[NK / 2 * c + i] = MODE == ELEMS_LOOSE && once ? x[i] & in[i] : x[i];
     }
     wave_lds_fence();
   };
@@ -902,9 +991,9 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
     if (!STATES) {
       f32x4 acc[2][NV];
       uint32_t Q[2][2 * NK], K1[2][2 * NK];
-      put_rows(q_run);
+      put_rows(q_run, true);
       get_tokens(Q);
-      put_rows(k_run);
+      put_rows(k_run, false);
       get_tokens(K1);
       f32x4 pt[3] = {zero, zero, zero};  // P^T: tokens 0-15 for 0-15, 0-15 for 16-31, 16-31 for 16-31
 #pragma unroll
@@ -1398,7 +1487,7 @@ static int decay_attention_bf16_tiles(const DaRoles& c, const DaPlan& p, float* 
 }
 
 // The kernel and the accesses that suit all of the roles, whose head sizes ask for the same tiles.  bf16 tensors have a kernel of
-// their own where 16-byte accesses are possible and a block of tokens spans less than 2^32 bytes.
+// their own, for heads of two columns at least (two to a register) and where a block of tokens spans less than 2^32 bytes.
 static int decay_attention_core(const DaRoles& r, int dtype, float* ws, hipStream_t s) {
   const int64_t most = (int64_t)1 << 32, most_bf16 = (most - 1024) / (2 * DB_TOKENS);
   const int bytes = elem_bytes(dtype);
@@ -1408,20 +1497,21 @@ static int decay_attention_core(const DaRoles& r, int dtype, float* ws, hipStrea
     OIGE_REQUIRE(c.q.st >= 0 && c.q.st < most && c.k.st >= 0 && c.k.st < most && c.v.st >= 0 && c.v.st < most,
                  "decay_attention: token strides must be below 2^32 elements and not negative");
     wide = wide && da_wide(c, bytes);
-    bf16 = bf16 && c.q.st <= most_bf16 && c.k.st <= most_bf16 && c.v.st <= most_bf16 && c.ot <= most_bf16;
+    bf16 = bf16 && c.dk > 1 && c.q.st <= most_bf16 && c.k.st <= most_bf16 && c.v.st <= most_bf16 && c.ot <= most_bf16;
   }
-  bf16 = bf16 && wide;
   const DaCore& c = r.c[0];
   const DaPlan p = decay_attention_plan(c.n, c.t, c.h, c.dk, c.dv, bf16, r.roles);
   bool full = wide;
   for (int i = 0; i < r.roles; ++i) full = full && r.c[i].dk == 16 * p.nk && r.c[i].dv == 16 * p.nv * p.slices;
-  if (bf16) return full ? decay_attention_bf16_tiles<ELEMS_FULL>(r, p, ws, s) : decay_attention_bf16_tiles<ELEMS_WIDE>(r, p, ws, s);
-  if (dtype == OIGE_BF16) return decay_attention_tiles<__bf16, ELEMS_SINGLE>(r, p, ws, s);
+  if (bf16)
+    return full ? decay_attention_bf16_tiles<ELEMS_FULL>(r, p, ws, s)
+                : wide ? decay_attention_bf16_tiles<ELEMS_WIDE>(r, p, ws, s) : decay_attention_bf16_tiles<ELEMS_LOOSE>(r, p, ws, s);
+  if (dtype == OIGE_BF16) return decay_attention_tiles<__bf16, ELEMS_LOOSE>(r, p, ws, s);
   if (dtype == OIGE_F16)
     return full ? decay_attention_tiles<_Float16, ELEMS_FULL>(r, p, ws, s)
-                : wide ? decay_attention_tiles<_Float16, ELEMS_WIDE>(r, p, ws, s) : decay_attention_tiles<_Float16, ELEMS_SINGLE>(r, p, ws, s);
+                : wide ? decay_attention_tiles<_Float16, ELEMS_WIDE>(r, p, ws, s) : decay_attention_tiles<_Float16, ELEMS_LOOSE>(r, p, ws, s);
   return full ? decay_attention_tiles<float, ELEMS_FULL>(r, p, ws, s)
-              : wide ? decay_attention_tiles<float, ELEMS_WIDE>(r, p, ws, s) : decay_attention_tiles<float, ELEMS_SINGLE>(r, p, ws, s);
+              : wide ? decay_attention_tiles<float, ELEMS_WIDE>(r, p, ws, s) : decay_attention_tiles<float, ELEMS_LOOSE>(r, p, ws, s);
 }
 
 static int decay_attention_share(const float* in_k, const float* in_v, const oige_decay_attention_io& io, hipStream_t s) {
