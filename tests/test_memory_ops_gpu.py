@@ -238,6 +238,33 @@ def test_decay_attention_shared_heads(n, t, h, hk, dk, dv, dtype):
     _check_attention(kw, d_o, d_state)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, t, h, hk, dk, dv", [
+    (1024, 34, 1, 1, 33, 61), (512, 19, 2, 1, 17, 47), (1, 6300, 2, 2, 101, 67), (3, 40, 2, 1, 2, 1), (3, 40, 2, 2, 1, 2), (2, 300, 1, 1, 65, 33),
+    (2, 33, 1, 1, 127, 17)])
+def test_decay_attention_odd_heads(n, t, h, hk, dk, dv, dtype):
+    """Rows on no boundary, heads whose last columns are held twice; what lies around the results is left alone."""
+    kw, d_o, d_state = _attention_inputs(n, t, h, hk, dk, dv, dtype, 23, resets=0.04, ragged=n > 1)
+    _check_attention(kw, d_o, d_state)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dk, dv", [(19, 35), (100, 101)])
+def test_decay_attention_odd_heads_with_values_that_are_not_finite(dk, dv, dtype):
+    kw, _, _ = _attention_inputs(2, 70, 2, 2, dk, dv, dtype, 24)
+    kw["resets"] = torch.zeros(2, 70, dtype=torch.bool, device=DEV)
+    kw["resets"][0, 50] = True
+    for name, column in (("q", 0), ("q", dk - 1), ("k", dk - 1), ("v", dv - 1), ("v", dv - 2)):
+        bad = dict(kw)
+        bad[name] = kw[name].clone()
+        bad[name][0, 40, 0, column] = inf
+        o, state = decay_attention(**bad)
+        hit = torch.zeros_like(o, dtype=torch.bool)
+        seen = slice(40, 41) if name == "q" else slice(40, 50)
+        hit[0, seen, 0, column if name == "v" else slice(None)] = True
+        assert o[~hit].isfinite().all() and state.isfinite().all() and not o[0, 40, 0, column if name == "v" else 0].isfinite().all()
+
+
 @pytest.mark.parametrize("decay", [0.0, 1.0, 1.01, 1e-30, 0.5])
 def test_decay_attention_extreme_decays(decay):
     kw, d_o, d_state = _attention_inputs(2, 150, 1, 1, 16, 16, torch.float32, 14, resets=0.02, decay=[decay])
