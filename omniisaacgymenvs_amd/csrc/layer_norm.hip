@@ -273,14 +273,16 @@ __global__ __launch_bounds__(LN_FOLD * LN_FOLD) void layer_norm_fold_kernel(cons
 }
 
 // How a row is laid over lanes: `vec` elements per access (16 bytes where width, strides and pointers allow), K accesses per lane,
-// `lanes` of a wave -- or of a workgroup of 256 to 1024, where 64 lanes would need more than 4 accesses each (8 single-element ones).
+// `lanes` of a wave -- or of a workgroup of 256 to 1024, where 64 lanes would hold more than 16 elements each (8 single ones; 16384 x
+// 2048 bf16: 44 us forward with 32 in a wave's lanes, 33 in a workgroup's).  A workgroup's lanes hold at most 16 of them, in the backward
+// pass, which keeps five such rows, 8 (8192 x 8192 fp32: 347 us with 16, 173 with 8), as long as 1024 lanes are enough.
 struct LnShape {
   int lanes, k;
   bool block;
 };
-static LnShape layer_norm_shape(int width, int vec) {
+static LnShape layer_norm_shape(int width, int vec, bool backward) {
   const int slots = (width + vec - 1) / vec;
-  const int kmax = vec > 1 ? 4 : 8;
+  const int kmax = vec == 8 ? 2 : vec == 4 ? 4 : 8;
   LnShape s{1, 1, false};
   if (slots <= WAVE * kmax) {
     while (s.lanes < slots && s.lanes < WAVE) s.lanes *= 2;
@@ -289,7 +291,8 @@ static LnShape layer_norm_shape(int width, int vec) {
   }
   s.block = true;
   s.lanes = LN_THREADS;
-  while (s.lanes < LN_MAX_THREADS && s.lanes * (vec == 8 ? 2 : 4) < slots) s.lanes *= 2;  // at most 16 elements a lane while it can
+  const int each = vec == 1 ? 4 : (backward ? 8 : 16) / vec;
+  while (s.lanes < LN_MAX_THREADS && s.lanes * each < slots) s.lanes *= 2;
   while (s.lanes * s.k < slots) s.k *= 2;
   return s;
 }
@@ -322,7 +325,7 @@ static int layer_norm_pick(const oige_layer_norm_io& io, const LnShape& s, int64
   }
   LN_CASE(1, false, true)
   LN_CASE(2, false, true)
-  LN_CASE(4, false, true)
+  LN_CASE(4, false, VEC < 8)
   LN_CASE(8, false, VEC == 1)
   LN_CASE(1, true, true)
   LN_CASE(2, true, true)
@@ -374,7 +377,7 @@ int oige_layer_norm_forward(const oige_layer_norm_io* io, oige_stream_t stream) 
   OIGE_REQUIRE(io->y, "layer_norm_forward: null y");
   OIGE_REQUIRE((io->mean == nullptr) == (io->rstd == nullptr), "layer_norm_forward: mean and rstd are kept together or not at all");
   const bool wide = layer_norm_wide(*io, false);
-  const LnShape s = layer_norm_shape(io->width, wide ? 16 / elem_bytes(io->dtype) : 1);
+  const LnShape s = layer_norm_shape(io->width, wide ? 16 / elem_bytes(io->dtype) : 1, false);
   return layer_norm_dispatch<false>(*io, wide, s, layer_norm_blocks(io->rows, s, wide ? LN_MAX_BLOCKS : LN_MAX_BLOCKS_SINGLE), (hipStream_t)stream);
 }
 
@@ -398,7 +401,7 @@ int oige_layer_norm_backward(const oige_layer_norm_io* io, oige_stream_t stream)
   int64_t blocks = 0;
   if (a.rows > 0) {
     const bool wide = layer_norm_wide(a, true);
-    const LnShape s = layer_norm_shape(a.width, wide ? 16 / elem_bytes(a.dtype) : 1);
+    const LnShape s = layer_norm_shape(a.width, wide ? 16 / elem_bytes(a.dtype) : 1, true);
     blocks = layer_norm_blocks(a.rows, s, LN_MAX_PARTS);
     const int rc2 = layer_norm_dispatch<true>(a, wide, s, blocks, (hipStream_t)stream);
     if (rc2) return rc2;
