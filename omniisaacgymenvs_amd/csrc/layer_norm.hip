@@ -19,7 +19,7 @@ namespace oige {
 constexpr int LN_THREADS = 256;
 constexpr int LN_MAX_THREADS = 1024;
 constexpr int LN_MAX_WIDTH = 16384;
-constexpr int LN_LDS_COLS = 2048;  // most columns of a wave row: 64 lanes x 4 pieces x 8 elements
+constexpr int LN_LDS_COLS = 1024;  // most columns of a row in one wave: 64 lanes x 16 elements
 
 // x + x of another lane, the lane found by the data path itself (no LDS round trip).
 template <int CTRL>
@@ -74,9 +74,16 @@ __device__ __forceinline__ float2 row_sum2(float2 v, int lanes, float* lds) {
   return v;
 }
 
+// Whether element e of the run from `off` counts: rows are read by accesses of VEC elements on any boundary, a run across the end starts
+// earlier and holds some elements a second time.  Those are computed and stored twice, to the same bits, and left out of the sums.
+template <int VEC, int MODE>
+__device__ __forceinline__ bool ln_once(int off, int e, int width) {
+  return MODE == ELEMS_LOOSE ? run_start<VEC, MODE>(off, width) + e >= off : off + e < width;
+}
+
 template <typename T, int VEC, int K, bool BLOCK>
 __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_norm_forward_kernel(const oige_layer_norm_io a, int lanes) {
-  constexpr int MODE = VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE;
+  constexpr int MODE = VEC == 1 ? ELEMS_SINGLE : ELEMS_LOOSE;
   __shared__ float lds[2 * LN_MAX_THREADS / WAVE];
   const int l = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
   const int rows_per_block = BLOCK ? 1 : LN_THREADS / lanes;
@@ -88,10 +95,11 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int col = (k * lanes + l) * VEC + e;
+      const int col = run_start<VEC, MODE>((k * lanes + l) * VEC, width) + e;
       w[k][e] = a.weight && col < width ? load_elem(a.weight, col, a.weight_dtype) : 1.f;
       b[k][e] = a.bias && col < width ? load_elem(a.bias, col, a.weight_dtype) : 0.f;
     }
+  const auto once = [&](int k, int e) { return ln_once<VEC, MODE>((k * lanes + l) * VEC, e, width); };
   // the next row is on its way while this one is summed
   const int64_t first = (int64_t)blockIdx.x * rows_per_block + sub, step = (int64_t)gridDim.x * rows_per_block;
   Run<T, VEC, MODE> run[K];
@@ -110,15 +118,15 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s += x[k][e];
+      for (int e = 0; e < VEC; ++e) s += once(k, e) ? x[k][e] : 0.f;
     const float mean = row_sum<BLOCK>(s, lanes, lds) * inv;
     float q = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        x[k][e] = (k * lanes + l) * VEC + e < width ? x[k][e] - mean : 0.f;
-        q = fmaf(x[k][e], x[k][e], q);
+        x[k][e] -= mean;
+        q = once(k, e) ? fmaf(x[k][e], x[k][e], q) : q;
       }
     const float rstd = 1.f / sqrtf(row_sum<BLOCK>(q, lanes, lds) * inv + a.eps);
     T* yr = static_cast<T*>(a.y) + row * (int64_t)width;
@@ -138,7 +146,7 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
 
 template <typename T, int VEC, int K, bool BLOCK>
 __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_norm_backward_kernel(const oige_layer_norm_io a, int lanes) {
-  constexpr int MODE = VEC == 1 ? ELEMS_SINGLE : ELEMS_WIDE;
+  constexpr int MODE = VEC == 1 ? ELEMS_SINGLE : ELEMS_LOOSE;
   __shared__ float lds[2 * LN_MAX_THREADS / WAVE];
   __shared__ float cols[BLOCK ? 1 : LN_THREADS / WAVE * LN_LDS_COLS];
   const int l = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
@@ -151,10 +159,11 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int col = (k * lanes + l) * VEC + e;
+      const int col = run_start<VEC, MODE>((k * lanes + l) * VEC, width) + e;
       w[k][e] = a.weight && col < width ? load_elem(a.weight, col, a.weight_dtype) : 1.f;
       dw[k][e] = db[k][e] = 0.f;
     }
+  const auto once = [&](int k, int e) { return ln_once<VEC, MODE>((k * lanes + l) * VEC, e, width); };
   const int64_t first = (int64_t)blockIdx.x * rows_per_block + sub, step = (int64_t)gridDim.x * rows_per_block;
   Run<T, VEC, MODE> x_run[K], g_run[K];
   float next_mean = 0.f, next_rstd = 0.f;
@@ -182,12 +191,12 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        x[k][e] = (k * lanes + l) * VEC + e < width ? (x[k][e] - mean) * rstd : 0.f;
+        x[k][e] = (x[k][e] - mean) * rstd;
         dw[k][e] = fmaf(g[k][e], x[k][e], dw[k][e]);
         db[k][e] += g[k][e];
         g[k][e] *= w[k][e];
-        s.x += g[k][e];
-        s.y = fmaf(g[k][e], x[k][e], s.y);
+        s.x = once(k, e) ? s.x + g[k][e] : s.x;
+        s.y = once(k, e) ? fmaf(g[k][e], x[k][e], s.y) : s.y;
       }
     s = row_sum2<BLOCK>(s, lanes, lds);
     const float mg = s.x * inv, mgx = s.y * inv;
@@ -209,7 +218,7 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const int col = (k * lanes + l) * VEC + e;
+        const int col = run_start<VEC, MODE>((k * lanes + l) * VEC, width) + e;
         if (col < width) {
           part[col] = dw[k][e];
           part[width + col] = db[k][e];
@@ -227,7 +236,7 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
       for (int e = 0; e < VEC; ++e) {
         float v = which ? db[k][e] : dw[k][e];
         for (int off = lanes; off < WAVE; off <<= 1) v += __shfl_xor(v, off, WAVE);  // the rows that shared this wave
-        const int col = (k * lanes + l) * VEC + e;
+        const int col = run_start<VEC, MODE>((k * lanes + l) * VEC, width) + e;
         if (col < width && lane_id() < lanes) cols[wv * LN_LDS_COLS + col] = v;
       }
     __syncthreads();
@@ -272,9 +281,8 @@ __global__ __launch_bounds__(LN_FOLD * LN_FOLD) void layer_norm_fold_kernel(cons
   }
 }
 
-// How a row is laid over lanes: `vec` elements per access (16 bytes where width, strides and pointers allow), K accesses per lane,
-// `lanes` of a wave -- or of a workgroup of 256 to 1024, where 64 lanes would hold more than 16 elements each (8 single ones; 16384 x
-// 2048 bf16: 44 us forward with 32 in a wave's lanes, 33 in a workgroup's).  A workgroup's lanes hold at most 16 of them, in the backward
+// How a row is laid over lanes: `vec` elements per access (16 bytes, on any boundary), K accesses per lane,
+// `lanes` of a wave -- or of a workgroup of 256 to 1024, where 64 lanes would hold more than 16 elements each (16384 x 2048 bf16: 44 us forward with 32 in a wave's lanes, 33 in a workgroup's).  A workgroup's lanes hold at most 16 of them, in the backward
 // pass, which keeps five such rows, 8 (8192 x 8192 fp32: 347 us with 16, 173 with 8), as long as 1024 lanes are enough.
 struct LnShape {
   int lanes, k;
@@ -282,7 +290,7 @@ struct LnShape {
 };
 static LnShape layer_norm_shape(int width, int vec, bool backward) {
   const int slots = (width + vec - 1) / vec;
-  const int kmax = vec == 8 ? 2 : vec == 4 ? 4 : 8;
+  const int kmax = vec == 8 ? 2 : 4;
   LnShape s{1, 1, false};
   if (slots <= WAVE * kmax) {
     while (s.lanes < slots && s.lanes < WAVE) s.lanes *= 2;
@@ -291,17 +299,16 @@ static LnShape layer_norm_shape(int width, int vec, bool backward) {
   }
   s.block = true;
   s.lanes = LN_THREADS;
-  const int each = vec == 1 ? 4 : (backward ? 8 : 16) / vec;
+  const int each = (backward ? 8 : 16) / vec;
   while (s.lanes < LN_MAX_THREADS && s.lanes * each < slots) s.lanes *= 2;
   while (s.lanes * s.k < slots) s.k *= 2;
   return s;
 }
 
 // Workgroups walk rows, so that weights stay in registers and the next row is on its way behind this one's sums.  Forward: 4 per CU
-// with 16-byte accesses (262144 x 1024 bf16: 225 us, 238 with 8 per CU, 635 with a workgroup for every 4 rows), 8 with single
-// elements, which have a quarter of the bytes in flight (65536 x 211 fp32: 21.2 us, 22.8 with 4).  Backward: 4 per CU, one partial
-// row of the parameters' gradients each (65536 x 512 bf16: 37 us, 40 with 2, 43 with 8).
-constexpr int64_t LN_MAX_BLOCKS = 1024, LN_MAX_BLOCKS_SINGLE = 2048, LN_MAX_PARTS = 1024;
+// (262144 x 1024 bf16: 225 us, 238 with 8 per CU, 635 with a workgroup for every 4 rows).  Backward: 4 per CU, one partial row of
+// the parameters' gradients each (65536 x 512 bf16: 37 us, 40 with 2, 43 with 8).
+constexpr int64_t LN_MAX_BLOCKS = 1024, LN_MAX_PARTS = 1024;
 
 static int64_t layer_norm_blocks(int64_t rows, const LnShape& s, int64_t most) {
   const int64_t per = s.block ? 1 : LN_THREADS / s.lanes;
@@ -324,14 +331,11 @@ static int layer_norm_pick(const oige_layer_norm_io& io, const LnShape& s, int64
     if (s.k == K && s.block == BLOCK) return layer_norm_launch<T, VEC, K, BLOCK, BACKWARD>(io, s, blocks, stream); \
   }
   LN_CASE(1, false, true)
-  LN_CASE(2, false, true)
-  LN_CASE(4, false, VEC < 8)
-  LN_CASE(8, false, VEC == 1)
-  LN_CASE(1, true, true)
-  LN_CASE(2, true, true)
-  LN_CASE(4, true, VEC < 8)
-  LN_CASE(8, true, VEC == 1)
-  LN_CASE(16, true, VEC == 1)
+  LN_CASE(2, false, VEC > 1)
+  LN_CASE(4, false, VEC == 4)
+  LN_CASE(1, true, VEC > 1)
+  LN_CASE(2, true, VEC > 1)
+  LN_CASE(4, true, VEC == 4)
 #undef LN_CASE
   return fail(OIGE_EINVAL, "layer_norm: no variant for %d lanes x %d accesses", s.lanes, s.k);
 }
@@ -347,16 +351,15 @@ static int layer_norm_check(const oige_layer_norm_io* io, const char* what) {
   return OIGE_OK;
 }
 
-// 16-byte accesses: rows of whole vectors that start on a boundary, in every tensor walked row by row.
-static bool layer_norm_wide(const oige_layer_norm_io& io, bool backward) {
+// Elements of an access: 16 bytes, single ones in rows that are shorter.
+static int layer_norm_vec(const oige_layer_norm_io& io) {
   const int v = 16 / elem_bytes(io.dtype);
-  bool ok = io.width % v == 0 && io.x_row_stride % v == 0 && aligned16(io.x);
-  if (!backward) return ok && aligned16(io.y);
-  return ok && io.dy_row_stride % v == 0 && aligned16(io.dy) && aligned16(io.dx);
+  return io.width >= v ? v : 1;
 }
 
 template <bool BACKWARD>
-static int layer_norm_dispatch(const oige_layer_norm_io& io, bool wide, const LnShape& s, int64_t blocks, hipStream_t stream) {
+static int layer_norm_dispatch(const oige_layer_norm_io& io, const LnShape& s, int64_t blocks, hipStream_t stream) {
+  const bool wide = layer_norm_vec(io) > 1;
   if (io.dtype == OIGE_F32)
     return wide ? layer_norm_pick<float, 4, BACKWARD>(io, s, blocks, stream) : layer_norm_pick<float, 1, BACKWARD>(io, s, blocks, stream);
   if (io.dtype == OIGE_F16)
@@ -376,9 +379,8 @@ int oige_layer_norm_forward(const oige_layer_norm_io* io, oige_stream_t stream) 
   if (io->rows == 0) return OIGE_OK;
   OIGE_REQUIRE(io->y, "layer_norm_forward: null y");
   OIGE_REQUIRE((io->mean == nullptr) == (io->rstd == nullptr), "layer_norm_forward: mean and rstd are kept together or not at all");
-  const bool wide = layer_norm_wide(*io, false);
-  const LnShape s = layer_norm_shape(io->width, wide ? 16 / elem_bytes(io->dtype) : 1, false);
-  return layer_norm_dispatch<false>(*io, wide, s, layer_norm_blocks(io->rows, s, wide ? LN_MAX_BLOCKS : LN_MAX_BLOCKS_SINGLE), (hipStream_t)stream);
+  const LnShape s = layer_norm_shape(io->width, layer_norm_vec(*io), false);
+  return layer_norm_dispatch<false>(*io, s, layer_norm_blocks(io->rows, s, LN_MAX_BLOCKS), (hipStream_t)stream);
 }
 
 int64_t oige_layer_norm_workspace_floats(int64_t rows, int32_t width) {
@@ -400,10 +402,9 @@ int oige_layer_norm_backward(const oige_layer_norm_io* io, oige_stream_t stream)
   if (!params) a.workspace = nullptr;
   int64_t blocks = 0;
   if (a.rows > 0) {
-    const bool wide = layer_norm_wide(a, true);
-    const LnShape s = layer_norm_shape(a.width, wide ? 16 / elem_bytes(a.dtype) : 1, true);
+    const LnShape s = layer_norm_shape(a.width, layer_norm_vec(a), true);
     blocks = layer_norm_blocks(a.rows, s, LN_MAX_PARTS);
-    const int rc2 = layer_norm_dispatch<true>(a, wide, s, blocks, (hipStream_t)stream);
+    const int rc2 = layer_norm_dispatch<true>(a, s, blocks, (hipStream_t)stream);
     if (rc2) return rc2;
   }
   if (!params) return OIGE_OK;

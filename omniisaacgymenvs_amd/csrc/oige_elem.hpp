@@ -121,7 +121,7 @@ __device__ __forceinline__ void store_run(const float (&in)[CNT], T* row, int of
   constexpr int W = MODE == ELEMS_SINGLE ? 1 : (CNT < VEC16<T> ? CNT : VEC16<T>);
 #pragma unroll
   for (int b = 0; b < CNT; b += W) {
-    if (MODE == ELEMS_LOOSE || MODE == ELEMS_FULL || off + b < limit) {
+    if (MODE == ELEMS_FULL || (MODE == ELEMS_LOOSE ? off : off + b) < limit) {
       Pack<T, W> x;
 #pragma unroll
       for (int e = 0; e < W; ++e) x.v[e] = (T)in[b + e];
