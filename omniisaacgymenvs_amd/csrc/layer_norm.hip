@@ -10,8 +10,9 @@
 // all rows a workgroup walks, written as one partial row per workgroup and added up by a second launch in a fixed order
 // (no atomics: the result does not depend on scheduling).
 //
-// Forward 262144 x 1024 bf16: 222 us, 4.8 TB/s (the copy rate is 5.4; without the next row in flight 268 us); 65536 x 211 fp32: 21 us;
-// one row: 5 us, a launch's latency.  Forward + backward 65536 x 512 bf16: 32 + 37 us, and 4 for the partial rows' sum.
+// Forward 262144 x 1024 bf16: 219 us, 4.9 TB/s (the copy rate is 5.4; without the next row in flight 268 us); 65536 x 211 fp32: 21 us;
+// one row: 2 us, a launch's latency (4 with the parameters read element by element).  Forward + backward 65536 x 512 bf16: 29 + 35 us,
+// and 4 for the partial rows' sum.
 #include "oige_elem.hpp"
 
 namespace oige {
@@ -81,6 +82,19 @@ __device__ __forceinline__ bool ln_once(int off, int e, int width) {
   return MODE == ELEMS_LOOSE ? run_start<VEC, MODE>(off, width) + e >= off : off + e < width;
 }
 
+// A run of the weight or the bias: of the rows' type or fp32, `none` everywhere where there is none.
+template <typename T, int VEC, int MODE>
+__device__ __forceinline__ void ln_param(float (&w)[VEC], const void* p, int dtype, int off, int width, float none) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) w[e] = none;
+  } else if (dtype == OIGE_F32) {
+    load_run<float, VEC, MODE>(w, static_cast<const float*>(p), off, width);
+  } else {
+    load_run<T, VEC, MODE>(w, static_cast<const T*>(p), off, width);
+  }
+}
+
 template <typename T, int VEC, int K, bool BLOCK>
 __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_norm_forward_kernel(const oige_layer_norm_io a, int lanes) {
   constexpr int MODE = VEC == 1 ? ELEMS_SINGLE : ELEMS_LOOSE;
@@ -92,13 +106,10 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
   const float inv = 1.f / (float)width;
   float w[K][VEC], b[K][VEC];
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int col = run_start<VEC, MODE>((k * lanes + l) * VEC, width) + e;
-      w[k][e] = a.weight && col < width ? load_elem(a.weight, col, a.weight_dtype) : 1.f;
-      b[k][e] = a.bias && col < width ? load_elem(a.bias, col, a.weight_dtype) : 0.f;
-    }
+  for (int k = 0; k < K; ++k) {
+    ln_param<T, VEC, MODE>(w[k], a.weight, a.weight_dtype, (k * lanes + l) * VEC, width, 1.f);
+    ln_param<T, VEC, MODE>(b[k], a.bias, a.weight_dtype, (k * lanes + l) * VEC, width, 0.f);
+  }
   const auto once = [&](int k, int e) { return ln_once<VEC, MODE>((k * lanes + l) * VEC, e, width); };
   // the next row is on its way while this one is summed
   const int64_t first = (int64_t)blockIdx.x * rows_per_block + sub, step = (int64_t)gridDim.x * rows_per_block;
@@ -156,13 +167,11 @@ __global__ __launch_bounds__(BLOCK ? LN_MAX_THREADS : LN_THREADS) void layer_nor
   const float inv = 1.f / (float)width;
   float w[K][VEC], dw[K][VEC], db[K][VEC];
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int k = 0; k < K; ++k) {
+    ln_param<T, VEC, MODE>(w[k], a.weight, a.weight_dtype, (k * lanes + l) * VEC, width, 1.f);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int col = run_start<VEC, MODE>((k * lanes + l) * VEC, width) + e;
-      w[k][e] = a.weight && col < width ? load_elem(a.weight, col, a.weight_dtype) : 1.f;
-      dw[k][e] = db[k][e] = 0.f;
-    }
+    for (int e = 0; e < VEC; ++e) dw[k][e] = db[k][e] = 0.f;
+  }
   const auto once = [&](int k, int e) { return ln_once<VEC, MODE>((k * lanes + l) * VEC, e, width); };
   const int64_t first = (int64_t)blockIdx.x * rows_per_block + sub, step = (int64_t)gridDim.x * rows_per_block;
   Run<T, VEC, MODE> x_run[K], g_run[K];
@@ -306,8 +315,8 @@ static LnShape layer_norm_shape(int width, int vec, bool backward) {
 }
 
 // Workgroups walk rows, so that weights stay in registers and the next row is on its way behind this one's sums.  Forward: 4 per CU
-// (262144 x 1024 bf16: 225 us, 238 with 8 per CU, 635 with a workgroup for every 4 rows).  Backward: 4 per CU, one partial row of
-// the parameters' gradients each (65536 x 512 bf16: 37 us, 40 with 2, 43 with 8).
+// (262144 x 1024 bf16: 219 us; when it took 225, 238 with 8 per CU and 635 with a workgroup for every 4 rows).  Backward: 4 per CU, one partial row of
+// the parameters' gradients each (65536 x 512 bf16: 35 us; when it took 37, 40 with 2 and 43 with 8).
 constexpr int64_t LN_MAX_BLOCKS = 1024, LN_MAX_PARTS = 1024;
 
 static int64_t layer_norm_blocks(int64_t rows, const LnShape& s, int64_t most) {

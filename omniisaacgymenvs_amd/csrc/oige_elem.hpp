@@ -20,12 +20,7 @@ constexpr int VEC16 = 16 / (int)sizeof(T);  // elements of a 16-byte access
 
 inline int elem_bytes(int dtype) { return dtype == OIGE_F32 ? 4 : (dtype == OIGE_F16 || dtype == OIGE_BF16 ? 2 : 0); }
 
-// One element of a buffer whose type is a launch constant (parameters of another type than the activations).
-__device__ __forceinline__ float load_elem(const void* p, int64_t i, int dtype) {
-  if (dtype == OIGE_F32) return static_cast<const float*>(p)[i];
-  if (dtype == OIGE_F16) return (float)static_cast<const _Float16*>(p)[i];
-  return (float)static_cast<const __bf16*>(p)[i];
-}
+// One element into a buffer whose type is a launch constant (parameters of another type than the activations).
 __device__ __forceinline__ void store_elem(void* p, int64_t i, float x, int dtype) {
   if (dtype == OIGE_F32) static_cast<float*>(p)[i] = x;
   else if (dtype == OIGE_F16) static_cast<_Float16*>(p)[i] = (_Float16)x;
