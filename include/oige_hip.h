@@ -1298,7 +1298,8 @@ int oige_layer_norm_backward(const oige_layer_norm_io* io, oige_stream_t stream)
  * Tensors are (N, T, heads, d) with element strides for the first three axes (the last one is contiguous); heads a multiple of
  * kv_heads; head sizes 1 .. 128; T below 2^30.  Tokens from lengths[n] on (clamped to 0 .. T) are not part of sequence n: they are not read
  * into anything, their rows of o and of the gradients are zero.  An infinite or NaN value reaches only the rows whose
- * tokens see it.  States are fp32, contiguous (N, heads, key_dim, value_dim).                                             */
+ * tokens see it.  States are fp32, contiguous (N, heads, key_dim, value_dim).  What a call writes must not overlap what it
+ * reads: a state is not handed on in place (oige_decay_attention_step does that).                                          */
 typedef struct oige_decay_attention_io {
   const void *q, *k, *v; /* (N, T, heads, key_dim), (N, T, kv_heads, key_dim), (N, T, kv_heads, value_dim) */
   void* o;               /* (N, T, heads, value_dim) */

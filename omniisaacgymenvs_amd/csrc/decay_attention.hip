@@ -1619,6 +1619,7 @@ int oige_decay_attention_forward(const oige_decay_attention_io* io, oige_stream_
   if (io->num_envs == 0) return OIGE_OK;
   OIGE_REQUIRE(io->num_tokens == 0 || (io->q && io->k && io->v && io->o), "decay_attention_forward: null q, k, v or o");
   OIGE_REQUIRE(io->num_tokens > 0 || io->state_out, "decay_attention_forward: no tokens and no final state asked for");
+  OIGE_REQUIRE(!io->state_out || io->state_out != io->state_in, "decay_attention_forward: state_out must not be state_in (other waves still read it)");
   const int64_t need = da_workspace(*io, false);
   OIGE_REQUIRE(need == 0 || (io->workspace && aligned16(io->workspace) && io->workspace_floats >= need),
                "decay_attention_forward: needs a 16-byte aligned workspace of %lld floats", (long long)need);
@@ -1646,6 +1647,8 @@ int oige_decay_attention_backward(const oige_decay_attention_io* io, oige_stream
   OIGE_REQUIRE(io->num_tokens == 0 || (io->q && io->k && io->v && io->d_o && io->dq && io->dk && io->dv),
                "decay_attention_backward: null q, k, v, d_o, dq, dk or dv");
   OIGE_REQUIRE(io->num_tokens > 0 || io->d_state_in, "decay_attention_backward: no tokens and no initial state's gradient asked for");
+  OIGE_REQUIRE(!io->d_state_in || (io->d_state_in != io->d_state_out && io->d_state_in != io->state_in),
+               "decay_attention_backward: d_state_in must be neither d_state_out nor state_in (other waves still read them)");
   const int64_t need = da_workspace(*io, true);
   OIGE_REQUIRE(need == 0 || (io->workspace && aligned16(io->workspace) && io->workspace_floats >= need),
                "decay_attention_backward: needs a 16-byte aligned workspace of %lld floats", (long long)need);

@@ -157,6 +157,20 @@ def test_abi_decay_attention_refuses():
     _fail(calls[1](C.byref(io), None), "no tokens")
 
 
+def test_abi_decay_attention_refuses_states_in_place():
+    lib = _lib.load()
+    io = _lib.DecayAttentionIo()
+    io.dtype, io.num_envs, io.num_tokens, io.heads, io.kv_heads, io.key_dim, io.value_dim = _lib.F32, 2, 4, 1, 1, 8, 8
+    for name in ("q", "k", "v", "o", "decay", "d_o", "dq", "dk", "dv"):
+        setattr(io, name, 16)
+    io.state_in = io.state_out = 32
+    _fail(lib.oige_decay_attention_forward(C.byref(io), None), "state_out must not be state_in")
+    io.d_state_in = 32
+    _fail(lib.oige_decay_attention_backward(C.byref(io), None), "d_state_in must be neither")
+    io.state_in, io.d_state_out = 48, 32
+    _fail(lib.oige_decay_attention_backward(C.byref(io), None), "d_state_in must be neither")
+
+
 def test_abi_decay_attention_step_refuses():
     lib = _lib.load()
     io = _lib.DecayAttentionStepIo()
