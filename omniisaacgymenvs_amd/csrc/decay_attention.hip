@@ -53,7 +53,8 @@ struct DaCore {
   const float* s_in;   // NULL: zero
   float* s_out;        // NULL: not wanted
   float* seg_states;   // states between time segments, in register order
-  float* seg_factors;  // (N, H, nseg): what a segment multiplies the state with, -1: it drops it
+  float* seg_factors;  // (N, H, nseg): what a segment multiplies the state with, -1: it drops it.  (Those that are read are powers of 32 m
+                       // tokens, segments between the first and the last: never negative, whatever the decay's sign.)
   const float* decay;
   const void* resets;
   const void* lengths;
@@ -97,27 +98,19 @@ __device__ __forceinline__ double da_power(double decay, int64_t n) {
   }
   return r;
 }
-struct DaPowers {  // decay^n for n in 0 .. 32 without a loop, within 5 roundings
-  double d16, d32;
-  float p1, p2, p4, p8, p16, p32;
-  __device__ __forceinline__ explicit DaPowers(double d) : p1((float)d), p2((float)(d * d)) {
-    const double d4 = (d * d) * (d * d);
-    p4 = (float)d4;
-    p8 = (float)(d4 * d4);
-    d16 = (d4 * d4) * (d4 * d4);
-    d32 = d16 * d16;
-    p16 = (float)d16;
-    p32 = (float)d32;
-  }
-  __device__ __forceinline__ float operator()(int n) const {
-    float r = (n & 1) ? p1 : 1.f;
-    r *= (n & 2) ? p2 : 1.f;
-    r *= (n & 4) ? p4 : 1.f;
-    r *= (n & 8) ? p8 : 1.f;
-    r *= (n & 16) ? p16 : 1.f;
-    return (n & 32) ? p32 : r;
-  }
-};
+// decay^n for n in 0 .. 32, a wave's table in LDS: products in 64 bits, rounded once.
+constexpr int DA_POWERS = 33;
+__device__ __forceinline__ void da_powers(float* table, double decay, int lane) {
+  const double d2 = decay * decay, d4 = d2 * d2, d8 = d4 * d4, d16 = d8 * d8;
+  double r = (lane & 1) ? decay : 1.0;
+  r *= (lane & 2) ? d2 : 1.0;
+  r *= (lane & 4) ? d4 : 1.0;
+  r *= (lane & 8) ? d8 : 1.0;
+  r *= (lane & 16) ? d16 : 1.0;
+  if (lane < DA_POWERS) table[lane] = (float)(lane == 32 ? d16 * d16 : r);
+  wave_lds_fence();
+}
+__device__ __forceinline__ float da_weight(const float* table, int n, float scale) { return n >= 0 ? table[n > 0 ? n : 0] * scale : 0.f; }
 
 // This wave's piece of a state matrix in memory: tile (s, sv), register r, lane (c, g) holds dk = NK (4 g + r) + s,
 // dv = dv0 + NV c + sv.
@@ -536,7 +529,9 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
   da_open<NK, NV, MODE, STATES>(S, a, w, lane);
 
   const double decay = (double)a.decay[h];
-  const DaPowers pw(decay);
+  __shared__ float lds_powers[DA_WAVES][DA_POWERS];
+  float* powers = lds_powers[threadIdx.x >> 6];
+  da_powers(powers, decay, lane);
   bool dropped = false;  // a reset inside the segment
   float head_w = 0.f, pair_w[4], tail_w[4], keep_hi = 0.f, keep_lo = 0.f, keep_off = 0.f;
   const uint32_t upto = (2u << c) - 1u;  // bits 0 .. i
@@ -546,15 +541,16 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
     if (p0 == begin || (a.reverse && p0 == DA_TOKENS) || L < DA_TOKENS) {
       const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
       const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
-      const double keep = L - first == DA_TOKENS ? pw.d16 : da_power(decay, L - first);
+      const double keep = da_power(decay, L - first);
+      const float pair_scale = a.kv_scale * a.out_scale;  // (one of them is 1)
       keep_hi = (float)keep;
       keep_lo = (float)(keep - (double)keep_hi);
-      head_w = pw(c + 1 - first) * a.out_scale;
+      head_w = da_weight(powers, c + 1 - first, a.out_scale);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = 4 * g + r;
-        pair_w[r] = j <= c ? pw(c - j) * a.kv_scale * a.out_scale : 0.f;
-        tail_w[r] = j < L ? pw(L - 1 - j) * a.kv_scale : 0.f;
+        pair_w[r] = da_weight(powers, c - j, pair_scale);
+        tail_w[r] = da_weight(powers, L - 1 - j, a.kv_scale);
       }
     }
     // bit i: a reset in front of the block's token i
@@ -954,7 +950,9 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
   da_open<NK, NV, MODE, STATES>(S, a, w, lane);
 
   const double decay = (double)a.decay[h];
-  const DaPowers pw(decay);
+  __shared__ float lds_powers[DA_WAVES][DA_POWERS];
+  float* powers = lds_powers[threadIdx.x >> 6];
+  da_powers(powers, decay, lane);
   bool dropped = false;
   float head_w[2] = {0.f, 0.f}, keep_hi = 0.f, keep_lo = 0.f, keep_off = 0.f;
   // this lane's weights: within 16 tokens, from the first 16 to the last, and the two halves' up to the block's end
@@ -965,19 +963,20 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
     if (p0 == begin || (rev && p0 == DB_TOKENS) || L < DB_TOKENS) {
       const int first = a.reverse && p0 == 0 ? 1 : 0;  // the first token in reverse: nothing decays in front of it
       const int c = da_here(lane) & 15, g = da_here(lane) >> 4;
-      const double keep = L - first == DB_TOKENS ? pw.d32 : da_power(decay, L - first);
+      const double keep = da_power(decay, L - first);
+      const float pair_scale = a.kv_scale * a.out_scale;  // (one of them is 1)
       keep_hi = (float)keep;
       keep_lo = (float)(keep - (double)keep_hi);
-      head_w[0] = pw(c + 1 - first) * a.out_scale;
-      head_w[1] = pw(c + 17 - first) * a.out_scale;
+      head_w[0] = da_weight(powers, c + 1 - first, a.out_scale);
+      head_w[1] = da_weight(powers, c + 17 - first, a.out_scale);
       float x[16];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = 4 * g + r;
-        x[r] = j <= c ? pw(c - j) * a.kv_scale * a.out_scale : 0.f;
-        x[4 + r] = pw(16 + c - j) * a.kv_scale * a.out_scale;
-        x[8 + r] = j < L ? pw(L - 1 - j) * a.kv_scale : 0.f;
-        x[12 + r] = j + 16 < L ? pw(L - 17 - j) * a.kv_scale : 0.f;
+        x[r] = da_weight(powers, c - j, pair_scale);
+        x[4 + r] = da_weight(powers, 16 + c - j, pair_scale);
+        x[8 + r] = da_weight(powers, L - 1 - j, a.kv_scale);
+        x[12 + r] = da_weight(powers, L - 17 - j, a.kv_scale);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) weights[i * WAVE] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};

@@ -2,11 +2,15 @@
 import pytest
 import torch
 
-from memory_cases import HALF_STEP, U32
+from memory_cases import HALF_STEP, U32, assert_within, attention, attention_bounds
 from omniisaacgymenvs_amd.utils.rlgames.memory_ops import decay_attention
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+
+
+def _cpu(x):
+    return None if x is None else x.detach().cpu()
 
 
 # ------------------------------------------------------------------------------------------------ 32-bit factors of bf16 products
@@ -54,3 +58,44 @@ def test_decay_attention_bf16_products_of_pairs_of_tokens_in_32_bits(name, one, 
     x[three][0, first, 0], x[three][0, second, 0] = 1.0, -1.0
     got = _results(x)[name][0, at, 0].double()
     assert ((got - _WANT).abs() <= _BOUND).all(), (float(got.min()), float(got.max()), _WANT)
+
+
+# ------------------------------------------------------------------------------------------------ decays below zero
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("decay", [[-1.0, -0.999], [-0.99, 0.99]])
+@pytest.mark.parametrize("t, resets", [(40, 0.0), (900, 0.0), (900, 0.004)])
+def test_decay_attention_decays_below_zero(t, resets, decay, dtype):
+    """Calls that are cut over time hand a state on with decay^tokens, an odd power in the backward pass."""
+    g = torch.Generator(device=DEV).manual_seed(50)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    kw = {n: r(2, t, 2, 16).to(dtype) for n in ("q", "k", "v")}
+    kw.update(decay=torch.tensor(decay, device=DEV), state=r(2, 2, 16, 16), resets=torch.rand(2, t, generator=g, device=DEV) < resets)
+    grads = {"d_o": r(2, t, 2, 16).to(dtype), "d_state": r(2, 2, 16, 16)}
+    leaves = [kw[n].requires_grad_(True) for n in ("q", "k", "v", "state")]
+    o, state = decay_attention(**kw)
+    got = dict(zip(("o", "state", "dq", "dk", "dv", "d_state_in"), (o.detach(), state.detach(), *torch.autograd.grad((o, state), leaves, tuple(grads.values())))))
+    cpu = {n: _cpu(x) for n, x in {**kw, **grads}.items()}
+    want = attention(**cpu)
+    bound = attention_bounds(want, **cpu, dtype=dtype)
+    for name, x in got.items():
+        assert_within(x, want[name], bound[name], name)
+
+
+# ------------------------------------------------------------------------------------------------ the weights of a block's tokens
+@pytest.mark.parametrize("dtype, d, roundings", [(torch.float32, 1, 2), (torch.float32, 2, 2), (torch.bfloat16, 1, 3), (torch.bfloat16, 2, 2)])
+def test_decay_attention_weights_are_rounded_once(dtype, d, roundings):
+    """One token of ones in front of t - 1 empty ones, then an initial state of ones: every result is one power of the decay times ones
+    (d of them in o).  The power's rounding and one more (by its scale) are all there is on a term's way in a block of 16 tokens (fp32) or
+    32 (bf16).  bf16 heads of one column take two blocks of 16: decay^15, the state's decay^16 and their product, a rounding each."""
+    t, h = (16 if dtype is torch.float32 else 32), 64
+    decay = (0.3 + 0.7 * torch.rand(h, generator=torch.Generator().manual_seed(60))).to(DEV)
+    power = decay.double().cpu()[:, None] ** torch.arange(t + 1)
+    q, k, v = (torch.ones(1, t, h, d, dtype=dtype, device=DEV) for _ in range(3))
+    k[:, 1:] = 0
+    o, state = decay_attention(q, k, v, decay, scale=1.0)
+    results = [("state", state[0].amax((1, 2)), power[:, t - 1]), ("state", state[0].amin((1, 2)), power[:, t - 1])]
+    if dtype is torch.float32:
+        results.append(("o", o[0, ..., 0].t(), d * power[:, :t]))
+        results.append(("o from the state", decay_attention(q, 0 * k, v, decay, torch.ones(1, h, d, d, device=DEV), scale=1.0)[0][0, ..., 0].t(), d * power[:, 1:]))
+    for name, got, want in results:
+        assert_within(got, want, roundings * U32 * want, name)
