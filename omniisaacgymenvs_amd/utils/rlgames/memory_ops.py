@@ -8,6 +8,7 @@ They work on what the tasks hand out: ``resets`` is a task's ``reset_buf`` as it
 may be stored time first (pass ``x.transpose(0, 1)``: only the last axis has to be contiguous, and results come back in the same
 order in memory).  fp32, fp16 and bf16; every sum, statistic and state is fp32.  Calls are asynchronous launches on torch's
 current stream of the tensors' device, allocate through torch and never synchronise, so they can be captured into a graph.
+Derivatives are reverse-mode, once; forward-mode tangents and traces (torch.jit.trace, make_fx) are refused.
 A backward pass inside a capture needs leaves no eager graph of which is alive: torch ties a leaf's gradient accumulation to
 the stream it was first used on (``detach().requires_grad_()`` inside the capture gives fresh leaves).
 No torch/CPU fallback: tensors must live on a ROCm device.
@@ -20,6 +21,7 @@ from struct import Struct as _Struct
 from typing import Callable, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import _lib
 
@@ -73,6 +75,19 @@ def _tensors(what: str, required, optional=()) -> None:
     for name, t in optional:
         if t is not None and not isinstance(t, torch.Tensor):
             raise _error(f"{what}: {name} must be a tensor, got {type(t).__name__}")
+    # A launch is no torch operation: a trace would record the empty result alone, and a tangent would be lost without a word
+    if torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack() and _recording()):
+        raise _error(f"{what}: cannot be traced (capture the call into a graph instead)")
+    if forward_ad._current_level >= 0:
+        for name, t in (*required, *optional):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise _error(f"{what}: {name} has a tangent; there is no forward-mode derivative")
+
+
+def _recording() -> bool:
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+    return get_proxy_mode() is not None
 
 
 def _on_device(what: str, device: torch.device, named) -> None:

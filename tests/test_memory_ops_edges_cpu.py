@@ -1,0 +1,41 @@
+"""CPU: calls of the recurrent-policy operators that tests/test_memory_ops_cpu.py does not make, without a launch."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from omniisaacgymenvs_amd import _lib
+from omniisaacgymenvs_amd.utils.rlgames.memory_ops import decay_attention, decay_attention_step, layer_norm
+
+
+def _calls():
+    """name, function, its tensor arguments."""
+    q, k, v, decay, state = torch.ones(2, 5, 4, 8), torch.ones(2, 5, 2, 8), torch.ones(2, 5, 2, 6), torch.ones(4), torch.ones(2, 4, 8, 6)
+    return [("layer_norm", layer_norm, [torch.ones(3, 4), torch.ones(4), torch.zeros(4)]),
+            ("decay_attention", decay_attention, [q, k, v, decay, state]),
+            ("decay_attention_step", decay_attention_step, [q[:, 0], k[:, 0], v[:, 0], decay, state])]
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_tangents_are_refused(which, requires_grad):
+    name, fn, args = _calls()[which]
+    for i in range(len(args)):
+        with forward_ad.dual_level():
+            dual = list(args)
+            dual[i] = forward_ad.make_dual(args[i].clone().requires_grad_(requires_grad), torch.ones_like(args[i]))
+            with pytest.raises(_lib.OigeError, match=f"{name}: .* has a tangent"):
+                fn(*dual)
+            with pytest.raises(_lib.OigeError, match="no CPU fallback"):  # none of the arguments has one: refused for another reason
+                fn(*args)
+    with pytest.raises(_lib.OigeError, match="has a tangent"):
+        torch.func.jvp(lambda x: fn(x, *args[1:]), (args[0],), (torch.ones_like(args[0]),))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_traces_are_refused(which):
+    name, fn, args = _calls()[which]
+    with pytest.raises(_lib.OigeError, match=f"{name}: cannot be traced"):
+        torch.jit.trace(fn, tuple(args), check_trace=False)
+    with pytest.raises(_lib.OigeError, match=f"{name}: cannot be traced"):
+        make_fx(lambda *a: fn(*a))(*args)
