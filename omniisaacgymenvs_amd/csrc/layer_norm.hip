@@ -402,6 +402,7 @@ int oige_layer_norm_backward(const oige_layer_norm_io* io, oige_stream_t stream)
   const int rc = layer_norm_check(io, "layer_norm_backward");
   if (rc) return rc;
   const bool params = io->dweight || io->dbias;
+  if (io->rows == 0 && !params) return OIGE_OK;  // (no rows have no dx: its pointer may be NULL)
   OIGE_REQUIRE(io->rows == 0 || (io->dy && io->mean && io->rstd), "layer_norm_backward: null dy, mean or rstd");
   OIGE_REQUIRE(io->dx || params, "layer_norm_backward: no gradient asked for");
   OIGE_REQUIRE(!params || io->rows == 0 || io->workspace, "layer_norm_backward: the weight's gradient needs a workspace");

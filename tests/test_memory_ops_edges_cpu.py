@@ -1,4 +1,6 @@
 """CPU: calls of the recurrent-policy operators that tests/test_memory_ops_cpu.py does not make, without a launch."""
+import ctypes as C
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -39,3 +41,14 @@ def test_traces_are_refused(which):
         torch.jit.trace(fn, tuple(args), check_trace=False)
     with pytest.raises(_lib.OigeError, match=f"{name}: cannot be traced"):
         make_fx(lambda *a: fn(*a))(*args)
+
+
+def test_abi_layer_norm_backward_without_rows():
+    """An empty dx has no address: with no parameter's gradient asked for there is nothing to do."""
+    lib = _lib.load()
+    io = _lib.LayerNormIo()
+    io.dtype = io.weight_dtype = _lib.F32
+    io.rows, io.width = 0, 8
+    assert lib.oige_layer_norm_backward(C.byref(io), None) == 0
+    io.rows = 1
+    assert lib.oige_layer_norm_backward(C.byref(io), None) < 0

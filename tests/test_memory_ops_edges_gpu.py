@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from memory_cases import HALF_STEP, U32, assert_within, attention, attention_bounds
-from omniisaacgymenvs_amd.utils.rlgames.memory_ops import decay_attention
+from omniisaacgymenvs_amd.utils.rlgames.memory_ops import decay_attention, layer_norm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -99,3 +99,13 @@ def test_decay_attention_weights_are_rounded_once(dtype, d, roundings):
         results.append(("o from the state", decay_attention(q, 0 * k, v, decay, torch.ones(1, h, d, d, device=DEV), scale=1.0)[0][0, ..., 0].t(), d * power[:, 1:]))
     for name, got, want in results:
         assert_within(got, want, roundings * U32 * want, name)
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layer_norm_no_rows_and_the_gradient_of_x_alone(dtype):
+    x = torch.zeros(0, 32, dtype=dtype, device=DEV, requires_grad=True)
+    w, b = torch.ones(32, device=DEV), torch.zeros(32, device=DEV)
+    for args in ((), (w,), (None, b), (w, b)):
+        dx, = torch.autograd.grad(layer_norm(x, *args), x, torch.zeros(0, 32, dtype=dtype, device=DEV))
+        assert dx.shape == (0, 32) and dx.dtype == dtype
