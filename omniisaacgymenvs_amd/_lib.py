@@ -520,6 +520,18 @@ def load() -> C.CDLL:
     return lib
 
 
+_increment_version = torch._C._increment_version
+
+
+def wrote(*tensors: torch.Tensor) -> None:
+    """A launch writes through raw pointers, unseen by torch: move the version counters of what it wrote on, as an operation in place
+    does, so that a backward pass that saved one of them raises instead of reading the new values."""
+    try:
+        _increment_version(tensors)
+    except RuntimeError:  # (inference tensors have no counter: nothing can have saved them)
+        _increment_version([t for t in tensors if not t.is_inference()])
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = load().oige_last_error()

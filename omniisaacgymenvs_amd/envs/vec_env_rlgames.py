@@ -26,6 +26,7 @@ from datetime import datetime
 
 import torch
 
+from .. import _lib
 from ..tasks.base.rl_task import quiesce_gc
 from .vec_env_base import VecEnvBase
 
@@ -115,6 +116,7 @@ class VecEnvRLGames(VecEnvBase):
             clamped = self._persistent("_obs_clamped", t.obs_buf)
             noise = t._dr_randomizer.fused_observations_args(t.obs_buf, clamped_out=clamped, clip=t.clip_obs)
             self._obs, self._rew, self._resets, self._extras = t.post_physics_step(obs_noise=noise)
+            _lib.wrote(clamped)
             self._obs, self._obs_is_clamped = clamped, True
             self._states = t.get_states()
             self._process_data()
@@ -195,6 +197,11 @@ class VecEnvRLGames(VecEnvBase):
         self._graph.replay()
         t._step_count = getattr(t, "_step_count", 0) + 1
         t._counts_key = None
+        t._wrote(_lib.STAGE_ALL)
+        obs_dict, rew, resets, _ = self._graph_out
+        _lib.wrote(obs_dict["obs"], obs_dict["states"], rew, resets)  # (the task's own, or the graph's copies of them)
+        if t.randomize_actions:
+            _lib.wrote(self._graph_actions)
         dr = getattr(t, "_dr_randomizer", None)
         if dr is not None:
             if hasattr(dr, "_observations_step") and t.randomize_observations:

@@ -181,6 +181,7 @@ class AnymalTask(RLTask):
         rc = _lib.load().oige_anymal_flat_post_physics(C.byref(p), C.byref(s), C.byref(b), self._num_envs, stages,
                                                        _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_anymal_flat_post_physics")
+        self._wrote(stages)
         if stages & _lib.STAGE_DONE:
             self._mark_counts(self.reset_buf)
 
@@ -261,6 +262,7 @@ class AnymalTask(RLTask):
         rc = _lib.load().oige_anymal_flat_pre_physics(C.byref(p), actions.data_ptr(), C.byref(b), C.byref(r),
                                                       self.actions.data_ptr(), n, flags, _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_anymal_flat_pre_physics")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         if self.sync_free:
             self._apply_reset_writes(None)
@@ -283,5 +285,6 @@ class AnymalTask(RLTask):
         rc = _lib.load().oige_anymal_flat_reset_idx(C.byref(p), C.byref(b), C.byref(r), self._num_envs, num_resets,
                                                     _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_anymal_flat_reset_idx")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         self._apply_reset_writes(num_resets)

@@ -446,6 +446,7 @@ class AnymalTerrainTask(RLTask):
         rc = _lib.load().oige_anymal_reset_idx(C.byref(p), C.byref(s), C.byref(b), C.byref(r), self._num_envs,
                                                _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_anymal_reset_idx")
+        _lib.wrote(self.progress_buf)
         self.reset_buf[env_ids] = 1  # :358, on whatever dtype reset_buf currently has
         self._apply_reset_writes(n)
         self._bind_extras()
@@ -528,12 +529,16 @@ class AnymalTerrainTask(RLTask):
             setattr(x, name, t.data_ptr())
         return x
 
+    def _wrote(self, stages: int) -> None:  # (the stages share most of them)
+        _lib.wrote(self.obs_buf, self.rew_buf, self._reset_bool, self.timeout_buf, self.progress_buf)
+
     def _stages(self, stages: int, noise_u=None, push: bool = False):
         """One ``oige_anymal_post_physics_stages`` call; returns the reset_io block it used."""
         p, s, b, r = self._params(), self._state(), self._buffers(), self._reset_io(noise_u=noise_u, push=push)
         rc = _lib.load().oige_anymal_post_physics_stages(C.byref(p), C.byref(s), C.byref(b), C.byref(r), C.byref(self._frame()),
                                                          self._num_envs, stages, _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_anymal_post_physics_stages")
+        self._wrote(stages)
         return r
 
     def post_physics_step(self, noise_u=None):
@@ -554,6 +559,7 @@ class AnymalTerrainTask(RLTask):
             rc = _lib.load().oige_anymal_post_physics(C.byref(p), C.byref(s), C.byref(b), C.byref(r), self._num_envs,
                                                       _lib.current_stream(self.obs_buf.device))
             _lib.check(rc, "oige_anymal_post_physics")
+            self._wrote(_lib.ANYMAL_STAGE_ALL)
         if r.push_velocities:  # :450 with a device-side count: N on a push step, 0 otherwise
             self._anymals.set_velocities(self.base_velocities, indices=self._all_indices, count=self._push_count)
         self.reset_buf = self._reset_bool  # bool, as the reference rebinds it (:465)

@@ -18,6 +18,7 @@ from typing import Optional
 import numpy as np
 import torch
 
+from ... import _lib
 from ...utils.domain_randomization.randomize import Randomizer
 from ...utils.spaces import Box
 
@@ -213,8 +214,6 @@ class RLTask:
             raise RuntimeError("capture_step needs the sync-free fused path (task.sync_free = task.fused = True)")
         if not self.world.is_playing():
             raise RuntimeError("capture_step: the world is not playing")
-        from ... import _lib
-
         dev = self.obs_buf.device
         _lib.require_device_tensor(actions, torch.float32, (self._num_envs, self.num_actions), "actions")
         # graphs of an earlier capture of this task are released NOW, before the window opens (their destructors call
@@ -262,10 +261,15 @@ class RLTask:
         self._graph.replay()
         self._step_count = getattr(self, "_step_count", 0) + 1
         self._counts_key = None
+        if self._graph_post is None:
+            self._wrote(_lib.STAGE_ALL)
+        else:
+            _lib.wrote(self.reset_buf, self.progress_buf)
 
     def replay_post(self):
         """The captured ``post_physics_step`` of a ``split=True`` capture."""
         self._graph_post.replay()
+        self._wrote(_lib.STAGE_ALL)
         return self.obs_buf, self.rew_buf, self.reset_buf, self.extras
 
     # ------------------------------------------------------------------ cached C-ABI argument blocks
@@ -294,12 +298,26 @@ class RLTask:
     def invalidate_blocks(self) -> None:
         self.__dict__.pop("_blocks", None)
 
+    # ------------------------------------------------------------------ what the kernels wrote, for torch's version counters
+    def _wrote(self, stages: int) -> None:
+        """Behind a post_physics launch, in front of ``_mark_counts``."""
+        if stages == _lib.STAGE_ALL:
+            return _lib.wrote(self.obs_buf, self.states_buf, self.rew_buf, self.reset_buf, self.progress_buf)
+        if stages & _lib.STAGE_PROGRESS:
+            _lib.wrote(self.progress_buf)
+        if stages & _lib.STAGE_OBS:
+            _lib.wrote(self.obs_buf, self.states_buf)
+        if stages & _lib.STAGE_METRICS:
+            _lib.wrote(self.rew_buf)
+        if stages & _lib.STAGE_DONE:
+            _lib.wrote(self.reset_buf)
+
     # ------------------------------------------------------------------ OIGE_PRE_COUNTS_VALID bookkeeping
     # The post kernels leave the per-tile counts of the reset flags they wrote; the next pre_physics_step may skip its
     # recount only while those flags are untouched.  The key holds the flag TENSORS (not their addresses: a rebound
     # reset_buf is a different object even when the allocator hands the old address out again, and holding the old one
     # keeps its memory from being recycled) and their torch version counters.  Writers torch cannot see (another library
-    # writing through the raw pointer) must set ``task._counts_key = None`` themselves.
+    # writing through the raw pointer) must set ``task._counts_key = None`` themselves.  Marked behind ``_wrote``.
     _counts_key = None
 
     def _mark_counts(self, *flag_bufs) -> None:

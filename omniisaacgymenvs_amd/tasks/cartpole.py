@@ -93,6 +93,7 @@ class CartpoleTask(RLTask):
             _lib.current_stream(self.obs_buf.device),
         )
         _lib.check(rc, "oige_cartpole_post_physics")
+        self._wrote(stages)
         if stages & _lib.STAGE_DONE:
             self._mark_counts(self.reset_buf)
 
@@ -163,6 +164,7 @@ class CartpoleTask(RLTask):
             _lib.current_stream(self.obs_buf.device),
         )
         _lib.check(rc, "oige_cartpole_pre_physics")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         if self.sync_free:
             kw = dict(indices=o["env_ids"], count=o["count"])
@@ -185,6 +187,7 @@ class CartpoleTask(RLTask):
             C.byref(p), C.byref(b), C.byref(r), self._num_envs, num_resets, _lib.current_stream(self.obs_buf.device)
         )
         _lib.check(rc, "oige_cartpole_reset_idx")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         # apply resets
         indices = o["env_ids"][:num_resets].to(dtype=torch.int32)

@@ -179,6 +179,7 @@ class CrazyflieTask(RLTask):
         rc = _lib.load().oige_crazyflie_post_physics(C.byref(p), C.byref(s), C.byref(b), self._num_envs, stages,
                                                      _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_crazyflie_post_physics")
+        self._wrote(stages)
         if stages & _lib.STAGE_DONE:  # the DONE stage leaves the tile counts of both lists pre_physics_step compacts
             self._mark_counts(self.reset_buf, self.progress_buf)
         elif stages & _lib.STAGE_PROGRESS:  # progress moved under the target list's counts (a raw-pointer write: no version bump)
@@ -273,6 +274,7 @@ class CrazyflieTask(RLTask):
         rc = _lib.load().oige_crazyflie_pre_physics(C.byref(p), actions.data_ptr(), self.root_rot.data_ptr(), C.byref(b), C.byref(r),
                                                     n, flags, _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_crazyflie_pre_physics")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None  # the kernel cleared the flags of the envs it reset (raw-pointer writes: no version bump)
         if self.sync_free:
             self._bind_extras()  # holds the last reset's means; untouched on steps without a reset, as in the reference
@@ -314,6 +316,7 @@ class CrazyflieTask(RLTask):
         rc = _lib.load().oige_crazyflie_reset_idx(C.byref(p), C.byref(b), C.byref(r), self._num_envs, num_resets,
                                                   _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_crazyflie_reset_idx")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._apply_reset_writes(num_resets)
         self.extras["episode"] = {}  # :331-335
         for key in self.episode_sums.keys():

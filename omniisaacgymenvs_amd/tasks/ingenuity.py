@@ -149,6 +149,7 @@ class IngenuityTask(RLTask):
         rc = _lib.load().oige_ingenuity_post_physics(C.byref(p), C.byref(s), C.byref(b), self._num_envs, stages,
                                                      _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_ingenuity_post_physics")
+        self._wrote(stages)
         if stages & _lib.STAGE_DONE:  # the DONE stage leaves the tile counts of both lists pre_physics_step compacts
             self._mark_counts(self.reset_buf, self.progress_buf)
         elif stages & _lib.STAGE_PROGRESS:  # progress moved under the target list's counts (a raw-pointer write: no version bump)
@@ -250,6 +251,7 @@ class IngenuityTask(RLTask):
         rc = _lib.load().oige_ingenuity_pre_physics(C.byref(p), actions.data_ptr(), C.byref(b), C.byref(r), n, flags,
                                                     _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_ingenuity_pre_physics")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None  # the kernel cleared the flags of the envs it reset (raw-pointer writes: no version bump)
         if self.sync_free:
             self._apply_reset_writes(None)
@@ -296,4 +298,5 @@ class IngenuityTask(RLTask):
         rc = _lib.load().oige_ingenuity_reset_idx(C.byref(p), C.byref(b), C.byref(r), self._num_envs, num_resets,
                                                   _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_ingenuity_reset_idx")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._apply_reset_writes(num_resets)

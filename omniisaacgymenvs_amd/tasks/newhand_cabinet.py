@@ -284,6 +284,7 @@ class _NewhandCabinetTask(RLTask):
         rc = _lib.load().oige_newhand_cabinet_post_physics(C.byref(p), C.byref(s), C.byref(b), self._num_envs, stages,
                                                            _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_newhand_cabinet_post_physics")
+        self._wrote(stages)
         if stages & _lib.STAGE_DONE:
             self._mark_counts(self.reset_buf)
 
@@ -368,6 +369,7 @@ class _NewhandCabinetTask(RLTask):
         rc = _lib.load().oige_newhand_cabinet_pre_physics(C.byref(p), actions.data_ptr(), C.byref(b), C.byref(r), n, flags,
                                                           _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_newhand_cabinet_pre_physics")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         if self.sync_free:
             self._apply_reset_writes(None)
@@ -391,6 +393,7 @@ class _NewhandCabinetTask(RLTask):
         rc = _lib.load().oige_newhand_cabinet_reset_idx(C.byref(p), C.byref(b), C.byref(r), self._num_envs, num,
                                                         _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_newhand_cabinet_reset_idx")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         self._apply_reset_writes(num)
 

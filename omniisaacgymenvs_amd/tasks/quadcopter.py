@@ -160,6 +160,7 @@ class QuadcopterTask(RLTask):
         rc = _lib.load().oige_quadcopter_post_physics(C.byref(p), C.byref(s), C.byref(b), self._num_envs, stages,
                                                       _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_quadcopter_post_physics")
+        self._wrote(stages)
         if stages & _lib.STAGE_DONE:
             self._mark_counts(self.reset_buf)
 
@@ -238,6 +239,7 @@ class QuadcopterTask(RLTask):
         rc = _lib.load().oige_quadcopter_pre_physics(C.byref(p), actions.data_ptr(), C.byref(b), C.byref(r), n, flags,
                                                      _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_quadcopter_pre_physics")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         if self.sync_free:
             self._apply_reset_writes(None)
@@ -268,6 +270,7 @@ class QuadcopterTask(RLTask):
         rc = _lib.load().oige_quadcopter_reset_idx(C.byref(p), C.byref(b), C.byref(r), self._num_envs, num_resets,
                                                    _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_quadcopter_reset_idx")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         self._apply_reset_writes(num_resets)
         self._balls.set_world_poses(positions=self.target_positions[:, 0:3] + self._env_pos)

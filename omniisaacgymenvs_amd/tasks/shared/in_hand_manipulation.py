@@ -267,8 +267,15 @@ class InHandManipulationTask(RLTask):
             rc = _lib.load().oige_hand_post_physics(C.byref(p), C.byref(s), C.byref(b), self._num_envs, stages,
                                                     _lib.current_stream(self.obs_buf.device))
             _lib.check(rc, "oige_hand_post_physics")
+        self._wrote(stages)
         if stages & _lib.STAGE_METRICS:
             self._mark_counts(self.reset_buf, self.reset_goal_buf)
+
+    def _wrote(self, stages: int) -> None:
+        if not stages & _lib.STAGE_METRICS:
+            return RLTask._wrote(self, stages)
+        seen = (self.obs_buf, self.states_buf) if stages & _lib.STAGE_OBS else ()
+        _lib.wrote(self.rew_buf, self.reset_buf, self.reset_goal_buf, self.progress_buf, *seen)  # the resets come with the reward
 
     # ------------------------------------------------------------------ RLTask methods
     def get_observations(self):
@@ -405,11 +412,13 @@ class InHandManipulationTask(RLTask):
                 C.byref(p), actions.data_ptr(), C.byref(b), C.byref(r), C.byref(action_noise), self.actions.data_ptr(),
                 self._targets_out.data_ptr(), n, flags, _lib.current_stream(self.obs_buf.device))
             _lib.check(rc, "oige_hand_pre_physics_dr")
+            _lib.wrote(actions)  # it leaves the noised values there
         else:
             rc = _lib.load().oige_hand_pre_physics(
                 C.byref(p), actions.data_ptr(), C.byref(b), C.byref(r), self.actions.data_ptr(), self._targets_out.data_ptr(),
                 n, flags, _lib.current_stream(self.obs_buf.device))
             _lib.check(rc, "oige_hand_pre_physics")
+        _lib.wrote(self.reset_buf, self.reset_goal_buf, self.progress_buf)
         self._counts_key = None
         if self.sync_free:
             self._apply_goal_writes(None)
@@ -434,6 +443,7 @@ class InHandManipulationTask(RLTask):
         rc = _lib.load().oige_hand_reset_target_pose(C.byref(p), C.byref(b), C.byref(r), self._num_envs, n,
                                                      _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_hand_reset_target_pose")
+        _lib.wrote(self.reset_goal_buf)
         self._counts_key = None
         self._apply_goal_writes(n)
 
@@ -453,6 +463,7 @@ class InHandManipulationTask(RLTask):
         rc = _lib.load().oige_hand_reset_idx(C.byref(p), C.byref(b), C.byref(r), self._num_envs, n,
                                              _lib.current_stream(self.obs_buf.device))
         _lib.check(rc, "oige_hand_reset_idx")
+        _lib.wrote(self.reset_buf, self.reset_goal_buf, self.progress_buf)
         self._counts_key = None
         self.hand_dof_targets[env_ids, :] = o["dof_pos"][:n]
         self._apply_reset_writes(n)

@@ -199,6 +199,7 @@ class LocomotionTask(RLTask):
             _lib.current_stream(self.obs_buf.device),
         )
         _lib.check(rc, "oige_locomotion_post_physics")
+        self._wrote(stages)
         if stages & _lib.STAGE_DONE:
             self._mark_counts(self.reset_buf)
 
@@ -300,6 +301,7 @@ class LocomotionTask(RLTask):
             n, flags, _lib.current_stream(self.obs_buf.device),
         )
         _lib.check(rc, "oige_locomotion_pre_physics")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         if self.sync_free:
             self._apply_reset_writes(None)
@@ -328,6 +330,7 @@ class LocomotionTask(RLTask):
             C.byref(p), C.byref(b), C.byref(r), self._num_envs, num_resets, _lib.current_stream(self.obs_buf.device)
         )
         _lib.check(rc, "oige_locomotion_reset_idx")
+        _lib.wrote(self.reset_buf, self.progress_buf)
         self._counts_key = None
         self._apply_reset_writes(num_resets)
 

@@ -125,5 +125,6 @@ def apply(buffer: torch.Tensor, reset_buf: torch.Tensor, counter: torch.Tensor, 
         a.interval_samples = (it if it is not None and m > 0 else one).data_ptr()
         keep += [rs, it, one]
     _lib.check(lib.oige_dr_noise_apply(C.byref(a), n, stream), "oige_dr_noise_apply")
+    _lib.wrote(*((buffer,) if clamped_out is None else (buffer, clamped_out)))
     state._keep = keep
     return buffer

@@ -9,6 +9,8 @@ may be stored time first (pass ``x.transpose(0, 1)``: only the last axis has to 
 order in memory).  fp32, fp16 and bf16; every sum, statistic and state is fp32.  Calls are asynchronous launches on torch's
 current stream of the tensors' device, allocate through torch and never synchronise, so they can be captured into a graph.
 Derivatives are reverse-mode, once; forward-mode tangents and traces (torch.jit.trace, make_fx) are refused.
+What a call saved for its backward pass and an env step has written since (``obs_buf``, ``reset_buf``, the clamped observations) makes
+that pass raise: a rollout that is trained on is a copy.
 A backward pass inside a capture needs leaves no eager graph of which is alive: torch ties a leaf's gradient accumulation to
 the stream it was first used on (``detach().requires_grad_()`` inside the capture gives fresh leaves).
 No torch/CPU fallback: tensors must live on a ROCm device.
