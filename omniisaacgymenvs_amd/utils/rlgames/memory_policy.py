@@ -39,6 +39,14 @@ class MemoryBlock(nn.Module):
         # memories from 4 to 512 steps long
         self.register_buffer("decay", 1 - torch.exp2(-2 - 7 * torch.arange(heads, dtype=torch.float32) / max(heads - 1, 1)))
 
+    def _apply(self, fn, recurse: bool = True):
+        """``.half()``, ``.to(torch.bfloat16)``: the decays stay in 32 bits (0.998 would be 1 in bf16) and move with the weights."""
+        decay = self.decay
+        super()._apply(fn, recurse)
+        if self.decay.dtype is not torch.float32:
+            self.decay = decay.to(self.decay.device)
+        return self
+
     def _heads(self, x: torch.Tensor):
         qkv = self.qkv(self.norm(x)).unflatten(-1, (3, self.heads, self.head_dim))
         return qkv.unbind(-3)
@@ -52,7 +60,8 @@ class MemoryBlock(nn.Module):
 
 
 class MemoryPolicy(nn.Module):
-    """Observations -> action means in (-1, 1) and values, through ``layers`` memory blocks."""
+    """Observations -> action means in (-1, 1) and values, through ``layers`` memory blocks.  Runs in fp32, cast to fp16 or bf16 (with
+    observations of that type), or under autocast."""
 
     def __init__(self, num_observations: int, num_actions: int, width: int = 256, heads: int = 4, layers: int = 1):
         super().__init__()
@@ -62,9 +71,9 @@ class MemoryPolicy(nn.Module):
         self.mu, self.value = nn.Linear(width, num_actions), nn.Linear(width, 1)
 
     def initial_state(self, num_envs: int) -> torch.Tensor:
-        """(layers, N, heads, head_dim, head_dim), empty memories."""
+        """(layers, N, heads, head_dim, head_dim), empty memories; in 32 bits whatever the policy's type."""
         b = self.blocks[0]
-        return torch.zeros(len(self.blocks), num_envs, b.heads, b.head_dim, b.head_dim, device=b.decay.device)
+        return torch.zeros(len(self.blocks), num_envs, b.heads, b.head_dim, b.head_dim, dtype=torch.float32, device=b.decay.device)
 
     def _read(self, x):
         x = self.norm(x)

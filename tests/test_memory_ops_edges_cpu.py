@@ -52,3 +52,20 @@ def test_abi_layer_norm_backward_without_rows():
     assert lib.oige_layer_norm_backward(C.byref(io), None) == 0
     io.rows = 1
     assert lib.oige_layer_norm_backward(C.byref(io), None) < 0
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.bfloat16().float(), lambda m: m.to("meta", torch.float16)])
+def test_policy_keeps_decays_and_states_in_32_bits(cast):
+    from omniisaacgymenvs_amd.utils.rlgames.memory_policy import MemoryPolicy
+
+    want = MemoryPolicy(10, 2, width=32, heads=4, layers=2).blocks[1].decay.clone()
+    policy = cast(MemoryPolicy(10, 2, width=32, heads=4, layers=2))
+    for block in policy.blocks:
+        assert block.decay.dtype == torch.float32 and block.decay.device == policy.mu.weight.device
+        assert block.decay.is_meta or torch.equal(block.decay, want)
+    torch.set_default_dtype(torch.float64)
+    try:
+        state = policy.initial_state(3)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert state.dtype == torch.float32 and state.device == policy.mu.weight.device and state.shape == (2, 3, 4, 8, 8)
