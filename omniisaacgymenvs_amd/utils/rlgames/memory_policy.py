@@ -11,7 +11,7 @@ from typing import Optional, Tuple
 import torch
 from torch import nn
 
-from .memory_ops import decay_attention, decay_attention_step, layer_norm
+from .memory_ops import MAX_HEAD_DIM, MAX_WIDTH, decay_attention, decay_attention_step, layer_norm
 
 
 class LayerNorm(nn.Module):
@@ -30,8 +30,10 @@ class MemoryBlock(nn.Module):
 
     def __init__(self, width: int, heads: int):
         super().__init__()
-        if width % heads:
+        if heads < 1 or width < 1 or width % heads:
             raise ValueError(f"MemoryBlock: width {width} is not a multiple of {heads} heads")
+        if width > MAX_WIDTH or width // heads > MAX_HEAD_DIM:
+            raise ValueError(f"MemoryBlock: width {width} over {heads} heads; heads are 1 to {MAX_HEAD_DIM} wide, all of them {MAX_WIDTH}")
         self.heads, self.head_dim = heads, width // heads
         self.norm = LayerNorm(width)
         self.qkv = nn.Linear(width, 3 * width, bias=False)
@@ -65,6 +67,8 @@ class MemoryPolicy(nn.Module):
 
     def __init__(self, num_observations: int, num_actions: int, width: int = 256, heads: int = 4, layers: int = 1):
         super().__init__()
+        if layers < 1:
+            raise ValueError(f"MemoryPolicy: {layers} layers")
         self.encoder = nn.Linear(num_observations, width)
         self.blocks = nn.ModuleList(MemoryBlock(width, heads) for _ in range(layers))
         self.norm = LayerNorm(width)

@@ -69,3 +69,14 @@ def test_policy_keeps_decays_and_states_in_32_bits(cast):
     finally:
         torch.set_default_dtype(torch.float32)
     assert state.dtype == torch.float32 and state.device == policy.mu.weight.device and state.shape == (2, 3, 4, 8, 8)
+
+
+@pytest.mark.parametrize("kw, match", [({"width": 1024, "heads": 4}, "1 to 128 wide"), ({"width": 129, "heads": 1}, "1 to 128 wide"),
+                                       ({"width": 128 * 129, "heads": 129}, "all of them 16384"), ({"width": 32, "heads": 0}, "not a multiple"),
+                                       ({"width": 0, "heads": 4}, "not a multiple"), ({"layers": 0}, "0 layers")])
+def test_policy_refuses_what_no_call_would_take(kw, match):
+    from omniisaacgymenvs_amd.utils.rlgames.memory_policy import MemoryPolicy
+
+    with pytest.raises(ValueError, match=match):
+        MemoryPolicy(10, 2, **kw)
+    MemoryPolicy(10, 2, width=128, heads=1)
