@@ -1355,6 +1355,8 @@ __global__ __launch_bounds__(256) void decay_attention_step_kernel(const DaStep 
 }
 
 // ---------------------------------------------------------------- host side
+constexpr int64_t DA_MAX_BLOCKS = ((int64_t)1 << 24) - 1;  // workgroups of 256: a launch's threads are counted in 32 bits
+
 struct DaPlan {
   int nk, nv, slices, nseg;
   int64_t seg_len, seg_floats;  // scratch: states between segments and the segments' factors
@@ -1408,7 +1410,7 @@ static int decay_attention_run(const DaRoles& in, const DaPlan& p, float* worksp
   DaRoles r = in;
   const int64_t heads = r.c[0].n * r.c[0].h, units = heads * p.slices, groups = ((units + DA_WAVES - 1) / DA_WAVES + DA_XCDS - 1) / DA_XCDS;
   const int64_t blocks = groups * DA_XCDS * r.roles, per_head = (int64_t)p.slices * NK * NV * WAVE;  // the last in 16-byte quads
-  OIGE_REQUIRE(groups * DA_XCDS * DA_WAVES < ((int64_t)1 << 31) && blocks < ((int64_t)1 << 31),
+  OIGE_REQUIRE(blocks <= DA_MAX_BLOCKS,
                "decay_attention: %lld sequences x heads are too many for one launch", (long long)heads);
   for (int i = 0; i < r.roles; ++i) {
     DaCore& c = r.c[i];
@@ -1515,22 +1517,29 @@ static int decay_attention_core(const DaRoles& r, int dtype, float* ws, hipStrea
               : wide ? decay_attention_tiles<float, ELEMS_WIDE>(r, p, ws, s) : decay_attention_tiles<float, ELEMS_LOOSE>(r, p, ws, s);
 }
 
-static int decay_attention_share(const float* in_k, const float* in_v, const oige_decay_attention_io& io, hipStream_t s) {
+// The share kernel's accesses and workgroups, checked in front of the pass's first launch.
+struct DaSharePlan {
+  DaShare k, v;
+  bool wide;  // four columns to a thread
+  int64_t rows, blocks;
+};
+static DaSharePlan decay_attention_share_plan(const float* in_k, const float* in_v, const oige_decay_attention_io& io) {
   const int64_t *sk = io.dk_stride, *sv = io.dv_stride;
-  const DaShare k{in_k, io.dk, sk[0], sk[1], sk[2], io.key_dim}, v{in_v, io.dv, sv[0], sv[1], sv[2], io.value_dim};
-  bool wide = true;  // four columns to a thread
-  for (const DaShare& x : {k, v})
-    wide = wide && x.d % 4 == 0 && x.on % 4 == 0 && x.ot % 4 == 0 && x.oh % 4 == 0 && aligned16(x.in) && aligned16(x.out);
-  const int64_t rows = io.num_envs * io.num_tokens * io.kv_heads;
-  const int d = io.key_dim > io.value_dim ? io.key_dim : io.value_dim, each = 256 / (wide ? d / 4 : d);
-  const int64_t blocks = (rows + each - 1) / each;
-  OIGE_REQUIRE(blocks < ((int64_t)1 << 31), "decay_attention_backward: too many key / value rows for one launch");
-  const dim3 grid((unsigned)blocks, 2);
+  DaSharePlan p{{in_k, io.dk, sk[0], sk[1], sk[2], io.key_dim}, {in_v, io.dv, sv[0], sv[1], sv[2], io.value_dim}, true, 0, 0};
+  for (const DaShare& x : {p.k, p.v})
+    p.wide = p.wide && x.d % 4 == 0 && x.on % 4 == 0 && x.ot % 4 == 0 && x.oh % 4 == 0 && aligned16(x.in) && aligned16(x.out);
+  p.rows = io.num_envs * io.num_tokens * io.kv_heads;
+  const int d = io.key_dim > io.value_dim ? io.key_dim : io.value_dim, each = 256 / (p.wide ? d / 4 : d);
+  p.blocks = (p.rows + each - 1) / each;
+  return p;
+}
+static int decay_attention_share(const DaSharePlan& p, const oige_decay_attention_io& io, hipStream_t s) {
+  const dim3 grid((unsigned)p.blocks, 2);
   const int t = (int)io.num_tokens, hk = (int)io.kv_heads, group = io.heads / io.kv_heads;
 #define OIGE_SHARE(T)                                                                                                                    \
   do {                                                                                                                                   \
-    if (wide) hipLaunchKernelGGL((decay_attention_share_kernel<T, 4>), grid, dim3(256), 0, s, k, v, rows, t, hk, group);                 \
-    else hipLaunchKernelGGL((decay_attention_share_kernel<T, 1>), grid, dim3(256), 0, s, k, v, rows, t, hk, group);                      \
+    if (p.wide) hipLaunchKernelGGL((decay_attention_share_kernel<T, 4>), grid, dim3(256), 0, s, p.k, p.v, p.rows, t, hk, group);         \
+    else hipLaunchKernelGGL((decay_attention_share_kernel<T, 1>), grid, dim3(256), 0, s, p.k, p.v, p.rows, t, hk, group);                \
   } while (0)
   if (io.dtype == OIGE_F32) OIGE_SHARE(float);
   else if (io.dtype == OIGE_F16) OIGE_SHARE(_Float16);
@@ -1660,9 +1669,12 @@ int oige_decay_attention_backward(const oige_decay_attention_io* io, oige_stream
   // shared heads: dk and dv per query head in fp32 behind the segments' scratch, then their sums
   const int64_t t = io->num_tokens, h = io->heads;
   float *wide_v = nullptr, *wide_k = nullptr;
+  DaSharePlan share{};
   if (group > 1) {
     wide_v = io->workspace + (need - io->num_envs * t * h * (io->key_dim + io->value_dim));
     wide_k = wide_v + io->num_envs * t * h * io->value_dim;
+    share = decay_attention_share_plan(wide_k, wide_v, *io);
+    OIGE_REQUIRE(share.blocks <= DA_MAX_BLOCKS, "decay_attention_backward: %lld key / value rows are too many for one launch", (long long)share.rows);
   }
   const int64_t rows_v[3] = {t * h * io->value_dim, h * io->value_dim, io->value_dim}, rows_k[3] = {t * h * io->key_dim, h * io->key_dim, io->key_dim};
   DaRoles r{};
@@ -1716,7 +1728,7 @@ int oige_decay_attention_backward(const oige_decay_attention_io* io, oige_stream
     }
   }
   if (group == 1) return OIGE_OK;
-  return decay_attention_share(wide_k, wide_v, *io, s);
+  return decay_attention_share(share, *io, s);
 }
 
 int oige_decay_attention_step(const oige_decay_attention_step_io* io, oige_stream_t stream) {
@@ -1759,7 +1771,7 @@ int oige_decay_attention_step(const oige_decay_attention_step_io* io, oige_strea
   while (a.lanes < pieces) a.lanes *= 2;  // 32 at most
   const bool big = io->key_dim * io->value_dim > 2048;
   const int64_t units = a.n * a.h, blocks = big ? units : (units + 3) / 4;
-  OIGE_REQUIRE(blocks < ((int64_t)1 << 31), "decay_attention_step: %lld sequences x heads are too many for one launch", (long long)units);
+  OIGE_REQUIRE(blocks <= DA_MAX_BLOCKS, "decay_attention_step: %lld sequences x heads are too many for one launch", (long long)units);
   hipStream_t s = (hipStream_t)stream;
 #define OIGE_STEP(T)                                                                                                                       \
   do {                                                                                                                                     \

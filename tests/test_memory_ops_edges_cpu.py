@@ -80,3 +80,37 @@ def test_policy_refuses_what_no_call_would_take(kw, match):
     with pytest.raises(ValueError, match=match):
         MemoryPolicy(10, 2, **kw)
     MemoryPolicy(10, 2, width=128, heads=1)
+
+
+# ------------------------------------------------------------------------------------------------ launches of 2^32 threads and more
+# (Only calls that are refused: the pointers are no memory.)
+def _attention_io(n, t, heads, kv_heads, d):
+    io = _lib.DecayAttentionIo()
+    io.dtype, io.num_envs, io.num_tokens, io.heads, io.kv_heads, io.key_dim, io.value_dim = _lib.F32, n, t, heads, kv_heads, d, d
+    for name in ("q", "k", "v", "o", "decay", "d_o", "dq", "dk", "dv", "workspace"):
+        setattr(io, name, 1 << 20)
+    return io
+
+
+@pytest.mark.parametrize("n, heads, d, back", [(1 << 26, 1, 8, 0), (1 << 24, 4, 16, 0), (1 << 25, 1, 128, 0), (1 << 25, 1, 16, 1), (22400000, 1, 8, 1), (1 << 40, 4, 1, 1)])
+def test_abi_decay_attention_refuses_too_many_sequences(n, heads, d, back):
+    lib, io = _lib.load(), _attention_io(n, 2, heads, heads, d)
+    io.workspace_floats = lib.oige_decay_attention_workspace_floats(C.byref(io), back)
+    fn = lib.oige_decay_attention_backward if back else lib.oige_decay_attention_forward
+    assert fn(C.byref(io), None) < 0 and "too many for one launch" in lib.oige_last_error().decode()
+
+
+def test_abi_decay_attention_refuses_too_many_shared_rows_in_front_of_the_first_launch():
+    lib, io = _lib.load(), _attention_io(1 << 12, 1 << 17, 2, 1, 128)
+    io.workspace_floats = lib.oige_decay_attention_workspace_floats(C.byref(io), 1)
+    assert lib.oige_decay_attention_backward(C.byref(io), None) < 0
+    assert f"{1 << 29} key / value rows are too many" in lib.oige_last_error().decode()
+
+
+@pytest.mark.parametrize("n, heads, d", [(1 << 26, 1, 8), (1 << 23, 8, 16), (1 << 24, 1, 64), (1 << 40, 2, 1)])
+def test_abi_decay_attention_step_refuses_too_many_sequences(n, heads, d):
+    lib, io = _lib.load(), _lib.DecayAttentionStepIo()
+    io.dtype, io.num_envs, io.heads, io.kv_heads, io.key_dim, io.value_dim = _lib.BF16, n, heads, heads, d, d
+    for name in ("q", "k", "v", "o", "state", "decay"):
+        setattr(io, name, 1 << 20)
+    assert lib.oige_decay_attention_step(C.byref(io), None) < 0 and "too many for one launch" in lib.oige_last_error().decode()
