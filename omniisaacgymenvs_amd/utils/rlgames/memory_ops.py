@@ -18,7 +18,6 @@ No torch/CPU fallback: tensors must live on a ROCm device.
 from __future__ import annotations
 
 import ctypes as C
-import math
 from struct import Struct as _Struct
 from typing import Callable, Optional, Tuple
 
@@ -34,6 +33,7 @@ MAX_WIDTH = 16384
 _TYPES = _lib.ELEM_TYPES
 _FLAGS = (torch.bool, torch.uint8, torch.int64)
 _error = _lib.OigeError
+_LARGEST = torch.finfo(torch.float32).max  # of eps and scale, which the kernels take in 32 bits
 
 
 def _packer(struct) -> Callable[..., bytes]:
@@ -184,7 +184,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise _error(f"layer_norm: weight is {weight.dtype} and bias {bias.dtype}; they need one type")
     eps = float(eps)
-    if not (math.isfinite(eps) and eps >= 0):
+    if not 0 <= eps <= _LARGEST:
         raise _error(f"layer_norm: eps = {eps}")
     _on_device("layer_norm", x.device, (("weight", weight), ("bias", bias)))
     weight = None if weight is None else _last_contiguous(weight)
@@ -326,7 +326,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     if lengths is not None and (lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != q.shape[:1]):
         raise _error(f"{what}: lengths must be int32 or int64 of shape {(q.shape[0],)}, got {lengths.dtype} {tuple(lengths.shape)}")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if not abs(scale) <= _LARGEST:
         raise _error(f"{what}: scale = {scale}")
     _on_device(what, q.device, (("k", k), ("v", v), ("decay", decay), ("state", state), ("resets", resets), ("lengths", lengths)))
     args = (_last_contiguous(q), _last_contiguous(k), _last_contiguous(v), None if state is None else state.contiguous(), decay.contiguous(),
@@ -347,7 +347,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, deca
     if _needs_grad(q, k, v, state):
         raise _error(f"{what}: updates the state in place and has no gradient; use decay_attention, or torch.no_grad()")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if not abs(scale) <= _LARGEST:
         raise _error(f"{what}: scale = {scale}")
     device = q.device
     _on_device(what, device, (("k", k), ("v", v), ("decay", decay), ("state", state), ("resets", resets)))

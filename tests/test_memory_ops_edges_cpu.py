@@ -114,3 +114,13 @@ def test_abi_decay_attention_step_refuses_too_many_sequences(n, heads, d):
     for name in ("q", "k", "v", "o", "state", "decay"):
         setattr(io, name, 1 << 20)
     assert lib.oige_decay_attention_step(C.byref(io), None) < 0 and "too many for one launch" in lib.oige_last_error().decode()
+
+
+@pytest.mark.parametrize("value", [1e39, -1e39, float("inf"), float("nan")])
+def test_scale_and_eps_beyond_32_bits_are_refused(value):
+    (_, norm, x), (_, attention, seq), (_, step, one) = _calls()
+    with pytest.raises(_lib.OigeError, match="eps"):
+        norm(*x, eps=value)
+    for fn, args in ((attention, seq), (step, one)):
+        with pytest.raises(_lib.OigeError, match="scale"):
+            fn(*args, scale=value)
