@@ -264,9 +264,26 @@ __device__ __forceinline__ void da_state_part(f32x4 (&acc)[NV], const f32x4 (&S)
 }
 
 // No conditional block stands between a matrix instruction and the first ordinary one that reads its result: with one, the
-// compiler has counted the wait states of the longer way only, and the shorter way read the registers too early.
-// da_settle() stands where the state's tiles leave the loop.
-__device__ __forceinline__ void da_settle() { asm volatile("s_nop 15" ::: "memory"); }
+// compiler has counted the wait states of the longer way only, and the shorter way read the registers too early.  Where branches
+// follow (the stores, the loop's end) the tiles pass through da_settle: the products come in front of its wait and whatever reads
+// them behind it, since both sides of the wait claim to change them.
+template <int A, int B>
+__device__ __forceinline__ void da_settle(f32x4 (&x)[A][B]) {
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int b = 0; b < B; ++b) asm volatile("" : "+v"(x[a][b]));
+  asm volatile("s_nop 15" ::: "memory");
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int b = 0; b < B; ++b) asm volatile("" : "+v"(x[a][b]));
+}
+
+template <int B>
+__device__ __forceinline__ void da_settle(f32x4 (&x)[B]) {
+  da_settle(reinterpret_cast<f32x4(&)[1][B]>(x));
+}
 
 // One block's rows of the operands.  Rows behind the block's L tokens re-read its last one; `low` is the earliest of its tokens
 // in memory, and in reverse the block's first token is the latest.
@@ -463,7 +480,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
   if (!w.live || (STATES && w.seg >= w.last)) return;
   const int64_t n = w.n;
   const int len = w.len, begin = w.begin, end = w.end;
-  const int h = w.h, seg = w.seg, slice = w.slice, dv0 = w.dv0;
+  const int h = w.h, dv0 = w.dv0;
 
   const T* qh = static_cast<const T*>(a.q.p) + n * a.q.sn + (int64_t)(h / a.q.group) * a.q.sh;
   const T* kh = static_cast<const T*>(a.k.p) + n * a.k.sn + (int64_t)(h / a.k.group) * a.k.sh;
@@ -609,13 +626,13 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
 #pragma unroll
           for (int sv = 0; sv < NV; ++sv)
             acc[sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(da_finite(V[r][sv]) ? V[r][sv] : 0.f, P[r], acc[sv], 0, 0, 0);
-        da_settle();
+        da_settle(acc);
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int sv = 0; sv < NV; ++sv) acc[sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[r][sv], P[r], acc[sv], 0, 0, 0);
-        da_settle();
+        da_settle(acc);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -672,7 +689,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_kernel(cons
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[s][sv] = __builtin_amdgcn_mfma_f32_16x16x4f32(K2[r][s], V[r][sv], S[s][sv], 0, 0, 0);
       }
-    da_settle();
+    da_settle(S);
     blk = next;
   }
   da_close<T, NK, NV, MODE, STATES>(S, da_again(roles), w, lane, decay, dropped);
@@ -1088,7 +1105,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
             for (int part = 0; part < 3; ++part) acc[it][sv] = db_mfma(v, parts[part][it], acc[it][sv]);
           }
         }
-        da_settle();
+        da_settle(acc);
       } else {
         u32x4 v[NV];
 #pragma unroll
@@ -1103,7 +1120,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
           for (int sv = 0; sv < NV; ++sv)
 #pragma unroll
             for (int it = 0; it < 2; ++it) acc[it][sv] = db_mfma(v[sv], parts[part][it], acc[it][sv]);
-        da_settle();
+        da_settle(acc);
       }
       if (more) issue_q(next);
       else forget(q_run);
@@ -1189,7 +1206,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
         for (int sv = 0; sv < NV; ++sv) S[s][sv] = db_mfma(k, part == 0 ? vl3[sv] : part == 1 ? vm3[sv] : vh3[sv], S[s][sv]);
     }
     wave_lds_fence();
-    da_settle();
+    da_settle(S);
     blk = next;
   }
   da_close<__bf16, NK, NV, MODE, STATES>(S, da_again(roles), w, lane, decay, dropped);
