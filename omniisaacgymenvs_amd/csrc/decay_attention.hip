@@ -53,8 +53,8 @@ struct DaCore {
   const float* s_in;   // NULL: zero
   float* s_out;        // NULL: not wanted
   float* seg_states;   // states between time segments, in register order
-  float* seg_factors;  // (N, H, nseg): what a segment multiplies the state with, -1: it drops it.  (Those that are read are powers of 32 m
-                       // tokens, segments between the first and the last: never negative, whatever the decay's sign.)
+  float2* seg_factors; // (N, H, nseg): what a segment multiplies the state with, and what its rounding left; {-1, 0}: it drops the state.  (Those
+                       // that are read are powers of 32 m tokens, of segments between the first and the last: never negative.)
   const float* decay;
   const void* resets;
   const void* lengths;
@@ -416,7 +416,9 @@ __device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, co
       for (int sv = 0; sv < NV; ++sv) *reinterpret_cast<f32x4*>(slot + ((s * NV + sv) * WAVE + lane) * 4) = S[s][sv];
     if (w.slice == 0 && lane == 0) {
       const int count = (w.end > w.begin ? w.end - w.begin : 0) - (a.reverse && w.seg == 0 && w.end > 0 ? 1 : 0);
-      a.seg_factors[w.nh * a.nseg + w.seg] = dropped ? -1.f : (float)da_power(decay, count);
+      const double factor = da_power(decay, count);
+      const float hi = (float)factor;
+      a.seg_factors[w.nh * a.nseg + w.seg] = dropped ? make_float2(-1.f, 0.f) : make_float2(hi, (float)(factor - (double)hi));
     }
     return;
   }
@@ -1220,7 +1222,7 @@ __global__ __launch_bounds__(256) void decay_attention_join_kernel(const DaRoles
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= quads) return;
   const DaCore& a = roles.c[blockIdx.y];
-  const float* factors = a.seg_factors;
+  const float2* factors = a.seg_factors;
   const int64_t nh = i / per_head, e = i % per_head;
   const int last = da_last_segment(a, da_length(a, nh / a.h));
   if (last == 0) return;
@@ -1229,7 +1231,7 @@ __global__ __launch_bounds__(256) void decay_attention_join_kernel(const DaRoles
   constexpr int U = 8;  // ends in flight (they do not depend on the carry, but lie where it goes)
   for (int seg0 = 1; seg0 <= last; seg0 += U) {
     f32x4 end[U];
-    float f[U];
+    float2 f[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int seg = seg0 + i < last ? seg0 + i : last - 1;  // (the last segment's own end is nobody's start)
@@ -1240,7 +1242,8 @@ __global__ __launch_bounds__(256) void decay_attention_join_kernel(const DaRoles
     for (int i = 0; i < U; ++i) {
       if (seg0 + i > last) break;
       s[(seg0 + i) * per_head] = carry;
-      carry = f[i] < 0.f ? end[i] : __builtin_elementwise_fma(carry, f32x4(f[i]), end[i]);
+      const f32x4 left = __builtin_elementwise_fma(carry, f32x4(f[i].y), end[i]);
+      carry = f[i].x < 0.f ? end[i] : __builtin_elementwise_fma(carry, f32x4(f[i].x), left);
     }
   }
 }
@@ -1436,7 +1439,7 @@ static int decay_attention_run(const DaRoles& in, const DaPlan& p, float* worksp
     c.seg_len = (int)p.seg_len;
     if (p.nseg > 1) {
       c.seg_states = workspace + i * p.seg_floats;
-      c.seg_factors = c.seg_states + heads * p.nseg * per_head * 4;
+      c.seg_factors = reinterpret_cast<float2*>(c.seg_states + heads * p.nseg * per_head * 4);
     }
   }
   void (*states)(DaRoles);

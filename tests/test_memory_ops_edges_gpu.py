@@ -109,3 +109,34 @@ def test_layer_norm_no_rows_and_the_gradient_of_x_alone(dtype):
     for args in ((), (w,), (None, b), (w, b)):
         dx, = torch.autograd.grad(layer_norm(x, *args), x, torch.zeros(0, 32, dtype=dtype, device=DEV))
         assert dx.shape == (0, 32) and dx.dtype == dtype
+
+
+# ------------------------------------------------------------------------------------------------ long memories
+def _drift(decay, tokens, times):
+    """Mean error, in 2^-24, of a state that is multiplied ``times`` times by decay^tokens as one 32-bit number."""
+    power = 1.0
+    for _ in range(tokens):
+        power *= float(decay)
+    return times * (float(torch.tensor(power, dtype=torch.float32)) - power) / power / U32
+
+
+@pytest.mark.parametrize("dtype, tokens, n, d, t, step", [
+    (torch.float32, 16, 1024, 4, 6400, 25), (torch.bfloat16, 32, 1024, 4, 12800, 53),                    # one wave from end to end
+    (torch.float32, 64, 1, 128, 12800, 17), (torch.bfloat16, 64, 1, 128, 12800, 17)])                    # 200 segments, joined
+def test_decay_attention_keeps_an_old_state_s_scale(dtype, tokens, n, d, t, step):
+    """An initial state of n d^2 = 16384 random values behind t empty tokens.  The decay is one whose power over a block (a segment) rounds by
+    nearly half a step: carried as one 32-bit number it shifts every value by the same 98 to 200 * 2^-24, as the first lines check.  What its
+    rounding leaves is carried along, so that only the products' own roundings are left, which have no mean: of 400 of them, uniform within
+    half a step of 2^-24 at most, over 16384 values six standard deviations are 6 * sqrt(400 / 16384 / 12) < 0.3; the carried remainder
+    and the last power's rounding add two."""
+    decay = torch.tensor(1 - 2.0 ** -14 * (1 + step / 64), dtype=torch.float32)
+    assert abs(_drift(decay, tokens, t // tokens)) > 97
+    empty = torch.zeros(1, 1, 1, d, dtype=dtype, device=DEV).expand(n, t, 1, d)
+    start = 0.5 + torch.rand(n, 1, d, d, generator=torch.Generator(device=DEV).manual_seed(70), device=DEV)
+    for reverse in (False, True):  # forward, and the gradient's way back
+        first = start.clone().requires_grad_(True)
+        o, last = decay_attention(empty, empty, empty, decay.view(1).to(DEV), first)
+        assert not o.any()
+        got = torch.autograd.grad(last, first, start)[0] if reverse else last.detach()
+        want = start.double().cpu() * float(decay) ** t
+        assert abs(float(((got.double().cpu() - want) / want).mean())) <= 3 * U32, reverse
