@@ -21,14 +21,13 @@
 //
 // Two kernels: v_mfma_f32_16x16x4_f32 on operands widened to fp32, which rounds nothing to fewer bits, and for bf16 tensors
 // v_mfma_f32_16x16x32_bf16 with the 32-bit factors split into bf16 numbers.  What bounds them:
-//   short sequences: HBM, for q, k, v, o and the states.  4096 environments x 4 heads x 16 tokens, 64 x 64, fp32: forward 170 us
-//     (805 MB, 4.7 TB/s; the copy rate is 5.4), backward 350 us (1.27 GB once, 3.6 TB/s).  Of the 28
-//     thousand cycles of a backward wave 17 pass until its first rows and its state are there; the three roles read them once from
-//     HBM and three times from the L2.
-//   long ones: the chain of a wave's blocks.  A bf16 block of 32 tokens with 64 x 64 of state is 100 matrix and 800 ordinary
-//     instructions and takes a wave 10.7 thousand cycles (state's part 3.4, state's update 2.2, rows through LDS 1.8, P V 1.0, loads
-//     and weights the rest): dependent instructions follow each other after 8 cycles, not 4, and two waves are all that a SIMD's
-//     registers hold.  2 sequences x 16 heads x 4096 tokens: forward 49 us (states 16, join 8, main 25), backward 90 (28, 11, 51).
+//   short sequences: HBM, for q, k, v, o and the states.  4096 environments x 4 heads x 16 tokens, 64 x 64, fp32: forward 175 us
+//     (805 MB, 4.6 TB/s; a large streaming copy reaches 6.4), backward 355 us (1.27 GB once, 3.6 TB/s): counted, every input comes from HBM
+//     once, and the three roles ask the L2 for 2.4 GB.  Of the 28 thousand cycles of a backward wave 17 pass until its first rows and its
+//     state are there.
+//   long ones: the chain of a wave's blocks.  A bf16 block of 32 tokens with 64 x 64 of state is 126 matrix and about 1050 vector
+//     instructions; two waves are all that a SIMD's registers hold, and take 7.7 us a block together (4096 heads x 512 tokens: 243 us).
+//     2 sequences x 16 heads x 4096 tokens: forward 53 us (states 16, join 9.5, main 27), backward 94 (27, 11.5, 55).
 #include "oige_elem.hpp"
 
 namespace oige {
@@ -1216,8 +1215,8 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
 
 // The states in front of every segment from those at the segments' ends (in place, register order): carry = factor carry + end.
 // Segment 0's end already holds the initial state.  A thread owns four floats of one (sequence, head) over all segments, eight of
-// them in flight.  It moves the states once each way (64 heads' 128 x 128 over 8 segments, 2 x 34 MB: 11 us; 32 heads' 64 x 64
-// over 32 segments, 2 x 17 MB: 8 us), mostly from and to the caches; 16 in flight are no faster.
+// them in flight.  It moves the states once each way (64 heads' 128 x 128 over 8 segments, 2 x 34 MB: 12 us; 32 heads' 64 x 64
+// over 32 segments, 2 x 17 MB: 9.5 us), mostly from and to the caches; 16 in flight are no faster.
 __global__ __launch_bounds__(256) void decay_attention_join_kernel(const DaRoles roles, int64_t quads, int64_t per_head, int nseg) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= quads) return;
@@ -1383,15 +1382,15 @@ struct DaPlan {
 };
 
 // Tiles per wave: 16 NK rows cover dk, 16 NV columns are a slice of dv; at most 16 tiles (64 registers) of state.  Wider slices share
-// q, k and their product among more columns (bf16, 64 x 64, 512 tokens of 4096 heads: 251 us with four tiles, 313 with two), narrower
+// q, k and their product among more columns (bf16, 64 x 64, 512 tokens of 4096 heads: 243 us with four tiles, 309 with two), narrower
 // ones leave fewer columns empty behind dv: the width with the least matrix instructions over all slices is taken.  Calls that
 // neither fill the chip nor have many tokens to a wave take narrower ones: the chain of one wave's blocks is what lasts (fp32,
 // 64 x 64, 128 tokens of 256 heads: 38 us with four tiles, 31 with two, 22 with one; with 2048 tokens four are the best).
 //
 // A call with fewer waves than the chip has SIMDs is cut over time, into pieces of 64 tokens at least: the pieces' end states first,
 // joined by one small launch, then every piece by itself.  Two launches more cost about 10 us: below 192 tokens (256 in bf16) the
-// call stays whole (64 heads of 64 x 64, bf16: 128 tokens 18 us cut and 14 whole, 384 tokens 24 cut and 30 whole; fp32: 128 tokens
-// 21 and 19, 192 tokens 23 and 27).  The aim is two waves per SIMD, and not one more, which would run alone behind the others.
+// call stays whole (64 heads of 64 x 64, bf16: 128 tokens 18 us cut and 14 whole, 256 tokens 21 cut and 24 whole; fp32: 128 tokens
+// 21 and 20, 192 tokens 23 and 28).  The aim is two waves per SIMD, and not one more, which would run alone behind the others.
 // Where lengths differ every sequence's own tokens are cut evenly (bf16 prompts between a quarter and all of 8192 tokens, 4 x 16 heads
 // of 128 x 128, mean of eight draws: 231 us; 252 with pieces of the same length in all, 247 with twice as many of them).
 constexpr int64_t DA_FEW_WAVES = 1024, DA_WANT_WAVES = 2048, DA_WIDE_TOKENS = 12288;
