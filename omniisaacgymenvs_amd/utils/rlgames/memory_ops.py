@@ -55,7 +55,12 @@ _pack_norm, _pack_attention, _pack_step = _packer(_lib.LayerNormIo), _packer(_li
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.data_ptr()
+    if t is None:
+        return 0
+    p = t.data_ptr()
+    if not p and t.numel():  # a wrapper or fake tensor would pass for an argument that was left out
+        raise _error(f"a {type(t).__name__} of shape {tuple(t.shape)} has no memory a kernel could read")
+    return p
 
 
 def _last_contiguous(t: torch.Tensor) -> torch.Tensor:

@@ -7,6 +7,7 @@ from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from omniisaacgymenvs_amd import _lib
+from omniisaacgymenvs_amd.utils.rlgames import memory_ops
 from omniisaacgymenvs_amd.utils.rlgames.memory_ops import decay_attention, decay_attention_step, layer_norm
 
 
@@ -124,3 +125,33 @@ def test_scale_and_eps_beyond_32_bits_are_refused(value):
     for fn, args in ((attention, seq), (step, one)):
         with pytest.raises(_lib.OigeError, match="scale"):
             fn(*args, scale=value)
+
+
+class _Wrapper(torch.Tensor):
+    """A tensor that holds its values elsewhere, as distributed tensors do."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+
+@pytest.mark.parametrize("which, name", [(0, "weight"), (0, "bias"), (1, "state"), (1, "resets"), (1, "lengths"), (2, "resets")])
+def test_tensors_without_memory_do_not_pass_for_arguments_left_out(which, name, monkeypatch):
+    """(The launch is replaced: nothing may get that far.)"""
+    def launched(*args):
+        raise AssertionError("launched")
+
+    monkeypatch.setattr(memory_ops, "_on_device", lambda *a: None)
+    monkeypatch.setattr(memory_ops, "_call", launched)
+    _, fn, args = _calls()[which]
+    given = dict(zip((("x", "weight", "bias"), ("q", "k", "v", "decay", "state"), ("q", "k", "v", "decay", "state"))[which], args))
+    given.update({"resets": torch.zeros(2, 5, dtype=torch.bool) if which == 1 else torch.zeros(2, dtype=torch.bool)} if name == "resets" else
+                 {"lengths": torch.zeros(2, dtype=torch.int64)} if name == "lengths" else {})
+    with pytest.raises(AssertionError, match="launched"):
+        fn(**given)
+    with pytest.raises(_lib.OigeError, match="no memory"):
+        fn(**{**given, name: _Wrapper(given[name])})
