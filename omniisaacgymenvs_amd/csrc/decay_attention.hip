@@ -417,7 +417,7 @@ __device__ __forceinline__ void da_close(f32x4 (&S)[NK][NV], const DaCore& a, co
       const int count = (w.end > w.begin ? w.end - w.begin : 0) - (a.reverse && w.seg == 0 && w.end > 0 ? 1 : 0);
       const double factor = da_power(decay, count);
       const float hi = (float)factor;
-      a.seg_factors[w.nh * a.nseg + w.seg] = dropped ? make_float2(-1.f, 0.f) : make_float2(hi, (float)(factor - (double)hi));
+      a.seg_factors[w.nh * a.nseg + w.seg] = dropped ? make_float2(-1.f, 0.f) : make_float2(hi, da_finite(hi) ? (float)(factor - (double)hi) : 0.f);
     }
     return;
   }
@@ -1027,11 +1027,11 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
         pt[1] = db_mfma(k[0], q[1], pt[1]);
         pt[2] = db_mfma(k[1], q[1], pt[2]);
       }
-        if (more) issue_k(next);
+      if (more) issue_k(next);
       else forget(k_run);
       const bool from_state[2] = {!(m & upto[0]), !(m & upto[1])};
       db_state_part<NK, NV>(acc, S, Q, from_state, head_w);
-        // a masked product may be infinite or NaN: selected away, not multiplied
+      // a masked product may be infinite or NaN: selected away, not multiplied
       const f32x4 w0 = weights[0], w1 = weights[WAVE];
       const float pair_w[4] = {w0.x, w0.y, w0.z, w0.w}, cross_w[4] = {w1.x, w1.y, w1.z, w1.w};
       float P[3][4] = {{pt[0].x, pt[0].y, pt[0].z, pt[0].w}, {pt[1].x, pt[1].y, pt[1].z, pt[1].w}, {pt[2].x, pt[2].y, pt[2].z, pt[2].w}};
@@ -1188,7 +1188,7 @@ __global__ __launch_bounds__(DA_WAVES* WAVE, 2) void decay_attention_bf16_kernel
     uint32_t kk[8];
 #pragma unroll
     for (int s = 0; s < NK; ++s) {
-        const int i = s / 2;
+      const int i = s / 2;
       if (!(s & 1)) {
         if constexpr (NK == 8 && !STATES) __builtin_amdgcn_sched_barrier(0);  // or all of k is read at once, into registers there are not
 #pragma unroll
@@ -1241,7 +1241,9 @@ __global__ __launch_bounds__(256) void decay_attention_join_kernel(const DaRoles
     for (int i = 0; i < U; ++i) {
       if (seg0 + i > last) break;
       s[(seg0 + i) * per_head] = carry;
-      const f32x4 left = __builtin_elementwise_fma(carry, f32x4(f[i].y), end[i]);
+      const f32x4 part = {da_finite(carry.x) ? carry.x : 0.f, da_finite(carry.y) ? carry.y : 0.f, da_finite(carry.z) ? carry.z : 0.f,
+                          da_finite(carry.w) ? carry.w : 0.f};  // (what is infinite stays so: no part of it of the other sign)
+      const f32x4 left = __builtin_elementwise_fma(part, f32x4(f[i].y), end[i]);
       carry = f[i].x < 0.f ? end[i] : __builtin_elementwise_fma(carry, f32x4(f[i].x), left);
     }
   }

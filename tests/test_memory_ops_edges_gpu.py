@@ -145,6 +145,15 @@ def test_decay_attention_keeps_an_old_state_s_scale(dtype, tokens, n, d, t, step
         assert abs(float(((got.double().cpu() - want) / want).mean())) <= 3 * U32, reverse
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decay_attention_states_that_outgrow_32_bits_become_infinite(dtype):
+    """A decay of 8 over 400 tokens: 2^1200.  Across segments as within them."""
+    empty, ones = torch.zeros(1, 400, 1, 8, dtype=dtype, device=DEV), torch.ones(1, 1, 8, 8, device=DEV)
+    for sign in (1, -1):
+        _, state = decay_attention(empty, empty, empty, torch.tensor([8.0], device=DEV), sign * ones)
+        assert (state == sign * float("inf")).all()
+
+
 # ------------------------------------------------------------------------------------------------ what lies around the results
 # Every result lies in a larger buffer of a pattern, with columns to spare between its rows where a call takes strides: the pattern has to
 # be there afterwards, bit for bit.
